@@ -443,6 +443,102 @@ int mmn_grad_reduce(const void *const *src, int nsrc, void *dst, int64_t numel, 
 int mmn_grad_nonfinite_scan(const void *grads, int64_t numel, int dtype, int *const *flags,
                             int nflags, int device, void *stream);
 
+/* ------------------------------------ operators that produce the grads */
+/*
+ * Layer norm and 4-bit linear products beside the step: their weights are the
+ * step's parameters (mmn_optim_slot_ptrs), their weight gradients go to its
+ * grad slots. Like mmn_grad_reduce they work on buffers the caller owns: every
+ * pointer is device memory of `device` aligned to its element (further
+ * alignment where stated), *_ld is the distance between rows in elements (at
+ * least the row; any value for a single row), work is enqueued on `stream`
+ * (NULL = legacy default stream) and the call returns without synchronising.
+ * Nothing is allocated, so the calls can be captured in a CUDA graph. An output
+ * either is one of the inputs where that is stated, or shares no element with
+ * any. A matrix without rows or columns is accepted and nothing of it is read.
+ */
+
+/* Layer norm over the last axis of x (rows x cols), the LayerNorm layer of
+ * crates/mmn-nn/src/lib.rs: y = (x - mean) / sqrt(var + eps) * gamma + beta with
+ * the biased variance. x and y are MMN_DTYPE_F32 or MMN_DTYPE_BF16 each, gamma
+ * and beta (cols) of param_dtype. mean and rstd (rows floats each, NULL to
+ * skip) receive the statistics the backward pass takes. Statistics are fp32, y
+ * is rounded once. y may be x (same pitch and dtype). */
+int mmn_layer_norm(const void *x, int64_t x_ld, int x_dtype, const void *gamma, const void *beta,
+                   int param_dtype, float eps, int64_t rows, int64_t cols, void *y, int64_t y_ld,
+                   int y_dtype, float *mean, float *rstd, int device, void *stream);
+
+/* Gradients of mmn_layer_norm: dx (rows x cols, x's dtype), and dgamma, dbeta
+ * (cols, grad_dtype), the sums over the rows; accumulate = 1 adds them to what
+ * the buffers hold (micro-batches, GradAccumulator of lib.rs:212-262). dy has
+ * dy_dtype; mean and rstd are those of the forward pass. dx may be dy or x
+ * (same pitch and dtype). The sums are fp32 in a fixed order: the result is the
+ * same in every run on one GPU. workspace is a 16-byte aligned buffer of the
+ * size that mmn_layer_norm_backward_workspace gives for rows, cols and device;
+ * calls that may overlap on the GPU need one each. Without rows, dgamma and
+ * dbeta become zero (accumulate: stay). */
+int mmn_layer_norm_backward_workspace(int64_t rows, int64_t cols, int device, int64_t *bytes);
+int mmn_layer_norm_backward(const void *dy, int64_t dy_ld, int dy_dtype, const void *x,
+                            int64_t x_ld, int x_dtype, const void *gamma, int param_dtype,
+                            const float *mean, const float *rstd, int64_t rows, int64_t cols,
+                            void *dx, int64_t dx_ld, void *dgamma, void *dbeta, int grad_dtype,
+                            int accumulate, void *workspace, int64_t workspace_bytes, int device,
+                            void *stream);
+
+/* A matrix in 4-bit microscaled floating point (OCP Microscaling v1.0 MXFP4).
+ * Each run of 32 columns of a row shares a scale 2^(s - 127), s one byte;
+ * elements are e2m1 (0, 1/2, 1, 3/2, 2, 3, 4, 6 with a sign). 17 bytes for 32
+ * values, against 64 in bf16.
+ *   codes  rows x ceil(cols / 32) * 16 bytes, row-major, the even column in the
+ *          low half of a byte, the last block of a row filled up with zeros;
+ *   scales ceil(rows / 128) x 2 * ceil(cols / 256) blocks of 512 bytes, the scale
+ *          of row r, columns 32k .. 32k + 31 in block (r / 128, k / 4) at byte
+ *          (r % 32) * 16 + (r / 32 % 4) * 4 + k % 4; unused bytes along a row's
+ *          last blocks are zero.
+ * Both buffers are 16-byte aligned device memory of the size mmn_mxfp4_size
+ * gives. rows and cols are at most 2^30. */
+typedef struct {
+    void *codes;
+    void *scales;
+    int64_t rows;
+    int64_t cols;
+} mmn_mxfp4;
+
+int mmn_mxfp4_size(int64_t rows, int64_t cols, int64_t *code_bytes, int64_t *scale_bytes);
+
+/* x (rows x cols, fp32 or bf16) to 4 bits: q (rows x cols) holds x, qt (cols x
+ * rows) its transpose, whose blocks run down x's columns; either may be NULL, x
+ * is read once for both. The scale of a block is 2^(floor(log2 max|x|) - 2), its
+ * elements round to nearest, ties to even, magnitudes above 6 scales to 6. A
+ * block with an Inf or NaN becomes NaN as a whole (scale byte 255). */
+int mmn_mxfp4_quantize(const void *x, int64_t x_ld, int dtype, int64_t rows, int64_t cols,
+                       const mmn_mxfp4 *q, const mmn_mxfp4 *qt, int device, void *stream);
+
+/* The values q stands for, as fp32 or bf16 (both hold every one exactly). */
+int mmn_mxfp4_dequantize(const mmn_mxfp4 *q, void *out, int64_t out_ld, int dtype, int device,
+                         void *stream);
+
+/* out (a.rows x b.rows, fp32 or bf16) = A B^T, summed over the cols of both in
+ * fp32 on the tensor cores and rounded once; accumulate = 1 adds it to what out
+ * holds first. With W of a Linear layer ([out, in], crates/mmn-nn/src/lib.rs:305-307):
+ * y = x W^T from (x, W); dx = dy W from (dy, W transposed); dW = dy^T x from (dy
+ * transposed, x transposed), for example into a grad slot. A NaN block makes
+ * the rows (columns) of out that sum over it NaN. */
+int mmn_mxfp4_matmul(const mmn_mxfp4 *a, const mmn_mxfp4 *b, void *out, int64_t out_ld, int dtype,
+                     int accumulate, int device, void *stream);
+
+/* The forward pass of a Linear layer in one call: x (rows x w.cols, fp32 or
+ * bf16) is rounded to 4 bits and multiplied: out (rows x w.rows) = q(x) W^T. xq
+ * (rows x w.cols) gives room for the rounded x; its contents afterwards are
+ * unspecified. */
+int mmn_mxfp4_linear(const void *x, int64_t x_ld, int x_dtype, int64_t rows, const mmn_mxfp4 *w,
+                     const mmn_mxfp4 *xq, void *out, int64_t out_ld, int out_dtype, int device,
+                     void *stream);
+
+/* Waits for `stream` and reports MMN_E_TIMEOUT when a kernel of
+ * mmn_mxfp4_matmul or mmn_mxfp4_linear on `device` gave up a bounded wait since
+ * the last report (mmn_optim_sync does this for a handle's kernels). */
+int mmn_kernel_status(int device, void *stream);
+
 /* Parameter counts: total registered, stepped by AdamW, stepped by Muon. */
 int mmn_optim_param_counts(mmn_optim_t *h, int64_t *total, int64_t *adamw, int64_t *muon);
 

@@ -70,7 +70,13 @@ class GatherLayoutC(ctypes.Structure):
                 ("muon_param_bf16", ctypes.c_void_p), ("muon_region", ctypes.c_int64)]
 
 
+class Mxfp4C(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int64)]
+
+
 _vp = ctypes.c_void_p
+_mxp = ctypes.POINTER(Mxfp4C)
 _i = ctypes.c_int
 _u64 = ctypes.c_uint64
 _i64 = ctypes.c_int64
@@ -139,6 +145,17 @@ SIGNATURES = {
     "mmn_optim_scan_grads": (_i, [_vp, _vp]),
     "mmn_grad_reduce": (_i, [ctypes.POINTER(_vp), _i, _vp, _i64, _i, _vp, _i, _vp]),
     "mmn_grad_nonfinite_scan": (_i, [_vp, _i64, _i, ctypes.POINTER(_vp), _i, _i, _vp]),
+    "mmn_layer_norm": (_i, [_vp, _i64, _i, _vp, _vp, _i, _f, _i64, _i64, _vp, _i64, _i, _vp, _vp,
+                            _i, _vp]),
+    "mmn_layer_norm_backward_workspace": (_i, [_i64, _i64, _i, _i64p]),
+    "mmn_layer_norm_backward": (_i, [_vp, _i64, _i, _vp, _i64, _i, _vp, _i, _vp, _vp, _i64, _i64,
+                                     _vp, _i64, _vp, _vp, _i, _i, _vp, _i64, _i, _vp]),
+    "mmn_mxfp4_size": (_i, [_i64, _i64, _i64p, _i64p]),
+    "mmn_mxfp4_quantize": (_i, [_vp, _i64, _i, _i64, _i64, _mxp, _mxp, _i, _vp]),
+    "mmn_mxfp4_dequantize": (_i, [_mxp, _vp, _i64, _i, _i, _vp]),
+    "mmn_mxfp4_matmul": (_i, [_mxp, _mxp, _vp, _i64, _i, _i, _i, _vp]),
+    "mmn_mxfp4_linear": (_i, [_vp, _i64, _i, _i64, _mxp, _mxp, _vp, _i64, _i, _i, _vp]),
+    "mmn_kernel_status": (_i, [_i, _vp]),
     "mmn_optim_plan": (_i, [_i64p, ctypes.POINTER(_i), ctypes.POINTER(_i), _i, _i, _i, _i,
                             ctypes.POINTER(_i), _i64p, _i64p, _i64p]),
     "mmn_optim_ns_flops": (_i, [_vp, ctypes.POINTER(ctypes.c_double)]),

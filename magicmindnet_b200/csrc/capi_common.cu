@@ -158,6 +158,29 @@ int check_device_ptr(const void* p, int device, const char* what) {
   return MMN_OK;
 }
 
+int check_device_elems(const void* p, size_t esize, int device, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) % esize)
+    return fail(MMN_E_INVALID, std::string(what) + ": not aligned to its element size");
+  return check_device_ptr(p, device, what);
+}
+
+// The device checks of the caller-buffer entry points: a usable sm_100 GPU.
+int percall_device(int device, int* sms) {
+  int count = 0;
+  if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
+    cudaGetLastError();
+    return fail(MMN_E_NO_DEVICE, "GPU missing, but CUDA was requested.");
+  }
+  if (device < 0 || device >= count) return fail(MMN_E_INVALID, "device ordinal out of range");
+  int major = 0, minor = 0;
+  MMN_CUDA_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+  MMN_CUDA_TRY(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
+  MMN_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+  if (major != 10 || minor != 0)
+    return fail(MMN_E_NO_DEVICE, "this library is built for sm_100a (B200) devices only");
+  return MMN_OK;
+}
+
 }  // namespace mmn
 
 extern "C" {

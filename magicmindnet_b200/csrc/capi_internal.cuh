@@ -77,6 +77,26 @@ int64_t shape_numel(const int64_t* shape, int ndim, int* err);
 // another GPU is refused: kernels here never read a peer's memory.
 int check_device_ptr(const void* p, int device, const char* what);
 
+// check_device_ptr, and `p` is aligned to its elements of `esize` bytes.
+int check_device_elems(const void* p, size_t esize, int device, const char* what);
+
+// The device checks of the caller-buffer entry points: a usable sm_100 GPU,
+// whose SM count goes to *sms.
+int percall_device(int device, int* sms);
+
+// An output matrix (rows x cols, row pitch in elements) may be one input (same
+// place, pitch and element size) or share no element with it; column slices
+// of one buffer share none. Else MMN_E_INVALID naming `what`.
+int check_out_overlap(const void* out, int64_t out_ld, size_t out_esz, const char* what,
+                      const void* in, int64_t in_ld, size_t in_esz, int64_t rows, int64_t cols);
+
+// Rows of a matrix (pitch ld, esz-byte elements) can be read v elements at a
+// time: base and pitch are multiples of that access, 16 bytes at most.
+inline bool vec_rows(const void* p, int64_t ld, size_t esz, int v) {
+  const size_t w = (size_t)v * esz < 16 ? (size_t)v * esz : 16;
+  return reinterpret_cast<uintptr_t>(p) % w == 0 && ((uintptr_t)ld * esz) % w == 0;
+}
+
 // fp32 -> tf32 value (10 leading mantissa bits), to nearest with ties to even
 // on the 13 discarded bits; Inf and NaN pass through. The host form of the
 // TF32 mode's rounding point.

@@ -695,23 +695,6 @@ int check_reachable(const void* p, int device, const std::string& what) {
   return MMN_OK;
 }
 
-// The device checks of the caller-buffer entry points: a usable sm_100 GPU.
-int percall_device(int device, int* sms) {
-  int count = 0;
-  if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
-    cudaGetLastError();
-    return fail(MMN_E_NO_DEVICE, "GPU missing, but CUDA was requested.");
-  }
-  if (device < 0 || device >= count) return fail(MMN_E_INVALID, "device ordinal out of range");
-  int major = 0, minor = 0;
-  MMN_CUDA_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
-  MMN_CUDA_TRY(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
-  MMN_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
-  if (major != 10 || minor != 0)
-    return fail(MMN_E_NO_DEVICE, "this library is built for sm_100a (B200) devices only");
-  return MMN_OK;
-}
-
 }  // namespace
 
 extern "C" int mmn_grad_reduce(const void* const* src, int nsrc, void* dst, int64_t numel,

@@ -267,6 +267,27 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
       : "memory");
 }
 
+// D[tmem] (+)= (A * SA) * (B * SB) (kind::mxf4): e2m1 operands packed two to a
+// byte in shared memory, one ue8m0 scale per 32 elements of K held in TMEM, fp32
+// accumulate; K = 64 per instruction.
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t sfa_tmem, uint32_t sfb_tmem,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], "
+      "p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate));
+}
+
+// One 512-byte block of scales (32 rows x 16 bytes) from shared memory to four
+// TMEM columns, repeated in the four lane quarters.
+__device__ __forceinline__ void tc_cp_scales(uint32_t taddr, uint64_t s_desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc)
+               : "memory");
+}
+
 // 32 lanes x 32 columns of fp32 from TMEM: thread t of the warp gets lane
 // (base lane + t), columns col .. col+31.
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, float (&v)[32]) {
@@ -346,6 +367,48 @@ __host__ __device__ constexpr uint32_t umma_idesc_tf32(int M, int N, bool a_mn_m
          | ((b_mn_major ? 1u : 0u) << 16)
          | ((uint32_t)(N >> 3) << 17)
          | ((uint32_t)(M >> 4) << 24);
+}
+
+// Shared-memory descriptor of a 512-byte block of scales: no swizzle, four
+// groups of 8 rows x 16 bytes, 128 bytes apart (SBO).
+__device__ __forceinline__ uint64_t umma_desc_scales(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)1u << 16;              // LBO: one group per row of groups, not used
+  d |= (uint64_t)(128u >> 4) << 32;     // SBO
+  d |= (uint64_t)1u << 46;              // descriptor version for tcgen05
+  return d;
+}
+
+// Instruction descriptor, kind::mxf4: e2m1 x e2m1 with ue8m0 scales, M x N tile,
+// both operands K-major. `half` (0 or 1) is the pair of scale bytes of the TMEM
+// columns that this MMA's 64 elements use.
+__host__ __device__ constexpr uint32_t umma_idesc_mxf4(int M, int N, int half) {
+  return ((uint32_t)(half * 2) << 4)     // B scale id
+         | (1u << 7)                     // A format: e2m1
+         | (1u << 10)                    // B format: e2m1
+         | ((uint32_t)(N >> 3) << 17)    // N / 8
+         | (1u << 23)                    // scale format: ue8m0
+         | ((uint32_t)(M >> 4) << 24)    // M / 16
+         | ((uint32_t)(half * 2) << 29);  // A scale id
+}
+
+// Untiled bulk copy global -> this CTA's shared memory; both addresses 16-byte
+// aligned, bytes a multiple of 16. No multicast.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(smem_u32(smem_dst)),
+      "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// 32-bit load from a shared::cluster address.
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
 }  // namespace mmn

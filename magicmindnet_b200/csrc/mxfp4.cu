@@ -1,0 +1,652 @@
+// 4-bit microscaled matrices (OCP Microscaling v1.0, MXFP4): quantisation along
+// the rows, the columns or both in one pass, the way back, and the products.
+//
+// A block is 32 consecutive elements of a row. With e = floor(log2 max |x|) over
+// the block, its scale is 2^(e - 2) (held as the byte e - 2 + 127, clamped at
+// 0), its elements x / scale rounded to the nearest of 0, 1/2, 1, 3/2, 2, 3, 4,
+// 6 with ties to the even code, values above 6 becoming 6. The division is by a
+// power of two, so it is exact where the result matters and the one rounding is
+// the conversion's. A block that holds an Inf or a NaN has the scale byte 255,
+// which the format reads as NaN for every element: a non-finite gradient stays
+// visible to the step's non-finite scan behind the product.
+//
+// Layout of a matrix of R rows and K columns: elements row-major, two to a byte
+// (the even column in the low half), rows padded with zeros to a multiple of 32;
+// scales in blocks of 128 rows x 128 columns, 512 bytes each, byte (r % 32) * 16 +
+// (r / 32 % 4) * 4 + (k / 32 % 4), the blocks of one 128-row tile one after the
+// other and padded to an even number with zero bytes. That is the form that
+// tcgen05 wants its scales in (mxfp4_gemm.cuh).
+#include "mxfp4_gemm.cuh"
+
+#include <mutex>
+
+#include "capi_internal.cuh"
+#include "ns_engine.cuh"
+
+namespace mmn {
+namespace {
+
+// -------------------------------------------------------------- conversions
+// Four e2m1 bytes from eight fp32 values (v[0] in the lowest four bits), to
+// nearest even, saturating.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// The value of a 4-bit code.
+__device__ __forceinline__ float e2m1_value(uint32_t c) {
+  const uint32_t e = (c >> 1) & 3u, m = c & 1u;
+  const float a = e ? (float)((2u + m) << e) * 0.25f : (float)m * 0.5f;
+  return (c & 8u) ? -a : a;
+}
+
+// Scale byte of a block from the bits of its largest magnitude as fp32 (taken
+// as an integer maximum, so that a NaN is not lost in it).
+__device__ __forceinline__ uint32_t mx_scale(uint32_t amax_bits) {
+  const uint32_t e = amax_bits >> 23;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+
+// 1 / scale (2^(127 - byte)); for a block without values any finite number.
+__device__ __forceinline__ float mx_inv_scale(uint32_t s) {
+  return s == 255u ? 1.0f : __uint_as_float((254u - s) << 23);
+}
+
+__device__ __forceinline__ float mx_scale_value(uint32_t s) {
+  if (s == 255u) return __uint_as_float(0x7FFFFFFFu);
+  return s ? __uint_as_float(s << 23) : __uint_as_float(0x00400000u);
+}
+
+// ------------------------------------------------------------- quantisation
+struct MxQuantArgs {
+  const void* x;
+  int64_t ld;
+  int rows, cols;
+  uint8_t *codes, *scales;      // of x, or null
+  uint8_t *codes_t, *scales_t;  // of x transposed, or null
+  int64_t pitch, pitch_t;       // bytes of one row of codes
+  int ka, ka_t;                 // scale blocks of one 128-row tile
+  int nct;                      // column tiles of the grid
+  int vec;                      // rows of x are 16-byte aligned
+};
+
+template <typename T>
+struct MxTile {
+  static constexpr int kPitch = 128 * sizeof(T) + 16;  // bytes; the skew spreads a column over banks
+  static constexpr int kCodePitch = 80;
+  static constexpr int kSmem = 128 * kPitch + 128 * kCodePitch + 1024;
+};
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)),
+               "l"(__cvta_generic_to_global(src)), "r"(bytes)
+               : "memory");
+}
+
+// One 128 x 128 tile per block: it goes to shared memory once; eight threads'
+// chunks of a row make the blocks of x, and thread columns of 32 rows the
+// blocks of x transposed, whose bytes are collected in shared memory so that
+// global memory sees 64 consecutive bytes per row of codes. A tile gives exactly
+// one 512-byte block of scales in each direction.
+template <typename T>
+__global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
+  constexpr int kPitch = MxTile<T>::kPitch;
+  constexpr bool kBf16 = sizeof(T) == 2;
+  extern __shared__ __align__(16) uint8_t sm[];
+  uint8_t* codes_s = sm + 128 * kPitch;
+  uint8_t* sf_row = codes_s + 128 * MxTile<T>::kCodePitch;
+  uint8_t* sf_col = sf_row + 512;
+  const int tid = threadIdx.x;
+  const int ct = blockIdx.x % a.nct, rt = blockIdx.x / a.nct;
+  const int c0 = ct * 128, r0 = rt * 128;
+  const bool in_c = c0 < a.cols, in_r = r0 < a.rows;
+  if (!in_c || !in_r) {
+    // padding of the scales to an even number of blocks
+    if (tid < 32) {
+      const uint4 z = make_uint4(0, 0, 0, 0);
+      if (in_r && a.scales)
+        reinterpret_cast<uint4*>(a.scales + ((int64_t)rt * a.ka + ct) * 512)[tid] = z;
+      if (in_c && a.scales_t)
+        reinterpret_cast<uint4*>(a.scales_t + ((int64_t)ct * a.ka_t + rt) * 512)[tid] = z;
+    }
+    return;
+  }
+  const T* x = static_cast<const T*>(a.x);
+  const int nr = min(128, a.rows - r0), nc = min(128, a.cols - c0);
+  if (a.vec) {
+    constexpr int kPer = 16 / sizeof(T), kCh = 128 / kPer;
+#pragma unroll
+    for (int i = 0; i < 128 * kCh / 256; ++i) {
+      const int id = i * 256 + tid, r = id / kCh, c = (id % kCh) * kPer;
+      const int bytes = r < nr ? max(0, min(kPer, nc - c)) * (int)sizeof(T) : 0;
+      const T* src = bytes ? x + (int64_t)(r0 + r) * a.ld + c0 + c : x;
+      cp_async16(sm + r * kPitch + c * sizeof(T), src, bytes);
+    }
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+  } else {
+    for (int id = tid; id < 128 * 128; id += 256) {
+      const int r = id >> 7, c = id & 127;
+      T v = T(0.0f);
+      if (r < nr && c < nc) v = x[(int64_t)(r0 + r) * a.ld + c0 + c];
+      *reinterpret_cast<T*>(sm + r * kPitch + c * sizeof(T)) = v;
+    }
+  }
+  __syncthreads();
+
+  if (a.codes) {
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+      const int id = i * 256 + tid, r = id >> 4, ch = id & 15;
+      float v[8];
+      uint32_t m;
+      if constexpr (kBf16) {
+        const uint4 u = *reinterpret_cast<const uint4*>(sm + r * kPitch + ch * 16);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        uint32_t mm = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          mm = __vmaxu2(mm, w[k] & 0x7FFF7FFFu);
+          v[2 * k] = __uint_as_float(w[k] << 16);
+          v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+        }
+        m = max(mm & 0xFFFFu, mm >> 16) << 16;
+      } else {
+        const float4 u0 = *reinterpret_cast<const float4*>(sm + r * kPitch + ch * 32);
+        const float4 u1 = *reinterpret_cast<const float4*>(sm + r * kPitch + ch * 32 + 16);
+        v[0] = u0.x, v[1] = u0.y, v[2] = u0.z, v[3] = u0.w;
+        v[4] = u1.x, v[5] = u1.y, v[6] = u1.z, v[7] = u1.w;
+        m = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+      }
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const uint32_t s = mx_scale(m);
+      const float inv = mx_inv_scale(s);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] *= inv;
+      const int64_t off = (int64_t)ct * 64 + ch * 4;
+      if (r < nr && off < a.pitch)
+        *reinterpret_cast<uint32_t*>(a.codes + (int64_t)(r0 + r) * a.pitch + off) = e2m1x8(v);
+      if ((ch & 3) == 0) sf_row[(r & 31) * 16 + (r >> 5) * 4 + (ch >> 2)] = (uint8_t)s;
+    }
+  }
+  if (a.codes_t) {
+    if constexpr (kBf16) {
+      const int cp = tid & 63, rb = tid >> 6;
+      uint32_t w[32], mm = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        w[i] = *reinterpret_cast<const uint32_t*>(sm + (rb * 32 + i) * kPitch + cp * 4);
+        mm = __vmaxu2(mm, w[i] & 0x7FFF7FFFu);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int c = cp * 2 + half;
+        const uint32_t s = mx_scale(half ? mm & 0xFFFF0000u : mm << 16);
+        const float inv = mx_inv_scale(s);
+        uint32_t o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            v[k] = __uint_as_float(half ? w[q * 8 + k] & 0xFFFF0000u : w[q * 8 + k] << 16) * inv;
+          o[q] = e2m1x8(v);
+        }
+        *reinterpret_cast<uint4*>(codes_s + c * MxTile<T>::kCodePitch + rb * 16) =
+            make_uint4(o[0], o[1], o[2], o[3]);
+        sf_col[(c & 31) * 16 + (c >> 5) * 4 + rb] = (uint8_t)s;
+      }
+    } else {
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const int c = tid & 127, rb = (tid >> 7) + 2 * h;
+        float w[32];
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          w[i] = *reinterpret_cast<const float*>(sm + (rb * 32 + i) * kPitch + c * 4);
+          m = max(m, __float_as_uint(w[i]) & 0x7FFFFFFFu);
+        }
+        const uint32_t s = mx_scale(m);
+        const float inv = mx_inv_scale(s);
+        uint32_t o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = w[q * 8 + k] * inv;
+          o[q] = e2m1x8(v);
+        }
+        *reinterpret_cast<uint4*>(codes_s + c * MxTile<T>::kCodePitch + rb * 16) =
+            make_uint4(o[0], o[1], o[2], o[3]);
+        sf_col[(c & 31) * 16 + (c >> 5) * 4 + rb] = (uint8_t)s;
+      }
+    }
+  }
+  __syncthreads();
+  if (a.codes_t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int id = i * 256 + tid, c = id >> 2, seg = id & 3;
+      const int64_t off = (int64_t)rt * 64 + seg * 16;
+      if (c < nc && off < a.pitch_t)
+        *reinterpret_cast<uint4*>(a.codes_t + (int64_t)(c0 + c) * a.pitch_t + off) =
+            *reinterpret_cast<const uint4*>(codes_s + c * MxTile<T>::kCodePitch + seg * 16);
+    }
+    if (tid >= 32 && tid < 64)
+      reinterpret_cast<uint4*>(a.scales_t + ((int64_t)ct * a.ka_t + rt) * 512)[tid - 32] =
+          reinterpret_cast<const uint4*>(sf_col)[tid - 32];
+  }
+  if (a.codes && tid < 32)
+    reinterpret_cast<uint4*>(a.scales + ((int64_t)rt * a.ka + ct) * 512)[tid] =
+        reinterpret_cast<const uint4*>(sf_row)[tid];
+}
+
+// ----------------------------------------------------------- the way back
+struct MxDequantArgs {
+  const uint8_t *codes, *scales;
+  void* out;
+  int64_t ld, pitch;
+  int64_t rows, cols, chunks;  // chunks of 8 columns per row
+  int ka;
+  int vec;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) mx_dequantize_kernel(const MxDequantArgs a) {
+  const int64_t n = a.rows * a.chunks;
+  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < n;
+       id += (int64_t)gridDim.x * 256) {
+    const int64_t r = id / a.chunks, c = (id - r * a.chunks) * 8;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(a.codes + r * a.pitch + c / 2);
+    const uint32_t s = a.scales[((r >> 7) * a.ka + (c >> 7)) * 512 + (r & 31) * 16 +
+                                ((r >> 5) & 3) * 4 + ((c >> 5) & 3)];
+    const float f = mx_scale_value(s);
+    T* o = static_cast<T*>(a.out) + r * a.ld + c;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = e2m1_value(w >> (4 * k)) * f;
+    if (a.vec && c + 8 <= a.cols) {
+      if constexpr (sizeof(T) == 2) {
+        uint4 u;
+        __nv_bfloat162* u2 = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u2[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+        *reinterpret_cast<uint4*>(o) = u;
+      } else {
+        reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c + k < a.cols) {
+          if constexpr (sizeof(T) == 2)
+            o[k] = __float2bfloat16_rn(v[k]);
+          else
+            o[k] = v[k];
+        }
+    }
+  }
+}
+
+// An empty sum: zeros, unless they are to be added.
+__global__ void __launch_bounds__(256) mx_zero_kernel(void* out, int64_t ld, int64_t rows,
+                                                      int64_t cols, int bf16) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * cols;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / cols, o = r * ld + (i - r * cols);
+    if (bf16)
+      static_cast<__nv_bfloat16*>(out)[o] = __float2bfloat16_rn(0.0f);
+    else
+      static_cast<float*>(out)[o] = 0.0f;
+  }
+}
+
+// A kernel of this file that gave up a bounded wait leaves its code here, per
+// device (mmn_kernel_status).
+__device__ int g_mx_status;
+
+// -------------------------------------------------------------------- host
+constexpr int64_t kMaxDim = int64_t(1) << 30;
+
+int64_t code_pitch(int64_t cols) { return (cols + 31) / 32 * 16; }
+int64_t scale_blocks(int64_t cols) { return (cols + 255) / 256 * 2; }
+int64_t code_bytes(int64_t rows, int64_t cols) { return rows * code_pitch(cols); }
+int64_t scale_bytes(int64_t rows, int64_t cols) {
+  return (rows + 127) / 128 * scale_blocks(cols) * 512;
+}
+
+bool bad_dtype(int d) { return d != MMN_DTYPE_F32 && d != MMN_DTYPE_BF16; }
+size_t esize(int d) { return d == MMN_DTYPE_BF16 ? 2 : 4; }
+
+int check_dims(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 0) return fail(MMN_E_INVALID, "negative dimension");
+  if (rows > kMaxDim || cols > kMaxDim)
+    return fail(MMN_E_SHAPE, "rows and cols must not exceed 2^30");
+  return MMN_OK;
+}
+
+// Pointers of a 4-bit matrix before any device is touched.
+int check_mx(const mmn_mxfp4* q, const char* what) {
+  int rc = check_dims(q->rows, q->cols);
+  if (rc != MMN_OK) return rc;
+  if (q->rows == 0 || q->cols == 0) return MMN_OK;
+  if (!q->codes || !q->scales)
+    return fail(MMN_E_INVALID, std::string(what) + ": null codes or scales");
+  if (reinterpret_cast<uintptr_t>(q->codes) % 16 || reinterpret_cast<uintptr_t>(q->scales) % 16)
+    return fail(MMN_E_INVALID, std::string(what) + ": codes or scales are not 16-byte aligned");
+  return MMN_OK;
+}
+
+int check_mx_device(const mmn_mxfp4* q, int device, const char* what) {
+  if (q->rows == 0 || q->cols == 0) return MMN_OK;
+  int rc = check_device_ptr(q->codes, device, what);
+  return rc != MMN_OK ? rc : check_device_ptr(q->scales, device, what);
+}
+
+struct Range {
+  const void* p;
+  int64_t bytes;
+};
+
+bool ranges_meet(const Range& a, const Range& b) {
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.p), b0 = reinterpret_cast<uintptr_t>(b.p);
+  return a.bytes > 0 && b.bytes > 0 && a0 < b0 + (uintptr_t)b.bytes && b0 < a0 + (uintptr_t)a.bytes;
+}
+
+Range matrix_range(const void* p, int64_t ld, int64_t rows, int64_t cols, size_t esz) {
+  return {p, rows && cols ? ((rows - 1) * ld + cols) * (int64_t)esz : 0};
+}
+Range codes_range(const mmn_mxfp4* q) { return {q->codes, code_bytes(q->rows, q->cols)}; }
+Range scales_range(const mmn_mxfp4* q) {
+  return {q->scales, q->cols ? scale_bytes(q->rows, q->cols) : 0};
+}
+
+// Shared memory of the kernels above 48 KB, once per device.
+int kernel_setup(int device) {
+  static std::mutex mu;
+  static uint64_t done = 0;
+  std::lock_guard<std::mutex> lock(mu);
+  if (device < 64 && (done >> device) & 1u) return MMN_OK;
+  const auto smem = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_quantize_kernel<float>, smem, MxTile<float>::kSmem));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<16, true>, smem, MxShape<16>::kSmemBytes));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<32, true>, smem, MxShape<32>::kSmemBytes));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<64, true>, smem, MxShape<64>::kSmemBytes));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<128, true>, smem, MxShape<128>::kSmemBytes));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<128, false>, smem, MxShape<128>::kSmemBytes));
+  if (device < 64) done |= uint64_t(1) << device;
+  return MMN_OK;
+}
+
+int launch_quantize(const void* x, int64_t ld, int dtype, int64_t rows, int64_t cols,
+                    const mmn_mxfp4* q, const mmn_mxfp4* qt, cudaStream_t s) {
+  MxQuantArgs a{};
+  a.x = x;
+  a.ld = ld;
+  a.rows = (int)rows;
+  a.cols = (int)cols;
+  if (q) {
+    a.codes = static_cast<uint8_t*>(q->codes);
+    a.scales = static_cast<uint8_t*>(q->scales);
+  }
+  if (qt) {
+    a.codes_t = static_cast<uint8_t*>(qt->codes);
+    a.scales_t = static_cast<uint8_t*>(qt->scales);
+  }
+  a.pitch = code_pitch(cols);
+  a.pitch_t = code_pitch(rows);
+  a.ka = (int)scale_blocks(cols);
+  a.ka_t = (int)scale_blocks(rows);
+  a.nct = q ? a.ka : (int)((cols + 127) / 128);
+  const int64_t nrt = qt ? a.ka_t : (rows + 127) / 128;
+  a.vec = vec_rows(x, ld, esize(dtype), 16);
+  const int64_t blocks = nrt * a.nct;
+  if (blocks > (int64_t(1) << 31) - 1) return fail(MMN_E_SHAPE, "matrix too large");
+  if (dtype == MMN_DTYPE_BF16)
+    mx_quantize_kernel<__nv_bfloat16>
+        <<<(unsigned)blocks, 256, MxTile<__nv_bfloat16>::kSmem, s>>>(a);
+  else
+    mx_quantize_kernel<float><<<(unsigned)blocks, 256, MxTile<float>::kSmem, s>>>(a);
+  MMN_CUDA_TRY(cudaGetLastError());
+  return MMN_OK;
+}
+
+int status_word(int** p) {
+  MMN_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(p), g_mx_status));
+  return MMN_OK;
+}
+
+template <int BN, bool TRANS>
+int launch_gemm(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, cudaStream_t s) {
+  CUtensorMap ta, tb;
+  std::string err = encode_byte_rows(&ta, a->codes, code_pitch(a->cols), a->rows, 128);
+  if (err.empty()) err = encode_byte_rows(&tb, b->codes, code_pitch(b->cols), b->rows, BN);
+  if (!err.empty()) return fail(MMN_E_CUDA, err);
+  g.sfa = static_cast<const uint8_t*>(a->scales);
+  g.sfb = static_cast<const uint8_t*>(b->scales);
+  g.ka = (int)scale_blocks(a->cols);
+  g.M = (int)a->rows;
+  g.N = (int)b->rows;
+  g.num_kb = (int)((a->cols + 255) / 256);
+  g.rt_b = (int)((b->rows + 127) / 128);
+  g.tiles_n = (int)((b->rows + BN - 1) / BN);
+  const int64_t tiles = (int64_t)((a->rows + 127) / 128) * g.tiles_n;
+  if (tiles > (int64_t(1) << 31) - 1) return fail(MMN_E_SHAPE, "product too large");
+  mx_gemm_kernel<BN, TRANS><<<(unsigned)tiles, 192, MxShape<BN>::kSmemBytes, s>>>(ta, tb, g);
+  MMN_CUDA_TRY(cudaGetLastError());
+  return MMN_OK;
+}
+
+// out (a.rows x b.rows) = A B^T, on checked arguments.
+int product(const mmn_mxfp4* a, const mmn_mxfp4* b, void* out, int64_t ld, int dtype,
+            int accumulate, cudaStream_t s) {
+  if (a->rows == 0 || b->rows == 0) return MMN_OK;
+  if (a->cols == 0) {
+    if (accumulate) return MMN_OK;
+    mx_zero_kernel<<<256, 256, 0, s>>>(out, ld, a->rows, b->rows, dtype == MMN_DTYPE_BF16);
+    MMN_CUDA_TRY(cudaGetLastError());
+    return MMN_OK;
+  }
+  MxGemmArgs g{};
+  g.out = out;
+  g.ld = ld;
+  g.out_bf16 = dtype == MMN_DTYPE_BF16;
+  g.accumulate = accumulate != 0;
+  g.vec = vec_rows(out, ld, esize(dtype), 8);
+  int rc = status_word(&g.status);
+  if (rc != MMN_OK) return rc;
+  // Few rows: the other operand's rows fill the 128 lanes.
+  if (a->rows <= 16) return launch_gemm<16, true>(b, a, g, s);
+  if (a->rows <= 32) return launch_gemm<32, true>(b, a, g, s);
+  if (a->rows <= 64) return launch_gemm<64, true>(b, a, g, s);
+  if (a->rows <= 128) return launch_gemm<128, true>(b, a, g, s);
+  return launch_gemm<128, false>(a, b, g, s);
+}
+
+int check_out(const void* out, int64_t ld, int dtype, int64_t rows, int64_t cols,
+              const Range* in, int n) {
+  if (rows == 0 || cols == 0) return MMN_OK;
+  if (!out) return fail(MMN_E_INVALID, "null output");
+  if (rows > 1 && ld < cols) return fail(MMN_E_INVALID, "a row pitch is smaller than the row");
+  const Range o = matrix_range(out, rows > 1 ? ld : cols, rows, cols, esize(dtype));
+  for (int i = 0; i < n; ++i)
+    if (ranges_meet(o, in[i])) return fail(MMN_E_INVALID, "the output overlaps an input");
+  return MMN_OK;
+}
+
+}  // namespace
+}  // namespace mmn
+
+using namespace mmn;
+
+extern "C" int mmn_mxfp4_size(int64_t rows, int64_t cols, int64_t* code_bytes_out,
+                              int64_t* scale_bytes_out) {
+  if (!code_bytes_out || !scale_bytes_out) return fail(MMN_E_INVALID, "null pointer");
+  const int rc = check_dims(rows, cols);
+  if (rc != MMN_OK) return rc;
+  *code_bytes_out = code_bytes(rows, cols);
+  *scale_bytes_out = cols ? scale_bytes(rows, cols) : 0;
+  return MMN_OK;
+}
+
+extern "C" int mmn_mxfp4_quantize(const void* x, int64_t x_ld, int dtype, int64_t rows,
+                                  int64_t cols, const mmn_mxfp4* q, const mmn_mxfp4* qt,
+                                  int device, void* stream) {
+  if (bad_dtype(dtype)) return fail(MMN_E_INVALID, "unknown dtype");
+  if (!q && !qt) return fail(MMN_E_INVALID, "neither q nor qt is given");
+  int rc, sms = 0;
+  if ((rc = check_dims(rows, cols)) != MMN_OK) return rc;
+  if (q && (q->rows != rows || q->cols != cols))
+    return fail(MMN_E_SHAPE, "q is not a rows x cols matrix");
+  if (qt && (qt->rows != cols || qt->cols != rows))
+    return fail(MMN_E_SHAPE, "qt is not a cols x rows matrix");
+  const bool empty = rows == 0 || cols == 0;
+  if (!empty && !x) return fail(MMN_E_INVALID, "null pointer");
+  if (rows > 1 && x_ld < cols) return fail(MMN_E_INVALID, "a row pitch is smaller than cols");
+  if (q && (rc = check_mx(q, "q")) != MMN_OK) return rc;
+  if (qt && (rc = check_mx(qt, "qt")) != MMN_OK) return rc;
+  if (!empty) {
+    const Range rx = matrix_range(x, rows > 1 ? x_ld : cols, rows, cols, esize(dtype));
+    Range r[5] = {rx};
+    int n = 1;
+    for (const mmn_mxfp4* m : {q, qt})
+      if (m) {
+        r[n++] = codes_range(m);
+        r[n++] = scales_range(m);
+      }
+    for (int i = 0; i < n; ++i)
+      for (int j = i + 1; j < n; ++j)
+        if (ranges_meet(r[i], r[j])) return fail(MMN_E_INVALID, "two of the buffers overlap");
+  }
+  if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
+  if (empty) return MMN_OK;
+  DeviceGuard guard(device);
+  if ((rc = check_device_elems(x, esize(dtype), device, "x")) != MMN_OK) return rc;
+  if (q && (rc = check_mx_device(q, device, "q")) != MMN_OK) return rc;
+  if (qt && (rc = check_mx_device(qt, device, "qt")) != MMN_OK) return rc;
+  if ((rc = kernel_setup(device)) != MMN_OK) return rc;
+  return launch_quantize(x, rows > 1 ? x_ld : cols, dtype, rows, cols, q, qt,
+                         static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mmn_mxfp4_dequantize(const mmn_mxfp4* q, void* out, int64_t out_ld, int dtype,
+                                    int device, void* stream) {
+  if (!q) return fail(MMN_E_INVALID, "null matrix");
+  if (bad_dtype(dtype)) return fail(MMN_E_INVALID, "unknown dtype");
+  int rc, sms = 0;
+  if ((rc = check_mx(q, "q")) != MMN_OK) return rc;
+  const Range in[] = {codes_range(q), scales_range(q)};
+  if ((rc = check_out(out, out_ld, dtype, q->rows, q->cols, in, 2)) != MMN_OK) return rc;
+  if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
+  if (q->rows == 0 || q->cols == 0) return MMN_OK;
+  DeviceGuard guard(device);
+  if ((rc = check_mx_device(q, device, "q")) != MMN_OK) return rc;
+  if ((rc = check_device_elems(out, esize(dtype), device, "out")) != MMN_OK) return rc;
+  MxDequantArgs a{};
+  a.codes = static_cast<const uint8_t*>(q->codes);
+  a.scales = static_cast<const uint8_t*>(q->scales);
+  a.out = out;
+  a.ld = q->rows > 1 ? out_ld : q->cols;
+  a.pitch = code_pitch(q->cols);
+  a.rows = q->rows;
+  a.cols = q->cols;
+  a.chunks = (q->cols + 7) / 8;
+  a.ka = (int)scale_blocks(q->cols);
+  a.vec = vec_rows(out, a.ld, esize(dtype), 8);
+  const int64_t blocks = (a.rows * a.chunks + 255) / 256;
+  const unsigned grid = (unsigned)(blocks < (int64_t)sms * 32 ? blocks : (int64_t)sms * 32);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == MMN_DTYPE_BF16)
+    mx_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+  else
+    mx_dequantize_kernel<float><<<grid, 256, 0, s>>>(a);
+  MMN_CUDA_TRY(cudaGetLastError());
+  return MMN_OK;
+}
+
+extern "C" int mmn_mxfp4_matmul(const mmn_mxfp4* a, const mmn_mxfp4* b, void* out, int64_t out_ld,
+                                int dtype, int accumulate, int device, void* stream) {
+  if (!a || !b) return fail(MMN_E_INVALID, "null matrix");
+  if (bad_dtype(dtype)) return fail(MMN_E_INVALID, "unknown dtype");
+  int rc, sms = 0;
+  if ((rc = check_mx(a, "a")) != MMN_OK || (rc = check_mx(b, "b")) != MMN_OK) return rc;
+  if (a->cols != b->cols)
+    return fail(MMN_E_SHAPE, "a and b differ in cols, the axis that is summed");
+  const Range in[] = {codes_range(a), scales_range(a), codes_range(b), scales_range(b)};
+  if ((rc = check_out(out, out_ld, dtype, a->rows, b->rows, in, 4)) != MMN_OK) return rc;
+  if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
+  if (a->rows == 0 || b->rows == 0) return MMN_OK;
+  DeviceGuard guard(device);
+  if ((rc = check_mx_device(a, device, "a")) != MMN_OK) return rc;
+  if ((rc = check_mx_device(b, device, "b")) != MMN_OK) return rc;
+  if ((rc = check_device_elems(out, esize(dtype), device, "out")) != MMN_OK) return rc;
+  if ((rc = kernel_setup(device)) != MMN_OK) return rc;
+  return product(a, b, out, a->rows > 1 ? out_ld : b->rows, dtype, accumulate,
+                 static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mmn_mxfp4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t rows,
+                                const mmn_mxfp4* w, const mmn_mxfp4* xq, void* out, int64_t out_ld,
+                                int out_dtype, int device, void* stream) {
+  if (!w || !xq) return fail(MMN_E_INVALID, "null matrix");
+  if (bad_dtype(x_dtype) || bad_dtype(out_dtype)) return fail(MMN_E_INVALID, "unknown dtype");
+  int rc, sms = 0;
+  if ((rc = check_dims(rows, w->cols)) != MMN_OK) return rc;
+  if (xq->rows != rows || xq->cols != w->cols)
+    return fail(MMN_E_SHAPE, "xq is not a rows x w.cols matrix");
+  if ((rc = check_mx(w, "w")) != MMN_OK || (rc = check_mx(xq, "xq")) != MMN_OK) return rc;
+  const int64_t cols = w->cols;
+  const bool empty = rows == 0 || cols == 0;
+  if (!empty && !x) return fail(MMN_E_INVALID, "null pointer");
+  if (rows > 1 && x_ld < cols) return fail(MMN_E_INVALID, "a row pitch is smaller than cols");
+  const Range in[] = {matrix_range(x, rows > 1 ? x_ld : cols, rows, cols, esize(x_dtype)),
+                      codes_range(w), scales_range(w), codes_range(xq), scales_range(xq)};
+  for (int i = 0; i < 3; ++i)
+    if (ranges_meet(in[i], in[3]) || ranges_meet(in[i], in[4]))
+      return fail(MMN_E_INVALID, "xq overlaps an input");
+  if (ranges_meet(in[3], in[4])) return fail(MMN_E_INVALID, "xq's codes and scales overlap");
+  if ((rc = check_out(out, out_ld, out_dtype, rows, w->rows, in, 5)) != MMN_OK) return rc;
+  if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
+  if (rows == 0 || w->rows == 0) return MMN_OK;
+  DeviceGuard guard(device);
+  if (cols && (rc = check_device_elems(x, esize(x_dtype), device, "x")) != MMN_OK) return rc;
+  if ((rc = check_mx_device(w, device, "w")) != MMN_OK) return rc;
+  if ((rc = check_mx_device(xq, device, "xq")) != MMN_OK) return rc;
+  if ((rc = check_device_elems(out, esize(out_dtype), device, "out")) != MMN_OK) return rc;
+  if ((rc = kernel_setup(device)) != MMN_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cols && (rc = launch_quantize(x, rows > 1 ? x_ld : cols, x_dtype, rows, cols, xq, nullptr,
+                                    s)) != MMN_OK)
+    return rc;
+  return product(xq, w, out, rows > 1 ? out_ld : w->rows, out_dtype, 0, s);
+}
+
+extern "C" int mmn_kernel_status(int device, void* stream) {
+  int rc, sms = 0;
+  if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
+  DeviceGuard guard(device);
+  int* word = nullptr;
+  if ((rc = status_word(&word)) != MMN_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int st = 0;
+  MMN_CUDA_TRY(cudaMemcpyAsync(&st, word, sizeof(int), cudaMemcpyDeviceToHost, s));
+  MMN_CUDA_TRY(cudaStreamSynchronize(s));
+  if (st == kDevOk) return MMN_OK;
+  MMN_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), s));
+  MMN_CUDA_TRY(cudaStreamSynchronize(s));
+  return fail(MMN_E_TIMEOUT,
+              "a kernel gave up a bounded wait (device status " + std::to_string(st) + ")");
+}

@@ -1,0 +1,298 @@
+// The product of two 4-bit microscaled matrices on the sm_100a tensor cores:
+// out[i, j] = sum_k A[i, k] B[j, k], A and B in MXFP4 (e2m1 elements, one ue8m0
+// scale per 32 elements of k), fp32 accumulation, rounded once.
+//
+// tcgen05.mma kind::mxf4 takes K = 64 per instruction (32 bytes of packed
+// elements), so a 128-byte swizzle row is 256 elements: a stage holds 256 of K,
+// four MMAs. The scales of 128 rows x 128 elements are one 512-byte block, laid
+// out in global memory as TMEM wants them (row r, block k at (r % 32) * 16 +
+// (r / 32) * 4 + k), so a stage copies them with one bulk load per 128 rows and
+// tcgen05.cp moves them to TMEM. Each stage has its own TMEM columns for its
+// scales: they are free again when the stage is, which the commit of its MMAs
+// says.
+#pragma once
+#include <cuda.h>
+
+#include "mmn_ptx.cuh"
+
+namespace mmn {
+
+struct MxGemmArgs {
+  const uint8_t* sfa;  // scale blocks of the operand on the 128-row side
+  const uint8_t* sfb;  // scale blocks of the other operand
+  int ka;              // scale blocks along K of one 128-row tile (even)
+  int M, N;            // rows of the two operands (128-row side first)
+  int num_kb;          // stages of 256 along K
+  int rt_b;            // 128-row tiles of the second operand
+  int tiles_n;
+  void* out;
+  long long ld;        // elements between rows of out
+  int out_bf16;
+  int accumulate;
+  int vec;             // out and ld are aligned for 16-byte accesses
+  int* status;
+};
+
+template <int BN>
+struct MxShape {
+  static constexpr int kABytes = 128 * 128;
+  static constexpr int kBBytes = BN * 128;
+  static constexpr int kTileBytes = kABytes + kBBytes;
+  static constexpr int kSfbTiles = (BN + 127) / 128;
+  static constexpr int kSfBytes = 1024 * (1 + kSfbTiles);
+  static constexpr int kStageBytes = kTileBytes + kSfBytes;
+  static constexpr int kStagesMax = 220000 / kStageBytes;
+  static constexpr int kStages = kStagesMax < 8 ? kStagesMax : 8;
+  static constexpr int kAccCols = BN < 32 ? 32 : BN;
+  static constexpr int kSfCols = 8 * (1 + kSfbTiles);  // TMEM columns of one stage's scales
+  static constexpr int kColsUsed = kAccCols + kStages * kSfCols;
+  static constexpr int kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128
+                                   : kColsUsed <= 256 ? 256 : 512;
+  static constexpr int kEpiBytes = 4 * 32 * 33 * 4;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 512 + kEpiBytes;
+  static_assert(kColsUsed <= 512, "TMEM has 512 columns");
+  static_assert(kSmemBytes <= 232448, "shared memory per CTA");
+  static_assert(kStages >= 3, "pipeline depth");
+};
+
+// Writes (or adds) a 32 x 32 block held one row per lane (v[j] = column j) to
+// out rows r0.., columns c0.., through the warp's 32 x 33 stage.
+__device__ __forceinline__ void mx_store_block(const MxGemmArgs& a, long long r0, long long c0,
+                                               int rows, int cols, const float (&v)[32],
+                                               float* tst) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) tst[lane * 33 + j] = v[j];
+  __syncwarp();
+  if (a.vec && cols == 32) {
+    if (a.out_bf16) {
+      const int rs = lane >> 2, c8 = (lane & 3) * 8;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = q * 8 + rs;
+        if (r < rows) {
+          uint4* p = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) +
+                                              (r0 + r) * a.ld + c0 + c8);
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = tst[r * 33 + c8 + i];
+          if (a.accumulate) {
+            const uint4 old = *p;
+            const __nv_bfloat162* o2 = reinterpret_cast<const __nv_bfloat162*>(&old);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f[2 * i] += __low2float(o2[i]);
+              f[2 * i + 1] += __high2float(o2[i]);
+            }
+          }
+          uint4 u;
+          __nv_bfloat162* u2 = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u2[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+          *p = u;
+        }
+      }
+    } else {
+      const int rs = lane >> 3, c4 = (lane & 7) * 4;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int r = q * 4 + rs;
+        if (r < rows) {
+          float4* p =
+              reinterpret_cast<float4*>(static_cast<float*>(a.out) + (r0 + r) * a.ld + c0 + c4);
+          const float* t = tst + r * 33 + c4;
+          float4 u = make_float4(t[0], t[1], t[2], t[3]);
+          if (a.accumulate) {
+            const float4 o = *p;
+            u.x += o.x;
+            u.y += o.y;
+            u.z += o.z;
+            u.w += o.w;
+          }
+          *p = u;
+        }
+      }
+    }
+  } else if (lane < cols) {
+    for (int r = 0; r < rows && r < 32; ++r) {
+      float f = tst[r * 33 + lane];
+      const long long i = (r0 + r) * a.ld + c0 + lane;
+      if (a.out_bf16) {
+        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out) + i;
+        if (a.accumulate) f += __bfloat162float(*p);
+        *p = __float2bfloat16_rn(f);
+      } else {
+        float* p = static_cast<float*>(a.out) + i;
+        *p = a.accumulate ? *p + f : f;
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// One 128 x BN tile per CTA. TRANS: the 128-row operand's rows are out's
+// columns. Warp 0 loads, warp 1 issues the copies and MMAs, warps 2-5 store.
+template <int BN, bool TRANS>
+__global__ void __launch_bounds__(192, 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
+                   const __grid_constant__ CUtensorMap tm_b, const MxGemmArgs args) {
+  using S = MxShape<BN>;
+  constexpr int STAGES = S::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* tiles = smem;
+  uint8_t* sfs = smem + STAGES * S::kTileBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sfs + STAGES * S::kSfBytes);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = full + 2 * STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tfull + 2);
+  float* epi = reinterpret_cast<float*>(sfs + STAGES * S::kSfBytes + 512);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tm = blockIdx.x / args.tiles_n, tn = blockIdx.x % args.tiles_n;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, S::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const int row0 = tm * 128, col0 = tn * BN;
+      uint32_t last = 0, issued = 0;  // parity of each stage's last load, stages used
+      for (int kb = 0; kb < args.num_kb; ++kb) {
+        const int s = kb % STAGES;
+        const uint32_t ph = (kb / STAGES) & 1;
+        if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) break;
+        mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+        uint8_t* t = tiles + s * S::kTileBytes;
+        tma_load_3d(t, &tm_a, &full[s], kb * 128, row0, 0);
+        tma_load_3d(t + S::kABytes, &tm_b, &full[s], kb * 128, col0, 0);
+        uint8_t* f = sfs + s * S::kSfBytes;
+        bulk_load(f, args.sfa + ((long long)tm * args.ka + kb * 2) * 512, 1024, &full[s]);
+#pragma unroll
+        for (int g = 0; g < S::kSfbTiles; ++g) {
+          // (a tile beyond the operand's last takes that one's scales: its
+          // elements are zero and its columns are not stored)
+          const int rt = min(col0 / 128 + g, args.rt_b - 1);
+          bulk_load(f + 1024 * (1 + g), args.sfb + ((long long)rt * args.ka + kb * 2) * 512, 1024,
+                    &full[s]);
+        }
+        issued |= 1u << s;
+        last = (last & ~(1u << s)) | (ph << s);
+      }
+      // every load lands before the CTA may exit
+      for (int s = 0; s < STAGES; ++s)
+        if (issued & (1u << s)) {
+          const uint64_t t0 = global_timer_ns();
+          while (!mbar_try_wait(&full[s], (last >> s) & 1u))
+            if (global_timer_ns() - t0 > kWaitLimitNs) {
+              *abort_flag = 1;
+              break;
+            }
+        }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int kb = 0; ok && kb < args.num_kb; ++kb) {
+        const int s = kb % STAGES;
+        if (!mbar_wait(&full[s], (kb / STAGES) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t t = smem_u32(tiles + s * S::kTileBytes);
+        const uint32_t f = smem_u32(sfs + s * S::kSfBytes);
+        // scale columns of the stage: [K half][4], then [K half][row group][4]
+        const uint32_t sa = tmem_base + S::kAccCols + s * S::kSfCols;
+        const uint32_t sb = sa + 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tc_cp_scales(sa + 4 * h, umma_desc_scales(f + 512 * h));
+#pragma unroll
+          for (int g = 0; g < S::kSfbTiles; ++g)
+            tc_cp_scales(sb + (h * S::kSfbTiles + g) * 4,
+                         umma_desc_scales(f + 1024 * (1 + g) + 512 * h));
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          constexpr uint32_t id0 = umma_idesc_mxf4(128, BN, 0), id1 = umma_idesc_mxf4(128, BN, 1);
+          const int h = kk >> 1;
+          tc_mma_mxf4(tmem_base, umma_desc_sw128(t + kk * 32, 16, 1024),
+                      umma_desc_sw128(t + S::kABytes + kk * 32, 16, 1024), (kk & 1) ? id1 : id0,
+                      sa + 4 * h, sb + h * S::kSfbTiles * 4, (kb | kk) != 0);
+        }
+        tc_commit(&empty[s]);
+      }
+      tc_commit(tfull);  // also on the way out after a time-out: what was issued ends first
+      if (!ok) {
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(tfull, 0))
+          if (global_timer_ns() - t0 > kWaitLimitNs) break;
+      }
+    }
+  } else {
+    const int sub = warp & 3;
+    const bool ready = mbar_wait(tfull, 0, abort_flag);
+    if (__all_sync(0xffffffffu, ready)) {  // tcgen05.ld is warp-collective
+      tc_fence_after();
+      float* tst = epi + (warp - 2) * 32 * 33;
+      const int m0 = tm * 128 + sub * 32;
+#pragma unroll 1
+      for (int ch = 0; ch < (BN + 31) / 32; ++ch) {
+        const int n0 = tn * BN + ch * 32;
+        float v[32];
+        tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(sub * 32) << 16) + ch * 32, v);
+        tmem_ld_wait();
+        const int mr = min(32, args.M - m0), nr = min(32, min(args.N, (tn + 1) * BN) - n0);
+        if (mr <= 0 || nr <= 0) continue;
+        if constexpr (TRANS) {
+          if (lane < mr) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < nr) {
+                const long long i = (long long)(n0 + j) * args.ld + m0 + lane;
+                if (args.out_bf16) {
+                  __nv_bfloat16* p = static_cast<__nv_bfloat16*>(args.out) + i;
+                  *p = __float2bfloat16_rn(args.accumulate ? v[j] + __bfloat162float(*p) : v[j]);
+                } else {
+                  float* p = static_cast<float*>(args.out) + i;
+                  *p = args.accumulate ? *p + v[j] : v[j];
+                }
+              }
+          }
+        } else {
+          mx_store_block(args, m0, n0, mr, nr, v, tst);
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && threadIdx.x == 0) atomicExch(args.status, kDevWaitTimeout);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, S::kTmemCols);
+  }
+}
+
+}  // namespace mmn

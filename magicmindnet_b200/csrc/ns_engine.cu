@@ -190,6 +190,22 @@ bool use_pairs(const NsClass& c) { return c.n >= 256; }
 
 }  // namespace
 
+std::string encode_byte_rows(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows,
+                             int box_rows) {
+  std::string err = get_encode();
+  if (!err.empty()) return err;
+  cuuint64_t dims[3] = {(cuuint64_t)row_bytes, (cuuint64_t)rows, 1};
+  cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)row_bytes * (cuuint64_t)rows};
+  cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")";
+  return "";
+}
+
 std::string ns_gemm_setup() {
   cudaError_t e = cudaSuccess;
 #define MMN_SET(BN, D, MN, E)                                  \

@@ -84,6 +84,12 @@ int ns_class_run(NsClass& c, int steps, int mode, int* status, int num_sms,
                  cudaStream_t stream, std::string* err, const NsFused* fused = nullptr,
                  const int* skip = nullptr);
 
+// Tensor map of a matrix of bytes (rows x row_bytes, pitch row_bytes, a multiple
+// of 16) for 128-byte-swizzled K-major operand boxes of box_rows x 128 bytes.
+// Returns an empty string on success, else a message.
+std::string encode_byte_rows(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows,
+                             int box_rows);
+
 // Opt-in shared memory for every GEMM instantiation (once per device).
 std::string ns_gemm_setup();
 

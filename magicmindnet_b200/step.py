@@ -180,6 +180,14 @@ class OptimizerStep:
         ptr = self._ptrs(slot)[2]
         return None if not ptr else _view(ptr, self.shapes[slot], "bf16", self.device)
 
+    def forward_param(self, slot: int):
+        """torch view of the copy of a slot's parameter that every rank holds after
+        a step: fp32, but on several ranks with bf16_param_shadow the bf16 one
+        (there the fp32 master stays with its owner)."""
+        if self.config.world_size > 1 and self.config.bf16_param_shadow:
+            return self.param_bf16(slot)
+        return self.param(slot)
+
     def _numel(self, slot: int) -> int:
         return int(np.prod(self.shapes[slot], dtype=np.int64))
 
