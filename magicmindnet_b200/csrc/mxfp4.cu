@@ -387,6 +387,7 @@ int kernel_setup(int device) {
   MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<64, true>, smem, MxShape<64>::kSmemBytes));
   MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<128, true>, smem, MxShape<128>::kSmemBytes));
   MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<128, false>, smem, MxShape<128>::kSmemBytes));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_pair_kernel, smem, MxPair::kSmemBytes));
   if (device < 64) done |= uint64_t(1) << device;
   return MMN_OK;
 }
@@ -450,9 +451,69 @@ int launch_gemm(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, cudaStrea
   return MMN_OK;
 }
 
+// The CTA pairs that fit on the GPU at once (a persistent grid must not exceed
+// them: a pair scheduled late would run its whole tile list after the others).
+int max_pairs(int sms, int* out) {
+  static std::mutex mu;
+  static int known_sms = 0, pairs = 0;  // every sm_100 device gives the same for its SM count
+  std::lock_guard<std::mutex> lock(mu);
+  if (known_sms != sms) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (sms / 2), 1, 1);
+    cfg.blockDim = dim3(MxPair::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = MxPair::kSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    MMN_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, mx_gemm_pair_kernel, &cfg));
+    if (n <= 0) return fail(MMN_E_CUDA, "no CTA pair fits on the device");
+    pairs = n < sms / 2 ? n : sms / 2;
+    known_sms = sms;
+  }
+  *out = pairs;
+  return MMN_OK;
+}
+
+int launch_gemm_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int sms,
+                     cudaStream_t s) {
+  CUtensorMap ta, tb, tsa, tsb;
+  const int64_t runs = scale_blocks(a->cols) / 2;
+  std::string err = encode_byte_rows(&ta, a->codes, code_pitch(a->cols), a->rows, 128);
+  if (err.empty()) err = encode_byte_rows(&tb, b->codes, code_pitch(b->cols), b->rows, 128);
+  if (err.empty()) err = encode_scale_runs(&tsa, a->scales, runs, (a->rows + 127) / 128, 1);
+  if (err.empty()) err = encode_scale_runs(&tsb, b->scales, runs, (b->rows + 127) / 128, 2);
+  if (!err.empty()) return fail(MMN_E_CUDA, err);
+  g.M = (int)a->rows;
+  g.N = (int)b->rows;
+  g.num_kb = (int)((a->cols + 255) / 256);
+  g.tiles_n = (int)((b->rows + 255) / 256);
+  const int64_t tiles_m = (a->rows + 255) / 256, tiles = tiles_m * g.tiles_n;
+  if (tiles > (int64_t(1) << 30)) return fail(MMN_E_SHAPE, "product too large");
+  int pairs = 0, rc = max_pairs(sms, &pairs);
+  if (rc != MMN_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs), 1, 1);
+  cfg.blockDim = dim3(MxPair::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = MxPair::kSmemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel, ta, tb, tsa, tsb, g, (int)tiles_m,
+                                  (int)tiles));
+  return MMN_OK;
+}
+
 // out (a.rows x b.rows) = A B^T, on checked arguments.
 int product(const mmn_mxfp4* a, const mmn_mxfp4* b, void* out, int64_t ld, int dtype,
-            int accumulate, cudaStream_t s) {
+            int accumulate, int sms, cudaStream_t s) {
   if (a->rows == 0 || b->rows == 0) return MMN_OK;
   if (a->cols == 0) {
     if (accumulate) return MMN_OK;
@@ -473,6 +534,7 @@ int product(const mmn_mxfp4* a, const mmn_mxfp4* b, void* out, int64_t ld, int d
   if (a->rows <= 32) return launch_gemm<32, true>(b, a, g, s);
   if (a->rows <= 64) return launch_gemm<64, true>(b, a, g, s);
   if (a->rows <= 128) return launch_gemm<128, true>(b, a, g, s);
+  if (a->rows > 256 && b->rows > 256) return launch_gemm_pair(a, b, g, sms, s);
   return launch_gemm<128, false>(a, b, g, s);
 }
 
@@ -594,7 +656,7 @@ extern "C" int mmn_mxfp4_matmul(const mmn_mxfp4* a, const mmn_mxfp4* b, void* ou
   if ((rc = check_mx_device(b, device, "b")) != MMN_OK) return rc;
   if ((rc = check_device_elems(out, esize(dtype), device, "out")) != MMN_OK) return rc;
   if ((rc = kernel_setup(device)) != MMN_OK) return rc;
-  return product(a, b, out, a->rows > 1 ? out_ld : b->rows, dtype, accumulate,
+  return product(a, b, out, a->rows > 1 ? out_ld : b->rows, dtype, accumulate, sms,
                  static_cast<cudaStream_t>(stream));
 }
 
@@ -631,7 +693,7 @@ extern "C" int mmn_mxfp4_linear(const void* x, int64_t x_ld, int x_dtype, int64_
   if (cols && (rc = launch_quantize(x, rows > 1 ? x_ld : cols, x_dtype, rows, cols, xq, nullptr,
                                     s)) != MMN_OK)
     return rc;
-  return product(xq, w, out, rows > 1 ? out_ld : w->rows, out_dtype, 0, s);
+  return product(xq, w, out, rows > 1 ? out_ld : w->rows, out_dtype, 0, sms, s);
 }
 
 extern "C" int mmn_kernel_status(int device, void* stream) {

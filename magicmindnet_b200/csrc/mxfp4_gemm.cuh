@@ -295,4 +295,245 @@ __global__ void __launch_bounds__(192, 1)
   }
 }
 
+// ---------------------------------------------------------------- CTA pairs
+// 256 x 256 tiles on CTA pairs, persistent: each CTA loads its 128 rows of A and
+// half of B's rows, and the scales of its rows of A and of all of B's.
+//
+// TMEM (512 columns): two accumulators of 256 columns that overlap by 96, and four
+// sets of scales of 24 columns. The epilogue drains the overlapping columns
+// first and releases them, so the next tile's MMAs start while the rest is
+// still being stored.
+struct MxPair {
+  static constexpr int kABytes = 128 * 128;
+  static constexpr int kBBytes = 128 * 128;
+  static constexpr int kTileBytes = kABytes + kBBytes;
+  static constexpr int kSfBytes = 3 * 1024;
+  static constexpr int kStageBytes = kTileBytes + kSfBytes;
+  static constexpr int kStages = 5;
+  static constexpr int kAcc1 = 160;    // first column of the second accumulator
+  static constexpr int kSfCol = 416;   // first column of the scales
+  static constexpr int kSfCols = 24;
+  static constexpr int kSfSets = 4;
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kEpiBytes = kEpiWarps * 32 * 33 * 4;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 512 + kEpiBytes;
+  static_assert(kSfCol + kSfSets * kSfCols == 512, "TMEM columns");
+  static_assert(kAcc1 + 256 <= kSfCol, "TMEM columns");
+  static_assert(kSmemBytes <= 232448, "shared memory per CTA");
+};
+
+// Tile order: bands of kBand tile rows, column by column within a band, so that
+// the pairs at work share operand tiles in L2.
+__device__ __forceinline__ void mx_tile(int tile, int tiles_m, int tiles_n, int& tm, int& tn) {
+  constexpr int kBand = 8;
+  const int band = tile / (kBand * tiles_n);
+  const int h = min(kBand, tiles_m - band * kBand);
+  const int r = tile - band * kBand * tiles_n;
+  tn = r / h;
+  tm = band * kBand + (r - tn * h);
+}
+
+__global__ void __launch_bounds__(MxPair::kThreads, 1)
+    mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
+                        const __grid_constant__ CUtensorMap tm_b,
+                        const __grid_constant__ CUtensorMap tm_sfa,
+                        const __grid_constant__ CUtensorMap tm_sfb, const MxGemmArgs args,
+                        int tiles_m, int num_tiles) {
+  using S = MxPair;
+  constexpr int STAGES = S::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* tiles = smem;
+  uint8_t* sfs = smem + STAGES * S::kTileBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sfs + STAGES * S::kSfBytes);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = full + 2 * STAGES;       // [2]
+  uint64_t* tempty = full + 2 * STAGES + 2;  // one phase per tile
+  uint64_t* drain = full + 2 * STAGES + 3;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + 2 * STAGES + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(full + 2 * STAGES + 5);
+  float* epi = reinterpret_cast<float*>(sfs + STAGES * S::kSfBytes + 512);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int group = blockIdx.x >> 1, groups = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&tfull[0], 1);
+    mbar_init(&tfull[1], 1);
+    mbar_init(tempty, 2 * S::kEpiWarps);  // one lane of every epilogue warp of the pair
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_b);
+    tma_prefetch_desc(&tm_sfa);
+    tma_prefetch_desc(&tm_sfb);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers are initialised, both TMEM allocations done
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0, last = 0;
+      bool ok = true;
+      for (int tile = group; ok && tile < num_tiles; tile += groups) {
+        int tm, tn;
+        mx_tile(tile, tiles_m, args.tiles_n, tm, tn);
+        for (int kb = 0; kb < args.num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (leader) mbar_arrive_expect_tx(&full[stage], 2 * S::kStageBytes);
+          const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);
+          uint8_t* t = tiles + stage * S::kTileBytes;
+          uint8_t* f = sfs + stage * S::kSfBytes;
+          tma_load_3d_pair(t, &tm_a, fb, kb * 128, tm * 256 + (int)rank * 128, 0);
+          tma_load_3d_pair(t + S::kABytes, &tm_b, fb, kb * 128, tn * 256 + (int)rank * 128, 0);
+          tma_load_3d_pair(f, &tm_sfa, fb, 0, kb, tm * 2 + (int)rank);
+          tma_load_3d_pair(f + 1024, &tm_sfb, fb, 0, kb, tn * 2);
+          issued |= 1u << stage;
+          last = (last & ~(1u << stage)) | (phase << stage);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // Every load lands before the CTA may exit; the leader's barriers count
+      // both CTAs' bytes, and the final cluster barrier holds the peer.
+      if (leader)
+        for (int s = 0; s < STAGES; ++s)
+          if (issued & (1u << s)) {
+            const uint64_t t0 = global_timer_ns();
+            while (!mbar_try_wait(&full[s], (last >> s) & 1u))
+              if (global_timer_ns() - t0 > kWaitLimitNs) {
+                *abort_flag = 1;
+                break;
+              }
+          }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      constexpr uint32_t id0 = umma_idesc_mxf4(256, 256, 0), id1 = umma_idesc_mxf4(256, 256, 1);
+      int stage = 0, g = 0, it = 0;  // g: k blocks so far, it: tiles so far
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = group; ok && tile < num_tiles; tile += groups, ++it) {
+        // the columns that the previous tile's accumulator shares with this one
+        if (it > 0 && !mbar_wait(tempty, (it - 1) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t acc = tmem_base + ((it & 1) ? S::kAcc1 : 0);
+        for (int kb = 0; kb < args.num_kb; ++kb, ++g) {
+          // the scale columns were last read by the MMAs of four k blocks ago
+          if (g >= S::kSfSets) {
+            const int o = g - S::kSfSets;
+            if (!mbar_wait(&empty[o % STAGES], (o / STAGES) & 1, abort_flag)) {
+              ok = false;
+              break;
+            }
+          }
+          if (!mbar_wait(&full[stage], phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t t = smem_u32(tiles + stage * S::kTileBytes);
+          const uint32_t f = smem_u32(sfs + stage * S::kSfBytes);
+          // [K half][4] for A, [K half][row group][4] for B
+          const uint32_t sa = tmem_base + S::kSfCol + (g % S::kSfSets) * S::kSfCols;
+          const uint32_t sb = sa + 8;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            tc_cp_scales_pair(sa + 4 * h, umma_desc_scales(f + 512 * h));
+            tc_cp_scales_pair(sb + 8 * h, umma_desc_scales(f + 1024 + 512 * h));
+            tc_cp_scales_pair(sb + 8 * h + 4, umma_desc_scales(f + 2048 + 512 * h));
+          }
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const int h = kk >> 1;
+            tc_mma_mxf4_pair(acc, umma_desc_sw128(t + kk * 32, 16, 1024),
+                             umma_desc_sw128(t + S::kABytes + kk * 32, 16, 1024),
+                             (kk & 1) ? id1 : id0, sa + 4 * h, sb + 8 * h, (kb | kk) != 0);
+          }
+          tc_commit_pair_mc(&empty[stage], 0x3);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair_mc(&tfull[it & 1], 0x3);
+      }
+      if (*abort_flag && g > 0) {
+        // what was issued ends before TMEM is freed
+        tc_commit_pair_mc(drain, 0x1);
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(drain, 0))
+          if (global_timer_ns() - t0 > kWaitLimitNs) break;
+      }
+    }
+  } else {
+    const int sub = warp & 3, half = (warp - 2) >> 2;
+    float* tst = epi + (warp - 2) * 32 * 33;
+    const uint32_t tempty_leader = mapa_shared(smem_u32(tempty), 0);
+    int it = 0;
+    for (int tile = group; tile < num_tiles; tile += groups, ++it) {
+      int tm, tn;
+      mx_tile(tile, tiles_m, args.tiles_n, tm, tn);
+      const bool ready = mbar_wait(&tfull[it & 1], (it >> 1) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ready)) break;  // tcgen05.ld is warp-collective
+      tc_fence_after();
+      const uint32_t acc = tmem_base + ((uint32_t)(sub * 32) << 16) + ((it & 1) ? S::kAcc1 : 0);
+      const int m0 = tm * 256 + (int)rank * 128 + sub * 32;
+      const int mr = min(32, args.M - m0);
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        // the first accumulator shares its last columns, the second its first
+        const int ord = 2 * i + half, ch = (it & 1) ? ord : 7 - ord;
+        const int n0 = tn * 256 + ch * 32;
+        float v[32];
+        tmem_ld_32x32b_x32(acc + ch * 32, v);
+        tmem_ld_wait();
+        if (i == 1) {
+          // the four outermost chunks are read: release them
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tempty_leader);
+        }
+        const int nr = min(32, args.N - n0);
+        if (mr > 0 && nr > 0) mx_store_block(args, m0, n0, mr, nr, v, tst);
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // peer loads landed, remote arrivals done, MMAs retired
+  if (*abort_flag && threadIdx.x == 0) atomicExch(args.status, kDevWaitTimeout);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
 }  // namespace mmn

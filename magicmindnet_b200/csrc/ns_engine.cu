@@ -206,6 +206,22 @@ std::string encode_byte_rows(CUtensorMap* map, const void* base, int64_t row_byt
   return "";
 }
 
+std::string encode_scale_runs(CUtensorMap* map, const void* base, int64_t pairs, int64_t tiles,
+                              int box_tiles) {
+  std::string err = get_encode();
+  if (!err.empty()) return err;
+  cuuint64_t dims[3] = {256, (cuuint64_t)pairs, (cuuint64_t)tiles};
+  cuuint64_t strides[2] = {1024, (cuuint64_t)pairs * 1024};
+  cuuint32_t box[3] = {256, 1, (cuuint32_t)box_tiles};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")";
+  return "";
+}
+
 std::string ns_gemm_setup() {
   cudaError_t e = cudaSuccess;
 #define MMN_SET(BN, D, MN, E)                                  \

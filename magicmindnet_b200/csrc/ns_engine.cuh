@@ -90,6 +90,11 @@ int ns_class_run(NsClass& c, int steps, int mode, int* status, int num_sms,
 std::string encode_byte_rows(CUtensorMap* map, const void* base, int64_t row_bytes, int64_t rows,
                              int box_rows);
 
+// Tensor map of MXFP4 scales: `tiles` 128-row tiles of `pairs` 1024-byte runs
+// (256 columns of K); a box is one run of box_tiles consecutive tiles.
+std::string encode_scale_runs(CUtensorMap* map, const void* base, int64_t pairs, int64_t tiles,
+                              int box_tiles);
+
 // Opt-in shared memory for every GEMM instantiation (once per device).
 std::string ns_gemm_setup();
 
