@@ -387,19 +387,23 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  // The loading and the issuing warp stay converged: all lanes wait, one elected
+  // lane issues. (With the waits inside a one-lane branch the scale copies did
+  // not overlap the MMAs: 183 instead of 128 clocks per MMA.)
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, issued = 0, last = 0;
-      bool ok = true;
-      for (int tile = group; ok && tile < num_tiles; tile += groups) {
-        int tm, tn;
-        mx_tile(tile, tiles_m, args.tiles_n, tm, tn);
-        for (int kb = 0; kb < args.num_kb; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
-            ok = false;
-            break;
-          }
+    const bool one = elect_one();
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, last = 0;
+    bool ok = true;
+    for (int tile = group; ok && tile < num_tiles; tile += groups) {
+      int tm, tn;
+      mx_tile(tile, tiles_m, args.tiles_n, tm, tn);
+      for (int kb = 0; kb < args.num_kb; ++kb) {
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1u, abort_flag)) {
+          ok = false;
+          break;
+        }
+        if (one) {
           if (leader) mbar_arrive_expect_tx(&full[stage], 2 * S::kStageBytes);
           const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);
           uint8_t* t = tiles + stage * S::kTileBytes;
@@ -408,89 +412,90 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
           tma_load_3d_pair(t + S::kABytes, &tm_b, fb, kb * 128, tn * 256 + (int)rank * 128, 0);
           tma_load_3d_pair(f, &tm_sfa, fb, 0, kb, tm * 2 + (int)rank);
           tma_load_3d_pair(f + 1024, &tm_sfb, fb, 0, kb, tn * 2);
-          issued |= 1u << stage;
-          last = (last & ~(1u << stage)) | (phase << stage);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        }
+        issued |= 1u << stage;
+        last = (last & ~(1u << stage)) | (phase << stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      // Every load lands before the CTA may exit; the leader's barriers count
-      // both CTAs' bytes, and the final cluster barrier holds the peer.
-      if (leader)
-        for (int s = 0; s < STAGES; ++s)
-          if (issued & (1u << s)) {
-            const uint64_t t0 = global_timer_ns();
-            while (!mbar_try_wait(&full[s], (last >> s) & 1u))
-              if (global_timer_ns() - t0 > kWaitLimitNs) {
-                *abort_flag = 1;
-                break;
-              }
-          }
     }
+    // Every load lands before the CTA may exit; the leader's barriers count
+    // both CTAs' bytes, and the final cluster barrier holds the peer.
+    if (leader)
+      for (int s = 0; s < STAGES; ++s)
+        if (issued & (1u << s)) {
+          const uint64_t t0 = global_timer_ns();
+          while (!mbar_try_wait(&full[s], (last >> s) & 1u))
+            if (global_timer_ns() - t0 > kWaitLimitNs) {
+              *abort_flag = 1;
+              break;
+            }
+        }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
+      const bool one = elect_one();
       constexpr uint32_t id0 = umma_idesc_mxf4(256, 256, 0), id1 = umma_idesc_mxf4(256, 256, 1);
       int stage = 0, g = 0, it = 0;  // g: k blocks so far, it: tiles so far
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = group; ok && tile < num_tiles; tile += groups, ++it) {
         // the columns that the previous tile's accumulator shares with this one
-        if (it > 0 && !mbar_wait(tempty, (it - 1) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
+        if (it > 0 && !mbar_wait_warp(tempty, (it - 1) & 1, abort_flag)) break;
         tc_fence_after();
         const uint32_t acc = tmem_base + ((it & 1) ? S::kAcc1 : 0);
         for (int kb = 0; kb < args.num_kb; ++kb, ++g) {
           // the scale columns were last read by the MMAs of four k blocks ago
-          if (g >= S::kSfSets) {
-            const int o = g - S::kSfSets;
-            if (!mbar_wait(&empty[o % STAGES], (o / STAGES) & 1, abort_flag)) {
-              ok = false;
-              break;
-            }
+          const int o = g - S::kSfSets;
+          if (o >= 0 && !mbar_wait_warp(&empty[o % STAGES], (o / STAGES) & 1, abort_flag)) {
+            ok = false;
+            break;
           }
-          if (!mbar_wait(&full[stage], phase, abort_flag)) {
+          if (!mbar_wait_warp(&full[stage], phase, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t t = smem_u32(tiles + stage * S::kTileBytes);
-          const uint32_t f = smem_u32(sfs + stage * S::kSfBytes);
-          // [K half][4] for A, [K half][row group][4] for B
-          const uint32_t sa = tmem_base + S::kSfCol + (g % S::kSfSets) * S::kSfCols;
-          const uint32_t sb = sa + 8;
+          if (one) {
+            const uint32_t t = smem_u32(tiles + stage * S::kTileBytes);
+            const uint32_t f = smem_u32(sfs + stage * S::kSfBytes);
+            // [K half][4] for A, [K half][row group][4] for B
+            const uint32_t sa = tmem_base + S::kSfCol + (g % S::kSfSets) * S::kSfCols;
+            const uint32_t sb = sa + 8;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            tc_cp_scales_pair(sa + 4 * h, umma_desc_scales(f + 512 * h));
-            tc_cp_scales_pair(sb + 8 * h, umma_desc_scales(f + 1024 + 512 * h));
-            tc_cp_scales_pair(sb + 8 * h + 4, umma_desc_scales(f + 2048 + 512 * h));
-          }
+            for (int h = 0; h < 2; ++h) {
+              tc_cp_scales_pair(sa + 4 * h, umma_desc_scales(f + 512 * h));
+              tc_cp_scales_pair(sb + 8 * h, umma_desc_scales(f + 1024 + 512 * h));
+              tc_cp_scales_pair(sb + 8 * h + 4, umma_desc_scales(f + 2048 + 512 * h));
+            }
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const int h = kk >> 1;
-            tc_mma_mxf4_pair(acc, umma_desc_sw128(t + kk * 32, 16, 1024),
-                             umma_desc_sw128(t + S::kABytes + kk * 32, 16, 1024),
-                             (kk & 1) ? id1 : id0, sa + 4 * h, sb + 8 * h, (kb | kk) != 0);
+            for (int kk = 0; kk < 4; ++kk) {
+              const int h = kk >> 1;
+              tc_mma_mxf4_pair(acc, umma_desc_sw128(t + kk * 32, 16, 1024),
+                               umma_desc_sw128(t + S::kABytes + kk * 32, 16, 1024),
+                               (kk & 1) ? id1 : id0, sa + 4 * h, sb + 8 * h, (kb | kk) != 0);
+            }
+            tc_commit_pair_mc(&empty[stage], 0x3);
           }
-          tc_commit_pair_mc(&empty[stage], 0x3);
+          __syncwarp();
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        tc_commit_pair_mc(&tfull[it & 1], 0x3);
+        if (one) tc_commit_pair_mc(&tfull[it & 1], 0x3);
+        __syncwarp();
       }
-      if (*abort_flag && g > 0) {
+      if (one && *abort_flag && g > 0) {
         // what was issued ends before TMEM is freed
         tc_commit_pair_mc(drain, 0x1);
         const uint64_t t0 = global_timer_ns();
         while (!mbar_try_wait(drain, 0))
           if (global_timer_ns() - t0 > kWaitLimitNs) break;
       }
+      __syncwarp();
     }
   } else {
     const int sub = warp & 3, half = (warp - 2) >> 2;
