@@ -123,6 +123,16 @@ __device__ __forceinline__ void tma_store_3d(const void* desc, const void* smem_
                : "memory");
 }
 
+// tma_store_3d that adds fp32 values to what the tensor holds.
+__device__ __forceinline__ void tma_add_3d(const void* desc, const void* smem_src, int x, int y,
+                                           int z) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], "
+      "[%1];" ::"l"(reinterpret_cast<uint64_t>(desc)),
+      "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -134,6 +144,11 @@ __device__ __forceinline__ void bulk_commit() {
 // The committed bulk stores have finished reading shared memory.
 __device__ __forceinline__ void bulk_wait_read_all() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
+// All but the last committed bulk store have finished reading shared memory.
+__device__ __forceinline__ void bulk_wait_read_but_one() {
+  asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
 }
 
 // The committed bulk stores are complete.

@@ -480,12 +480,19 @@ int max_pairs(int sms, int* out) {
 
 int launch_gemm_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int sms,
                      cudaStream_t s) {
-  CUtensorMap ta, tb, tsa, tsb;
+  CUtensorMap ta, tb, tsa, tsb, to;
   const int64_t runs = scale_blocks(a->cols) / 2;
   std::string err = encode_byte_rows(&ta, a->codes, code_pitch(a->cols), a->rows, 128);
   if (err.empty()) err = encode_byte_rows(&tb, b->codes, code_pitch(b->cols), b->rows, 128);
   if (err.empty()) err = encode_scale_runs(&tsa, a->scales, runs, (a->rows + 127) / 128, 1);
   if (err.empty()) err = encode_scale_runs(&tsb, b->scales, runs, (b->rows + 127) / 128, 2);
+  // bf16 values are added in the epilogue's registers: a TMA addition would round
+  // the product to bf16 before the sum
+  g.tma_out = g.vec && !(g.out_bf16 && g.accumulate);
+  if (!g.tma_out)
+    to = ta;
+  else if (err.empty())
+    err = encode_store_rows(&to, g.out, a->rows, b->rows, g.ld, g.out_bf16 ? 2 : 4);
   if (!err.empty()) return fail(MMN_E_CUDA, err);
   g.M = (int)a->rows;
   g.N = (int)b->rows;
@@ -506,8 +513,8 @@ int launch_gemm_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int 
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel, ta, tb, tsa, tsb, g, (int)tiles_m,
-                                  (int)tiles));
+  MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel, ta, tb, tsa, tsb, to, g,
+                                  (int)tiles_m, (int)tiles));
   return MMN_OK;
 }
 

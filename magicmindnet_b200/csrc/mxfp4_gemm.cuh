@@ -30,6 +30,7 @@ struct MxGemmArgs {
   int out_bf16;
   int accumulate;
   int vec;             // out and ld are aligned for 16-byte accesses
+  int tma_out;         // the pair kernel stores through its tensor map
   int* status;
 };
 
@@ -316,8 +317,10 @@ struct MxPair {
   static constexpr int kSfSets = 4;
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
-  static constexpr int kEpiBytes = kEpiWarps * 32 * 33 * 4;
+  static constexpr int kEpiWarpBytes = 4608;  // two 2 KB store boxes, or a 32 x 33 fp32 tile
+  static constexpr int kEpiBytes = kEpiWarps * kEpiWarpBytes;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 512 + kEpiBytes;
+  static_assert(kEpiWarpBytes >= 32 * 33 * 4 && kEpiWarpBytes % 512 == 0, "epilogue stage");
   static_assert(kSfCol + kSfSets * kSfCols == 512, "TMEM columns");
   static_assert(kAcc1 + 256 <= kSfCol, "TMEM columns");
   static_assert(kSmemBytes <= 232448, "shared memory per CTA");
@@ -334,11 +337,54 @@ __device__ __forceinline__ void mx_tile(int tile, int tiles_m, int tiles_n, int&
   tm = band * kBand + (r - tn * h);
 }
 
+// One 32 x 32 block (v[j] = column c0 + j of the lane's row) to out by TMA: rows
+// of 64 bytes (all 32 columns in bf16, 16 of fp32) are staged with the 64-byte
+// swizzle (conflict-free 16-byte stores) in two buffers that alternate, so a
+// store is read out of shared memory while the next is filled. Clipped at the
+// matrix edge by the tensor map. ADD (fp32): added to what out holds.
+template <bool BF16>
+__device__ __forceinline__ void mx_store_tma(const CUtensorMap* map, uint8_t* stage, int c0, int r0,
+                                             bool add, const float (&v)[32], int& buf) {
+  const int lane = threadIdx.x & 31, sw = (lane >> 1) & 3;
+#pragma unroll
+  for (int h = 0; h < (BF16 ? 1 : 2); ++h) {
+    uint8_t* st = stage + buf * 2048;
+    buf ^= 1;
+    if (lane == 0) bulk_wait_read_but_one();
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint4 u;
+      if constexpr (BF16) {
+        __nv_bfloat162* u2 = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          u2[i] = __floats2bfloat162_rn(v[c * 8 + 2 * i], v[c * 8 + 2 * i + 1]);
+      } else {
+        u = make_uint4(__float_as_uint(v[h * 16 + c * 4]), __float_as_uint(v[h * 16 + c * 4 + 1]),
+                       __float_as_uint(v[h * 16 + c * 4 + 2]),
+                       __float_as_uint(v[h * 16 + c * 4 + 3]));
+      }
+      *reinterpret_cast<uint4*>(st + lane * 64 + ((c ^ sw) << 4)) = u;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (!BF16 && add)
+        tma_add_3d(map, st, c0 + h * 16, r0, 0);
+      else
+        tma_store_3d(map, st, c0 + h * 16, r0, 0);
+      bulk_commit();
+    }
+  }
+}
+
 __global__ void __launch_bounds__(MxPair::kThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
                         const __grid_constant__ CUtensorMap tm_b,
                         const __grid_constant__ CUtensorMap tm_sfa,
-                        const __grid_constant__ CUtensorMap tm_sfb, const MxGemmArgs args,
+                        const __grid_constant__ CUtensorMap tm_sfb,
+                        const __grid_constant__ CUtensorMap tm_out, const MxGemmArgs args,
                         int tiles_m, int num_tiles) {
   using S = MxPair;
   constexpr int STAGES = S::kStages;
@@ -354,7 +400,7 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
   uint64_t* drain = full + 2 * STAGES + 3;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + 2 * STAGES + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(full + 2 * STAGES + 5);
-  float* epi = reinterpret_cast<float*>(sfs + STAGES * S::kSfBytes + 512);
+  uint8_t* epi = sfs + STAGES * S::kSfBytes + 512;  // 512-byte aligned, as the swizzle needs
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -499,7 +545,8 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
     }
   } else {
     const int sub = warp & 3, half = (warp - 2) >> 2;
-    float* tst = epi + (warp - 2) * 32 * 33;
+    uint8_t* stg = epi + (warp - 2) * S::kEpiWarpBytes;
+    int buf = 0;
     const uint32_t tempty_leader = mapa_shared(smem_u32(tempty), 0);
     int it = 0;
     for (int tile = group; tile < num_tiles; tile += groups, ++it) {
@@ -511,25 +558,40 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
       const uint32_t acc = tmem_base + ((uint32_t)(sub * 32) << 16) + ((it & 1) ? S::kAcc1 : 0);
       const int m0 = tm * 256 + (int)rank * 128 + sub * 32;
       const int mr = min(32, args.M - m0);
+      // The first accumulator shares its last columns with the second, that one
+      // its first: the outermost four of the eight 32-column chunks are read
+      // first, two a warp, and released before anything is stored.
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        // the first accumulator shares its last columns, the second its first
-        const int ord = 2 * i + half, ch = (it & 1) ? ord : 7 - ord;
-        const int n0 = tn * 256 + ch * 32;
-        float v[32];
-        tmem_ld_32x32b_x32(acc + ch * 32, v);
+      for (int i = 0; i < 4; i += 2) {
+        const int o0 = 2 * i + half, o1 = o0 + 2;
+        const int ch0 = (it & 1) ? o0 : 7 - o0, ch1 = (it & 1) ? o1 : 7 - o1;
+        float v[32], w[32];
+        tmem_ld_32x32b_x32(acc + ch0 * 32, v);
+        tmem_ld_32x32b_x32(acc + ch1 * 32, w);
         tmem_ld_wait();
-        if (i == 1) {
-          // the four outermost chunks are read: release them
+        if (i == 0) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(tempty_leader);
         }
-        const int nr = min(32, args.N - n0);
-        if (mr > 0 && nr > 0) mx_store_block(args, m0, n0, mr, nr, v, tst);
+        auto store = [&](int ch, const float (&x)[32]) {
+          const int n0 = tn * 256 + ch * 32, nr = min(32, args.N - n0);
+          if (mr <= 0 || nr <= 0) return;
+          if (args.tma_out) {
+            if (args.out_bf16)
+              mx_store_tma<true>(&tm_out, stg, n0, m0, false, x, buf);
+            else
+              mx_store_tma<false>(&tm_out, stg, n0, m0, args.accumulate, x, buf);
+          } else {
+            mx_store_block(args, m0, n0, mr, nr, x, reinterpret_cast<float*>(stg));
+          }
+        };
+        store(ch0, v);
+        store(ch1, w);
       }
       tc_fence_before();
     }
+    if (args.tma_out && lane == 0) bulk_wait_all();  // the stage outlives the stores that read it
   }
   tc_fence_before();
   __syncthreads();

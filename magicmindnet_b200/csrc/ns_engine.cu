@@ -206,6 +206,21 @@ std::string encode_byte_rows(CUtensorMap* map, const void* base, int64_t row_byt
   return "";
 }
 
+std::string encode_store_rows(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int64_t ld,
+                              int esize) {
+  std::string err = get_encode();
+  if (!err.empty()) return err;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
+  cuuint64_t strides[2] = {(cuuint64_t)(ld * esize), (cuuint64_t)(ld * esize)};
+  cuuint32_t box[3] = {(cuuint32_t)(64 / esize), 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, map_type(esize), 3, base, dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")";
+  return "";
+}
+
 std::string encode_scale_runs(CUtensorMap* map, const void* base, int64_t pairs, int64_t tiles,
                               int box_tiles) {
   std::string err = get_encode();

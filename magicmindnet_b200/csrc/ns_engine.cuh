@@ -95,6 +95,12 @@ std::string encode_byte_rows(CUtensorMap* map, const void* base, int64_t row_byt
 std::string encode_scale_runs(CUtensorMap* map, const void* base, int64_t pairs, int64_t tiles,
                               int box_tiles);
 
+// Tensor map for TMA stores of 32-row x 64-byte boxes (64-byte swizzle) into a
+// rows x cols matrix of bf16 (esize 2) or fp32 (esize 4), pitch ld elements;
+// base and pitch are multiples of 16 bytes.
+std::string encode_store_rows(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int64_t ld,
+                              int esize);
+
 // Opt-in shared memory for every GEMM instantiation (once per device).
 std::string ns_gemm_setup();
 
