@@ -300,10 +300,11 @@ __global__ void __launch_bounds__(192, 1)
 // 256 x 256 tiles on CTA pairs, persistent: each CTA loads its 128 rows of A and
 // half of B's rows, and the scales of its rows of A and of all of B's.
 //
-// TMEM (512 columns): two accumulators of 256 columns that overlap by 96, and four
-// sets of scales of 24 columns. The epilogue drains the overlapping columns
-// first and releases them, so the next tile's MMAs start while the rest is
-// still being stored.
+// TMEM (512 columns): two accumulators of 256 columns that overlap by 120, and a
+// set of 24 columns of scales per stage (a stage that has been loaded again has
+// had its MMAs completed, so its scale columns are free too). The epilogue
+// drains the overlapping columns first and releases them, so the next tile's
+// MMAs start while the rest is still being stored.
 struct MxPair {
   static constexpr int kABytes = 128 * 128;
   static constexpr int kBBytes = 128 * 128;
@@ -311,18 +312,16 @@ struct MxPair {
   static constexpr int kSfBytes = 3 * 1024;
   static constexpr int kStageBytes = kTileBytes + kSfBytes;
   static constexpr int kStages = 5;
-  static constexpr int kAcc1 = 160;    // first column of the second accumulator
-  static constexpr int kSfCol = 416;   // first column of the scales
   static constexpr int kSfCols = 24;
-  static constexpr int kSfSets = 4;
+  static constexpr int kSfCol = 512 - kStages * kSfCols;  // first column of the scales
+  static constexpr int kAcc1 = kSfCol - 256;  // first column of the second accumulator
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kEpiWarpBytes = 4608;  // two 2 KB store boxes, or a 32 x 33 fp32 tile
   static constexpr int kEpiBytes = kEpiWarps * kEpiWarpBytes;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 512 + kEpiBytes;
   static_assert(kEpiWarpBytes >= 32 * 33 * 4 && kEpiWarpBytes % 512 == 0, "epilogue stage");
-  static_assert(kSfCol + kSfSets * kSfCols == 512, "TMEM columns");
-  static_assert(kAcc1 + 256 <= kSfCol, "TMEM columns");
+  static_assert(256 - kAcc1 <= 128, "the epilogue releases four chunks of 32 columns first");
   static_assert(kSmemBytes <= 232448, "shared memory per CTA");
 };
 
@@ -483,38 +482,40 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
     if (leader) {
       const bool one = elect_one();
       constexpr uint32_t id0 = umma_idesc_mxf4(256, 256, 0), id1 = umma_idesc_mxf4(256, 256, 1);
-      int stage = 0, g = 0, it = 0;  // g: k blocks so far, it: tiles so far
+      int stage = 0, it = 0;  // it: tiles so far
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = group; ok && tile < num_tiles; tile += groups, ++it) {
-        // the columns that the previous tile's accumulator shares with this one
-        if (it > 0 && !mbar_wait_warp(tempty, (it - 1) & 1, abort_flag)) break;
-        tc_fence_after();
         const uint32_t acc = tmem_base + ((it & 1) ? S::kAcc1 : 0);
-        for (int kb = 0; kb < args.num_kb; ++kb, ++g) {
-          // the scale columns were last read by the MMAs of four k blocks ago
-          const int o = g - S::kSfSets;
-          if (o >= 0 && !mbar_wait_warp(&empty[o % STAGES], (o / STAGES) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
+        for (int kb = 0; kb < args.num_kb; ++kb) {
           if (!mbar_wait_warp(&full[stage], phase, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
+          const uint32_t t = smem_u32(tiles + stage * S::kTileBytes);
+          const uint32_t f = smem_u32(sfs + stage * S::kSfBytes);
+          // [K half][4] for A, [K half][row group][4] for B
+          const uint32_t sa = tmem_base + S::kSfCol + stage * S::kSfCols;
+          const uint32_t sb = sa + 8;
           if (one) {
-            const uint32_t t = smem_u32(tiles + stage * S::kTileBytes);
-            const uint32_t f = smem_u32(sfs + stage * S::kSfBytes);
-            // [K half][4] for A, [K half][row group][4] for B
-            const uint32_t sa = tmem_base + S::kSfCol + (g % S::kSfSets) * S::kSfCols;
-            const uint32_t sb = sa + 8;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               tc_cp_scales_pair(sa + 4 * h, umma_desc_scales(f + 512 * h));
               tc_cp_scales_pair(sb + 8 * h, umma_desc_scales(f + 1024 + 512 * h));
               tc_cp_scales_pair(sb + 8 * h + 4, umma_desc_scales(f + 2048 + 512 * h));
             }
+          }
+          __syncwarp();
+          if (kb == 0 && it > 0) {
+            // the columns that the previous tile's accumulator shares with this one
+            if (!mbar_wait_warp(tempty, (it - 1) & 1, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
+          if (one) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
               const int h = kk >> 1;
@@ -534,7 +535,7 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
         if (one) tc_commit_pair_mc(&tfull[it & 1], 0x3);
         __syncwarp();
       }
-      if (one && *abort_flag && g > 0) {
+      if (one && *abort_flag) {
         // what was issued ends before TMEM is freed
         tc_commit_pair_mc(drain, 0x1);
         const uint64_t t0 = global_timer_ns();
