@@ -42,11 +42,20 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   return r;
 }
 
-// The value of a 4-bit code.
-__device__ __forceinline__ float e2m1_value(uint32_t c) {
-  const uint32_t e = (c >> 1) & 3u, m = c & 1u;
-  const float a = e ? (float)((2u + m) << e) * 0.25f : (float)m * 0.5f;
-  return (c & 8u) ? -a : a;
+// The values of four 4-bit codes, through bf16, which holds them: the byte
+// permutation looks up the high and the low byte of 0, 1/2, 1, 3/2, 2, 3, 4, 6.
+__device__ __forceinline__ void e2m1x4_values(uint32_t w, float* v) {
+  const uint32_t sel = w & 0x7777u;
+  const uint32_t hi = __byte_perm(0x3F3F3F00u, 0x40404040u, sel);
+  const uint32_t lo = __byte_perm(0xC0800000u, 0xC0804000u, sel);
+  const uint32_t p0 =
+      __byte_perm(lo, hi, 0x5140) | ((w & 0x8u) << 12) | ((w & 0x80u) << 24);
+  const uint32_t p1 =
+      __byte_perm(lo, hi, 0x7362) | ((w & 0x800u) << 4) | ((w & 0x8000u) << 16);
+  v[0] = __uint_as_float(p0 << 16);
+  v[1] = __uint_as_float(p0 & 0xFFFF0000u);
+  v[2] = __uint_as_float(p1 << 16);
+  v[3] = __uint_as_float(p1 & 0xFFFF0000u);
 }
 
 // Scale byte of a block from the bits of its largest magnitude as fp32 (taken
@@ -83,7 +92,7 @@ template <typename T>
 struct MxTile {
   static constexpr int kPitch = 128 * sizeof(T) + 16;  // bytes; the skew spreads a column over banks
   static constexpr int kCodePitch = 80;
-  static constexpr int kSmem = 128 * kPitch + 128 * kCodePitch + 1024;
+  static constexpr int kSmem = 128 * kPitch + 1024;
 };
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
@@ -92,18 +101,17 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes
                : "memory");
 }
 
-// One 128 x 128 tile per block: it goes to shared memory once; eight threads'
-// chunks of a row make the blocks of x, and thread columns of 32 rows the
-// blocks of x transposed, whose bytes are collected in shared memory so that
-// global memory sees 64 consecutive bytes per row of codes. A tile gives exactly
-// one 512-byte block of scales in each direction.
+// One 128 x 128 tile per block: it goes to shared memory once; threads take its
+// blocks of 32 along the rows, then down the columns, whose bytes are collected
+// in shared memory so that global memory sees 64 consecutive bytes per row of
+// codes. A tile gives exactly one 512-byte block of scales in each direction.
 template <typename T>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
   constexpr int kPitch = MxTile<T>::kPitch;
   constexpr bool kBf16 = sizeof(T) == 2;
   extern __shared__ __align__(16) uint8_t sm[];
-  uint8_t* codes_s = sm + 128 * kPitch;
-  uint8_t* sf_row = codes_s + 128 * MxTile<T>::kCodePitch;
+  uint8_t* codes_s = sm;  // the transposed codes take the tile's place once it is read
+  uint8_t* sf_row = sm + 128 * kPitch;
   uint8_t* sf_col = sf_row + 512;
   const int tid = threadIdx.x;
   const int ct = blockIdx.x % a.nct, rt = blockIdx.x / a.nct;
@@ -143,44 +151,66 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
   __syncthreads();
 
   if (a.codes) {
-#pragma unroll 2
-    for (int i = 0; i < 8; ++i) {
-      const int id = i * 256 + tid, r = id >> 4, ch = id & 15;
-      float v[8];
-      uint32_t m;
+    // a thread per block of 32: eight rows at a time read the same columns, so the
+    // skewed rows spread over the banks, and a row's four blocks leave together
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = (i * 8 + (tid >> 5)) * 8 + (tid & 7), k4 = (tid >> 3) & 3;
+      uint32_t q4[4], s;
       if constexpr (kBf16) {
-        const uint4 u = *reinterpret_cast<const uint4*>(sm + r * kPitch + ch * 16);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        uint4 u[4];
         uint32_t mm = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          mm = __vmaxu2(mm, w[k] & 0x7FFF7FFFu);
-          v[2 * k] = __uint_as_float(w[k] << 16);
-          v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+        for (int q = 0; q < 4; ++q) {
+          u[q] = *reinterpret_cast<const uint4*>(sm + r * kPitch + k4 * 64 + q * 16);
+          mm = __vmaxu2(mm, __vmaxu2(__vmaxu2(u[q].x & 0x7FFF7FFFu, u[q].y & 0x7FFF7FFFu),
+                                     __vmaxu2(u[q].z & 0x7FFF7FFFu, u[q].w & 0x7FFF7FFFu)));
         }
-        m = max(mm & 0xFFFFu, mm >> 16) << 16;
+        s = mx_scale(max(mm & 0xFFFFu, mm >> 16) << 16);
+        const float inv = mx_inv_scale(s);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[2 * k] = __uint_as_float(w[k] << 16) * inv;
+            v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u) * inv;
+          }
+          q4[q] = e2m1x8(v);
+        }
       } else {
-        const float4 u0 = *reinterpret_cast<const float4*>(sm + r * kPitch + ch * 32);
-        const float4 u1 = *reinterpret_cast<const float4*>(sm + r * kPitch + ch * 32 + 16);
-        v[0] = u0.x, v[1] = u0.y, v[2] = u0.z, v[3] = u0.w;
-        v[4] = u1.x, v[5] = u1.y, v[6] = u1.z, v[7] = u1.w;
-        m = 0;
+        float w[32];
+        uint32_t m = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7FFFFFFFu);
+        for (int q = 0; q < 8; ++q) {
+          const float4 f = *reinterpret_cast<const float4*>(sm + r * kPitch + k4 * 128 + q * 16);
+          w[4 * q] = f.x, w[4 * q + 1] = f.y, w[4 * q + 2] = f.z, w[4 * q + 3] = f.w;
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) m = max(m, __float_as_uint(w[k]) & 0x7FFFFFFFu);
+        s = mx_scale(m);
+        const float inv = mx_inv_scale(s);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = w[q * 8 + k] * inv;
+          q4[q] = e2m1x8(v);
+        }
       }
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const uint32_t s = mx_scale(m);
-      const float inv = mx_inv_scale(s);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= inv;
-      const int64_t off = (int64_t)ct * 64 + ch * 4;
+      const int64_t off = (int64_t)ct * 64 + k4 * 16;
       if (r < nr && off < a.pitch)
-        *reinterpret_cast<uint32_t*>(a.codes + (int64_t)(r0 + r) * a.pitch + off) = e2m1x8(v);
-      if ((ch & 3) == 0) sf_row[(r & 31) * 16 + (r >> 5) * 4 + (ch >> 2)] = (uint8_t)s;
+        *reinterpret_cast<uint4*>(a.codes + (int64_t)(r0 + r) * a.pitch + off) =
+            make_uint4(q4[0], q4[1], q4[2], q4[3]);
+      sf_row[(r & 31) * 16 + (r >> 5) * 4 + k4] = (uint8_t)s;
     }
   }
   if (a.codes_t) {
+    // 64 values per thread: two columns of 32 rows (bf16, read as words), or one
+    // column in two blocks of rows
+    uint4 o[2];
+    uint32_t sb[2];
     if constexpr (kBf16) {
       const int cp = tid & 63, rb = tid >> 6;
       uint32_t w[32], mm = 0;
@@ -191,26 +221,23 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int c = cp * 2 + half;
-        const uint32_t s = mx_scale(half ? mm & 0xFFFF0000u : mm << 16);
-        const float inv = mx_inv_scale(s);
-        uint32_t o[4];
+        sb[half] = mx_scale(half ? mm & 0xFFFF0000u : mm << 16);
+        const float inv = mx_inv_scale(sb[half]);
+        uint32_t q4[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k)
             v[k] = __uint_as_float(half ? w[q * 8 + k] & 0xFFFF0000u : w[q * 8 + k] << 16) * inv;
-          o[q] = e2m1x8(v);
+          q4[q] = e2m1x8(v);
         }
-        *reinterpret_cast<uint4*>(codes_s + c * MxTile<T>::kCodePitch + rb * 16) =
-            make_uint4(o[0], o[1], o[2], o[3]);
-        sf_col[(c & 31) * 16 + (c >> 5) * 4 + rb] = (uint8_t)s;
+        o[half] = make_uint4(q4[0], q4[1], q4[2], q4[3]);
       }
     } else {
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        const int c = tid & 127, rb = (tid >> 7) + 2 * h;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int c = tid & 127, rb = (tid >> 7) + 2 * half;
         float w[32];
         uint32_t m = 0;
 #pragma unroll
@@ -218,20 +245,26 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
           w[i] = *reinterpret_cast<const float*>(sm + (rb * 32 + i) * kPitch + c * 4);
           m = max(m, __float_as_uint(w[i]) & 0x7FFFFFFFu);
         }
-        const uint32_t s = mx_scale(m);
-        const float inv = mx_inv_scale(s);
-        uint32_t o[4];
+        sb[half] = mx_scale(m);
+        const float inv = mx_inv_scale(sb[half]);
+        uint32_t q4[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] = w[q * 8 + k] * inv;
-          o[q] = e2m1x8(v);
+          q4[q] = e2m1x8(v);
         }
-        *reinterpret_cast<uint4*>(codes_s + c * MxTile<T>::kCodePitch + rb * 16) =
-            make_uint4(o[0], o[1], o[2], o[3]);
-        sf_col[(c & 31) * 16 + (c >> 5) * 4 + rb] = (uint8_t)s;
+        o[half] = make_uint4(q4[0], q4[1], q4[2], q4[3]);
       }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int c = kBf16 ? (tid & 63) * 2 + half : tid & 127;
+      const int rb = kBf16 ? tid >> 6 : (tid >> 7) + 2 * half;
+      *reinterpret_cast<uint4*>(codes_s + c * MxTile<T>::kCodePitch + rb * 16) = o[half];
+      sf_col[(c & 31) * 16 + (c >> 5) * 4 + rb] = (uint8_t)sb[half];
     }
   }
   __syncthreads();
@@ -258,45 +291,73 @@ struct MxDequantArgs {
   const uint8_t *codes, *scales;
   void* out;
   int64_t ld, pitch;
-  int64_t rows, cols, chunks;  // chunks of 8 columns per row
+  int rows, cols;
   int ka;
+  int nct;  // 256-column tiles
   int vec;
 };
 
+// 32 rows x 256 columns per block. A lane turns four bytes into eight bf16, or two
+// bytes into four fp32 (in two halves of the columns), so that every store of a
+// warp is 512 consecutive bytes; the loads of a lane's rows are issued first.
 template <typename T>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const MxDequantArgs a) {
-  const int64_t n = a.rows * a.chunks;
-  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < n;
-       id += (int64_t)gridDim.x * 256) {
-    const int64_t r = id / a.chunks, c = (id - r * a.chunks) * 8;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(a.codes + r * a.pitch + c / 2);
-    const uint32_t s = a.scales[((r >> 7) * a.ka + (c >> 7)) * 512 + (r & 31) * 16 +
-                                ((r >> 5) & 3) * 4 + ((c >> 5) & 3)];
-    const float f = mx_scale_value(s);
-    T* o = static_cast<T*>(a.out) + r * a.ld + c;
-    float v[8];
+  constexpr int V = 16 / sizeof(T), NH = 256 / (32 * V), NR = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int ct = blockIdx.x % a.nct, rt = blockIdx.x / a.nct;
+  uint32_t w[NH][NR], s[NH][NR];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = e2m1_value(w >> (4 * k)) * f;
-    if (a.vec && c + 8 <= a.cols) {
-      if constexpr (sizeof(T) == 2) {
-        uint4 u;
-        __nv_bfloat162* u2 = reinterpret_cast<__nv_bfloat162*>(&u);
+  for (int h = 0; h < NH; ++h) {
+    const int c = ct * 256 + (h * 32 + lane) * V;
+    const uint8_t* sc = a.scales + ((int64_t)(rt >> 2) * a.ka + (c >> 7)) * 512 + (rt & 3) * 4 +
+                        ((c >> 5) & 3);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) u2[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-        *reinterpret_cast<uint4*>(o) = u;
-      } else {
-        reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    for (int i = 0; i < NR; ++i) {
+      const int rr = warp + 8 * i;
+      w[h][i] = s[h][i] = 0;
+      if (c < a.cols && rt * 32 + rr < a.rows) {
+        const uint8_t* p = a.codes + (int64_t)(rt * 32 + rr) * a.pitch + c / 2;
+        w[h][i] = V == 8 ? *reinterpret_cast<const uint32_t*>(p)
+                         : *reinterpret_cast<const uint16_t*>(p);
+        s[h][i] = sc[rr * 16];
       }
-    } else {
+    }
+  }
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c + k < a.cols) {
-          if constexpr (sizeof(T) == 2)
-            o[k] = __float2bfloat16_rn(v[k]);
-          else
-            o[k] = v[k];
+  for (int i = 0; i < NR; ++i) {
+    const int r = rt * 32 + warp + 8 * i;
+    if (r >= a.rows) break;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      const int c = ct * 256 + (h * 32 + lane) * V;
+      if (c >= a.cols) break;
+      const float f = mx_scale_value(s[h][i]);
+      T* o = static_cast<T*>(a.out) + (int64_t)r * a.ld + c;
+      float v[V];
+#pragma unroll
+      for (int k = 0; k < V; k += 4) e2m1x4_values(w[h][i] >> (4 * k), v + k);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] *= f;
+      if (a.vec && c + V <= a.cols) {
+        if constexpr (sizeof(T) == 2) {
+          uint4 u;
+          __nv_bfloat162* u2 = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) u2[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+          *reinterpret_cast<uint4*>(o) = u;
+        } else {
+          *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
         }
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (c + k < a.cols) {
+            if constexpr (sizeof(T) == 2)
+              o[k] = __float2bfloat16_rn(v[k]);
+            else
+              o[k] = v[k];
+          }
+      }
     }
   }
 }
@@ -630,13 +691,14 @@ extern "C" int mmn_mxfp4_dequantize(const mmn_mxfp4* q, void* out, int64_t out_l
   a.out = out;
   a.ld = q->rows > 1 ? out_ld : q->cols;
   a.pitch = code_pitch(q->cols);
-  a.rows = q->rows;
-  a.cols = q->cols;
-  a.chunks = (q->cols + 7) / 8;
+  a.rows = (int)q->rows;
+  a.cols = (int)q->cols;
   a.ka = (int)scale_blocks(q->cols);
+  a.nct = (int)((q->cols + 255) / 256);
   a.vec = vec_rows(out, a.ld, esize(dtype), 8);
-  const int64_t blocks = (a.rows * a.chunks + 255) / 256;
-  const unsigned grid = (unsigned)(blocks < (int64_t)sms * 32 ? blocks : (int64_t)sms * 32);
+  const int64_t blocks = (q->rows + 31) / 32 * a.nct;
+  if (blocks > (int64_t(1) << 31) - 1) return fail(MMN_E_SHAPE, "matrix too large");
+  const unsigned grid = (unsigned)blocks;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MMN_DTYPE_BF16)
     mx_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
