@@ -534,9 +534,9 @@ int mmn_mxfp4_linear(const void *x, int64_t x_ld, int x_dtype, int64_t rows, con
                      const mmn_mxfp4 *xq, void *out, int64_t out_ld, int out_dtype, int device,
                      void *stream);
 
-/* Waits for `stream` and reports MMN_E_TIMEOUT when a kernel of
- * mmn_mxfp4_matmul or mmn_mxfp4_linear on `device` gave up a bounded wait since
- * the last report (mmn_optim_sync does this for a handle's kernels). */
+/* Waits for `stream` and reports MMN_E_TIMEOUT when a kernel of the calls above
+ * gave up a bounded wait on `device` since the last report (mmn_optim_sync does
+ * this for a handle's kernels). */
 int mmn_kernel_status(int device, void *stream);
 
 /* Parameter counts: total registered, stepped by AdamW, stepped by Muon. */

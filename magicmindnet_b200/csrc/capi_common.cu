@@ -158,6 +158,15 @@ int check_device_ptr(const void* p, int device, const char* what) {
   return MMN_OK;
 }
 
+// A caller-buffer kernel that gave up a bounded wait leaves its code here, per
+// device (mmn_kernel_status).
+__device__ int g_kernel_status;
+
+int kernel_status_word(int** p) {
+  MMN_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(p), g_kernel_status));
+  return MMN_OK;
+}
+
 int check_device_elems(const void* p, size_t esize, int device, const char* what) {
   if (reinterpret_cast<uintptr_t>(p) % esize)
     return fail(MMN_E_INVALID, std::string(what) + ": not aligned to its element size");

@@ -80,6 +80,9 @@ int check_device_ptr(const void* p, int device, const char* what);
 // check_device_ptr, and `p` is aligned to its elements of `esize` bytes.
 int check_device_elems(const void* p, size_t esize, int device, const char* what);
 
+// The current device's status word of the caller-buffer kernels (mmn_kernel_status).
+int kernel_status_word(int** p);
+
 // The device checks of the caller-buffer entry points: a usable sm_100 GPU,
 // whose SM count goes to *sms.
 int percall_device(int device, int* sms);

@@ -15,8 +15,10 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "capi_internal.cuh"
+#include "mmn_ptx.cuh"
 
 namespace mmn {
 namespace {
@@ -194,14 +196,314 @@ __global__ void __launch_bounds__(512) ln_fwd_wide_kernel(const LnFwd a) {
   }
 }
 
+// ------------------------------------------------------- pairs of fp32 values
+// sm_100 adds, multiplies and fuses two fp32 values per instruction; each half
+// rounds as the scalar instruction does.
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ f2 dup2(float v) { return pack2(v, v); }
+__device__ __forceinline__ float2 unpack2(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float sum2(f2 v) {
+  const float2 f = unpack2(v);
+  return f.x + f.y;
+}
+
+// V consecutive elements as V / 2 pairs, and back (rounded to T).
+template <typename T, int V>
+__device__ __forceinline__ void load_pairs(const T* p, f2* v) {
+  const Vec<T, V> u = load_vec<T, V>(p);
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j)
+      v[j] = pack2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) v[j] = pack2(to_f32(u.e[2 * j]), to_f32(u.e[2 * j + 1]));
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pairs(T* p, const f2* v) {
+  Vec<T, V> u;
+#pragma unroll
+  for (int j = 0; j < V / 2; ++j) {
+    const float2 f = unpack2(v[j]);
+    if constexpr (sizeof(T) == 2) {
+      reinterpret_cast<__nv_bfloat162*>(&u)[j] = __floats2bfloat162_rn(f.x, f.y);
+    } else {
+      from_f32(u.e[2 * j], f.x);
+      from_f32(u.e[2 * j + 1], f.y);
+    }
+  }
+  *reinterpret_cast<Vec<T, V>*>(p) = u;
+}
+template <int V>
+__device__ __forceinline__ void load_param_pairs(const void* p, bool bf16, int64_t c, f2* v) {
+  float u[V];
+  load_param<V>(p, bf16, c, u);
+#pragma unroll
+  for (int j = 0; j < V / 2; ++j) v[j] = pack2(u[2 * j], u[2 * j + 1]);
+}
+
+// A row's sum over the TR threads that hold it (red: one entry per warp of the row;
+// another buffer for the next call).
+template <int TR>
+__device__ __forceinline__ float row_sum1(float v, float* red) {
+#pragma unroll
+  for (int o = (TR < 32 ? TR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (TR > 32) {
+    constexpr int W = TR / 32;
+    if ((threadIdx.x & 31) == 0) red[(threadIdx.x >> 5) & (W - 1)] = v;
+    __syncthreads();
+    if constexpr (W == 2) {
+      v = red[0] + red[1];
+    } else {
+      v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; w += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(red + w);
+        v += (u.x + u.y) + (u.z + u.w);
+      }
+    }
+  }
+  return v;
+}
+
+// Two sums at once: the lanes with bit 4 clear go on with the first, the others
+// with the second (5 exchanges a warp in place of 10).
+template <int TR>
+__device__ __forceinline__ float2 ring_sum2(float x, float y, float2* red) {
+  const bool up = (threadIdx.x & 16) != 0;
+  float v = (up ? y : x) + __shfl_xor_sync(0xffffffffu, up ? x : y, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (TR == 32) {
+    return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+  } else {
+    constexpr int W = TR / 32;
+    if ((threadIdx.x & 15) == 0) reinterpret_cast<float*>(red)[(threadIdx.x >> 5) * 2 + (up ? 1 : 0)] = v;
+    __syncthreads();
+    f2 t = 0;
+#pragma unroll
+    for (int w = 0; w < W; w += 2) {
+      const float4 u = *reinterpret_cast<const float4*>(red + w);
+      t = add2(t, add2(pack2(u.x, u.y), pack2(u.z, u.w)));
+    }
+    return unpack2(t);
+  }
+}
+
+constexpr int kRingMax = 4;  // rows in flight per row group, at most (more gained nothing)
+constexpr int kFwdRing = 2;  // ... in the forward kernel
+
+// The forward kernel for rows that can be read four elements at a time: TR threads
+// hold one row, NE columns each, a block a row (or a few short ones). Chunks of
+// four keep every access, the fp32 parameters' too, to whole consecutive lines
+// per warp. A block lives 2 to 3 us, most of it waiting, so what is in flight is
+// what the blocks on the GPU hold: enough for fp32 rows (16384 x 4096 in 80.6
+// us, 6.66 TB/s) and not for bf16 ones (64 us, 4.2 TB/s; ln_fwd_ring_kernel).
+__host__ __device__ constexpr int ln_rows_block(int tr) { return tr <= 32 ? 128 : tr; }
+
+template <typename XT, typename YT, int TR, int NE>
+__global__ void __launch_bounds__(ln_rows_block(TR), ln_rows_block(TR) > 512 ? 1 : 1536 / ln_rows_block(TR))
+    ln_fwd_rows_kernel(const LnFwd a) {
+  constexpr int kBlock = ln_rows_block(TR), RB = kBlock / TR, V = 4, NC = NE / V, H = V / 2;
+  __shared__ __align__(16) float red[2][RB][32];
+  const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
+  const int64_t row = (int64_t)blockIdx.x * RB + sub;
+  const bool ok = row < a.rows;
+  const int cols = ok ? (int)a.cols : 0;
+  const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
+  f2 v[NE / 2];
+  f2 s = 0;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (i * TR + t) * V;
+    if (c < cols) {
+      load_pairs<XT, V>(x + c, v + i * H);
+    } else {
+#pragma unroll
+      for (int j = 0; j < H; ++j) v[i * H + j] = 0;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NE / 2; ++j) s = add2(s, v[j]);
+  const float inv_n = 1.0f / (float)a.cols;
+  const float mean = row_sum1<TR>(sum2(s), red[0][sub]) * inv_n;
+  const f2 nm = dup2(-mean);
+  f2 q = 0;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if ((i * TR + t) * V < cols) {
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        v[i * H + j] = add2(v[i * H + j], nm);
+        q = fma2(v[i * H + j], v[i * H + j], q);
+      }
+    }
+  const float var = row_sum1<TR>(sum2(q), red[1][sub]) * inv_n;
+  const float rstd = 1.0f / sqrtf(var + a.eps);
+  if (t == 0 && ok) {
+    if (a.mean) a.mean[row] = mean;
+    if (a.rstd) a.rstd[row] = rstd;
+  }
+  const f2 r2 = dup2(rstd);
+  YT* y = static_cast<YT*>(a.y) + row * a.y_ld;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (i * TR + t) * V;
+    if (c < cols) {
+      f2 ga[H], be[H];
+      load_param_pairs<V>(a.gamma, a.param_bf16, c, ga);
+      load_param_pairs<V>(a.beta, a.param_bf16, c, be);
+#pragma unroll
+      for (int j = 0; j < H; ++j) ga[j] = fma2(mul2(v[i * H + j], r2), ga[j], be[j]);
+      store_pairs<YT, V>(y + c, ga);
+    }
+  }
+}
+
+// bf16 rows, many of them: blocks walk the rows. gamma and beta stay in registers,
+// each row group keeps a ring of rows in flight through bulk copies, and a
+// thread takes 32 columns, since the conversions and the two sums across the
+// threads cost more instructions than the arithmetic. Needs rows that start and
+// end on 16 bytes.
+__host__ __device__ constexpr int ln_ring_block(int tr) { return tr <= 64 ? 128 : tr; }
+__host__ __device__ constexpr int ln_ring_blocks(int tr) { return 512 / ln_ring_block(tr); }
+
+template <typename XT, typename YT, int TR, int NE>
+__global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR))
+    ln_fwd_ring_kernel(const LnFwd a, int depth, int* status) {
+  constexpr int V = sizeof(XT) == 2 && sizeof(YT) == 2 ? 8 : 4;
+  constexpr int kBlock = ln_ring_block(TR), RB = kBlock / TR, NC = NE / V, H = V / 2;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ __align__(16) float red[2][RB][32];
+  __shared__ __align__(8) uint64_t bars[RB][kRingMax];
+  __shared__ volatile int abort_flag;
+  const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
+  const int cols = (int)a.cols, rb = cols * (int)sizeof(XT);
+  uint8_t* ring = dyn + sub * depth * rb;
+  const int64_t first = (int64_t)blockIdx.x * RB + sub, step = (int64_t)gridDim.x * RB;
+  if (threadIdx.x == 0) {
+    for (int g = 0; g < RB; ++g)
+      for (int d = 0; d < depth; ++d) mbar_init(&bars[g][d], 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  // rows of this group; the block runs as many trips as its first group has
+  const int mine = first < a.rows ? (int)((a.rows - first + step - 1) / step) : 0;
+  const int trips = (int)((a.rows - (int64_t)blockIdx.x * RB + step - 1) / step);
+  const XT* x = static_cast<const XT*>(a.x) + first * a.x_ld;
+  YT* y = static_cast<YT*>(a.y) + first * a.y_ld;
+  auto issue = [&](int k, int slot) {  // row k of this group into a slot
+    mbar_arrive_expect_tx(&bars[sub][slot], rb);
+    bulk_load(ring + slot * rb, x + k * step * a.x_ld, rb, &bars[sub][slot]);
+  };
+  if (t == 0)
+    for (int k = 0; k < depth && k < mine; ++k) issue(k, k);
+  f2 ga[NE / 2], be[NE / 2];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (i * TR + t) * V;
+    if (c < cols) {
+      load_param_pairs<V>(a.gamma, a.param_bf16, c, ga + i * H);
+      load_param_pairs<V>(a.beta, a.param_bf16, c, be + i * H);
+    }
+  }
+  const float inv_n = 1.0f / (float)cols;
+  int slot = 0;
+  uint32_t phase = 0;
+  for (int k = 0; k < trips; ++k) {
+    const int lim = k < mine ? cols : 0;
+    const XT* sx = reinterpret_cast<const XT*>(ring + slot * rb);
+    // (a wait that gives up marks the status; the loop runs on so that every
+    // barrier is met)
+    if (lim) mbar_wait(&bars[sub][slot], phase, &abort_flag);
+    f2 v[NE / 2], s = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (i * TR + t) * V;
+      if (c < lim) {
+        load_pairs<XT, V>(sx + c, v + i * H);
+#pragma unroll
+        for (int j = 0; j < H; ++j) s = add2(s, v[i * H + j]);
+      }
+    }
+    const float mean = row_sum1<TR>(sum2(s), red[0][sub]) * inv_n;
+    if constexpr (TR <= 32) __syncwarp();
+    // every thread of the group has the row in registers: its slot is free
+    if (t == 0 && k + depth < mine) issue(k + depth, slot);
+    const f2 nm = dup2(-mean);
+    f2 q = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if ((i * TR + t) * V < lim) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          v[i * H + j] = add2(v[i * H + j], nm);
+          q = fma2(v[i * H + j], v[i * H + j], q);
+        }
+      }
+    const float var = row_sum1<TR>(sum2(q), red[1][sub]) * inv_n;
+    const float rstd = 1.0f / sqrtf(var + a.eps);
+    if (t == 0 && lim) {
+      if (a.mean) a.mean[first + k * step] = mean;
+      if (a.rstd) a.rstd[first + k * step] = rstd;
+    }
+    const f2 r2 = dup2(rstd);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (i * TR + t) * V;
+      if (c < lim) {
+#pragma unroll
+        for (int j = 0; j < H; ++j)
+          v[i * H + j] = fma2(mul2(v[i * H + j], r2), ga[i * H + j], be[i * H + j]);
+        store_pairs<YT, V>(y + c, v + i * H);
+      }
+    }
+    y += step * a.y_ld;
+    if (++slot == depth) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  if (abort_flag && threadIdx.x == 0) atomicExch(status, kDevWaitTimeout);
+}
+
 // ------------------------------------------------------------------ backward
 // Blocks walk the rows; a thread owns the same columns in every row and keeps
 // their dgamma and dbeta sums in registers, so the rows are read once for both
 // results. Each block writes its sums; ln_bwd_sum_kernel adds them in a fixed
 // order (no atomics: the result does not depend on timing).
-__host__ __device__ constexpr int ln_bwd_block(int tr) { return tr <= 32 ? 256 : tr; }
+__host__ __device__ constexpr int ln_bwd_block(int tr) {
+  return tr == 8 ? 256 : tr == 32 ? 64 : tr;
+}
 __host__ __device__ constexpr int ln_bwd_min_blocks(int tr) {
-  return tr <= 32 ? 2 : tr == 128 ? 4 : tr == 256 ? 2 : 1;
+  return tr == 8 ? 2 : 512 / ln_bwd_block(tr);
 }
 
 template <typename XT, typename DT, int V, int TR, int NE>
@@ -309,6 +611,186 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
   }
 }
 
+// The same walk with the rows brought in by bulk copies: every row group keeps a
+// ring of `depth` rows of x and dy in flight in shared memory, so the loads of
+// the next rows run under the sums, the barrier and the stores of this one
+// (16384 x 4096 bf16: 113 us with the rows loaded into registers).
+// Needs rows that start and end on 16 bytes. NE <= 16: gamma, h and g live in
+// registers. NE = 32 (rows of 8192 to 16384): gamma is kept in shared memory, and
+// the second pass reads the row again.
+template <typename XT, typename DT, int V, int TR, int NE>
+__global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
+    ln_bwd_ring_kernel(const LnBwd a, int depth, int* status) {
+  constexpr int kBlock = ln_bwd_block(TR), RB = kBlock / TR, NC = NE / V, H = V / 2;
+  constexpr bool kReread = NE > 16;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  __shared__ __align__(16) float2 red[2][32];
+  __shared__ __align__(8) uint64_t bars[RB][kRingMax];
+  __shared__ volatile int abort_flag;
+  const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
+  const int xb = (int)(a.cols * sizeof(XT)), db = (int)(a.cols * sizeof(DT)), rb = xb + db;
+  const int gb = kReread ? (int)a.cols * 4 : 0;
+  float* gs = reinterpret_cast<float*>(dyn);  // gamma (kReread)
+  uint8_t* ring = dyn + gb + sub * depth * rb;
+  const int64_t first = (int64_t)blockIdx.x * RB + sub, step = (int64_t)gridDim.x * RB;
+  auto issue = [&](int64_t k, int slot) {  // row k of this group into a slot
+    const int64_t row = first + k * step;
+    mbar_arrive_expect_tx(&bars[sub][slot], rb);
+    bulk_load(ring + slot * rb, static_cast<const XT*>(a.x) + row * a.x_ld, xb, &bars[sub][slot]);
+    bulk_load(ring + slot * rb + xb, static_cast<const DT*>(a.dy) + row * a.dy_ld, db,
+              &bars[sub][slot]);
+  };
+  if (threadIdx.x == 0) {
+    for (int g = 0; g < RB; ++g)
+      for (int d = 0; d < depth; ++d) mbar_init(&bars[g][d], 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  // rows of this group; the block runs as many trips as its first group has
+  const int64_t mine = first < a.rows ? (a.rows - first + step - 1) / step : 0;
+  const int64_t first0 = (int64_t)blockIdx.x * RB;
+  const int64_t trips = first0 < a.rows ? (a.rows - first0 + step - 1) / step : 0;
+  if (t == 0)
+    for (int k = 0; k < depth && k < mine; ++k) issue(k, k);
+  f2 ga[kReread ? 1 : NE / 2];
+  if constexpr (kReread) {
+    for (int c = threadIdx.x; c < a.cols; c += kBlock)
+      gs[c] = a.param_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.gamma)[c])
+                           : static_cast<const float*>(a.gamma)[c];
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (i * TR + t) * V;
+      if (c < a.cols) load_param_pairs<V>(a.gamma, a.param_bf16, c, ga + i * H);
+    }
+  }
+  const float inv_n = 1.0f / (float)a.cols;
+  f2 sg[NE / 2], sb[NE / 2];
+#pragma unroll
+  for (int k = 0; k < NE / 2; ++k) sg[k] = sb[k] = 0;
+  float mean = 0.0f, rstd = 0.0f;
+  if (mine > 0) {
+    mean = a.mean[first];
+    rstd = a.rstd[first];
+  }
+  int slot = 0, prev = 0;
+  uint32_t phase = 0;
+  for (int64_t k = 0; k < trips; ++k) {
+    const bool ok = k < mine;
+    const int64_t row = first + k * step;
+    const uint8_t* sx = ring + slot * rb;
+    float mean2 = 0.0f, rstd2 = 0.0f;  // of the group's next row
+    if (k + 1 < mine) {
+      mean2 = a.mean[row + step];
+      rstd2 = a.rstd[row + step];
+    }
+    // (a wait that gives up marks the status; the loop runs on so that every
+    // barrier is met)
+    if (ok) mbar_wait(&bars[sub][slot], phase, &abort_flag);
+    const f2 nm = dup2(-mean), r2 = dup2(rstd);
+    f2 h[kReread ? 1 : NE / 2], g[kReread ? 1 : NE / 2];
+    f2 s1 = 0, s2 = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (i * TR + t) * V;
+      if (ok && c < a.cols) {
+        f2 x[H], d[H], gm[H];
+        load_pairs<XT, V>(reinterpret_cast<const XT*>(sx) + c, x);
+        load_pairs<DT, V>(reinterpret_cast<const DT*>(sx + xb) + c, d);
+        if constexpr (kReread) load_pairs<float, V>(gs + c, gm);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          const int e = i * H + j;
+          const f2 hh = mul2(add2(x[j], nm), r2);
+          const f2 gg = mul2(d[j], kReread ? gm[j] : ga[kReread ? 0 : e]);
+          s1 = add2(s1, gg);
+          s2 = fma2(gg, hh, s2);
+          sg[e] = fma2(d[j], hh, sg[e]);
+          sb[e] = add2(sb[e], d[j]);
+          if constexpr (!kReread) {
+            h[e] = hh;
+            g[e] = gg;
+          }
+        }
+      }
+    }
+    const float2 s = ring_sum2<TR>(sum2(s1), sum2(s2), red[k & 1]);
+    // every thread of the group is past the previous row: its slot is free
+    if (t == 0 && k > 0 && k - 1 + depth < mine) issue(k - 1 + depth, prev);
+    const f2 c1 = dup2(-s.x * inv_n), c2 = dup2(-s.y * inv_n);
+    if (ok) {
+      XT* dx = static_cast<XT*>(a.dx) + row * a.dx_ld;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = (i * TR + t) * V;
+        if (c < a.cols) {
+          f2 o[H];
+          if constexpr (kReread) {
+            f2 x[H], d[H], gm[H];
+            load_pairs<XT, V>(reinterpret_cast<const XT*>(sx) + c, x);
+            load_pairs<DT, V>(reinterpret_cast<const DT*>(sx + xb) + c, d);
+            load_pairs<float, V>(gs + c, gm);
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+              o[j] = mul2(fma2(mul2(add2(x[j], nm), r2), c2, add2(mul2(d[j], gm[j]), c1)), r2);
+          } else {
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+              o[j] = mul2(fma2(h[i * H + j], c2, add2(g[i * H + j], c1)), r2);
+          }
+          store_pairs<XT, V>(dx + c, o);
+        }
+      }
+    }
+    mean = mean2;
+    rstd = rstd2;
+    prev = slot;
+    if (++slot == depth) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  griddep_launch_dependents();  // ln_bwd_sum_kernel may take its place; it waits for the sums
+  if (abort_flag && threadIdx.x == 0) atomicExch(status, kDevWaitTimeout);
+  float* out = a.partial + (int64_t)blockIdx.x * 2 * a.cols;
+  if constexpr (RB == 1) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (i * TR + t) * V;
+      if (c < a.cols) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          const float2 u = unpack2(sg[i * H + j]), w = unpack2(sb[i * H + j]);
+          *reinterpret_cast<float2*>(out + c + 2 * j) = u;
+          *reinterpret_cast<float2*>(out + a.cols + c + 2 * j) = w;
+        }
+      }
+    }
+  } else {
+    // the block's row groups, added in order; the ring has been read
+    float* acc = reinterpret_cast<float*>(dyn);
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < H; ++j)
+          *reinterpret_cast<float2*>(acc + sub * TR * NE + (i * TR + t) * V + 2 * j) =
+              unpack2(pass ? sb[i * H + j] : sg[i * H + j]);
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.cols; c += kBlock) {
+        float v = 0.0f;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) v += acc[r * TR * NE + c];
+        out[pass * a.cols + c] = v;
+      }
+    }
+  }
+}
+
 // Rows too wide for the registers: the column sums first (dx may overwrite dy
 // or x), then dx row by row.
 template <typename XT, typename DT>
@@ -357,8 +839,10 @@ __global__ void __launch_bounds__(512) ln_bwd_wide_rows_kernel(const LnBwd a) {
   }
 }
 
-// dgamma and dbeta from the blocks' sums: 32 columns a block, 8 threads a
-// column, each adding every eighth partial in order, the eight added in order.
+// dgamma and dbeta from the blocks' sums: 32 columns a block, 32 threads a
+// column, each adding every 32nd partial in order (their loads are all in
+// flight at once), the 32 added in a fixed tree. Launched as a programmatic
+// dependent, so its start overlaps the backward kernel's end.
 struct LnSum {
   const float* partial;
   void* dgamma;
@@ -369,21 +853,25 @@ struct LnSum {
   int accumulate;
 };
 
-__global__ void __launch_bounds__(256) ln_bwd_sum_kernel(const LnSum a) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) ln_bwd_sum_kernel(const LnSum a) {
+  __shared__ float red[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+  const int64_t col = (int64_t)blockIdx.x * 32 + tx;
+  griddep_wait();
   float v = 0.0f;
-  if (c < a.cols) {
-    const float* p = a.partial + (int64_t)blockIdx.y * a.cols + c;
-#pragma unroll 4
-    for (int k = ty; k < a.parts; k += 8) v += p[(int64_t)k * 2 * a.cols];
+  if (col < a.cols) {
+    const float* p = a.partial + (int64_t)blockIdx.y * a.cols + col;
+#pragma unroll 10
+    for (int k = ty; k < a.parts; k += 32) v += p[(int64_t)k * 2 * a.cols];
   }
   red[ty][tx] = v;
   __syncthreads();
-  if (ty != 0 || c >= a.cols) return;
+  // warp ty now takes column ty of the block: lane l holds partial sum l
+  v = red[tx][ty];
 #pragma unroll
-  for (int k = 1; k < 8; ++k) v += red[k][tx];
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int64_t c = (int64_t)blockIdx.x * 32 + ty;
+  if (tx != 0 || c >= a.cols) return;
   void* out = blockIdx.y ? a.dbeta : a.dgamma;
   if (a.grad_bf16) {
     __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out) + c;
@@ -396,56 +884,118 @@ __global__ void __launch_bounds__(256) ln_bwd_sum_kernel(const LnSum a) {
 
 // ------------------------------------------------------------------ dispatch
 // How a row is spread: the threads of a row by its width, so that a thread
-// holds at most 32 elements forward and 16 backward (where x, dy and two sums
-// per column are live).
+// holds 8 or 16 elements of a row.
 constexpr int64_t kFwdMaxCols = 16384;
-constexpr int64_t kBwdMaxCols = 8192;
+constexpr int64_t kBwdMaxCols = 8192;    // rows in registers
+constexpr int64_t kRingMaxCols = 16384;  // rows through shared memory
 
-template <typename XT, typename YT, int V, int TR, int NE>
-void fwd_launch(const LnFwd& a, cudaStream_t s) {
+template <typename XT, typename YT, int TR, int NE>
+void fwd_scalar(const LnFwd& a, cudaStream_t s) {
   constexpr int kBlock = TR <= 32 ? 128 : TR, RB = kBlock / TR;
-  ln_fwd_kernel<XT, YT, V, TR, NE><<<(unsigned)((a.rows + RB - 1) / RB), kBlock, 0, s>>>(a);
+  ln_fwd_kernel<XT, YT, 1, TR, NE><<<(unsigned)((a.rows + RB - 1) / RB), kBlock, 0, s>>>(a);
 }
 
-template <typename XT, typename YT, int V>
-void fwd_width(const LnFwd& a, cudaStream_t s) {
-  if (a.cols <= 64)
-    fwd_launch<XT, YT, V, 8, 8>(a, s);
-  else if (a.cols <= 256)
-    fwd_launch<XT, YT, V, 32, 8>(a, s);
-  else if (a.cols <= 1024)
-    fwd_launch<XT, YT, V, 128, 8>(a, s);
-  else if (a.cols <= 2048)
-    fwd_launch<XT, YT, V, 128, 16>(a, s);
-  else if (a.cols <= 4096)
-    fwd_launch<XT, YT, V, 256, 16>(a, s);
-  else if (a.cols <= 8192)
-    fwd_launch<XT, YT, V, 512, 16>(a, s);
-  else
-    fwd_launch<XT, YT, V, 512, 32>(a, s);
+template <typename XT, typename YT, int TR, int NE>
+void fwd_rows(const LnFwd& a, cudaStream_t s) {
+  constexpr int64_t kRows = ln_rows_block(TR) / TR;
+  ln_fwd_rows_kernel<XT, YT, TR, NE>
+      <<<(unsigned)((a.rows + kRows - 1) / kRows), ln_rows_block(TR), 0, s>>>(a);
+}
+
+// Shared memory above 48 KB for a kernel, once per device (`done`: the devices
+// that have it).
+template <typename K>
+int raise_smem(K kernel, int device, std::mutex& mu, uint64_t& done) {
+  std::lock_guard<std::mutex> lock(mu);
+  if (device < 64 && (done >> device) & 1u) return MMN_OK;
+  MMN_CUDA_TRY(
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+  if (device < 64) done |= uint64_t(1) << device;
+  return MMN_OK;
 }
 
 template <typename XT, typename YT>
-void fwd_types(const LnFwd& a, bool vec, cudaStream_t s) {
-  constexpr int V = sizeof(XT) == 2 && sizeof(YT) == 2 ? 8 : 4;
+void fwd_width(const LnFwd& a, cudaStream_t s) {
+  if (a.cols <= 64)
+    fwd_rows<XT, YT, 8, 8>(a, s);
+  else if (a.cols <= 256)
+    fwd_rows<XT, YT, 32, 8>(a, s);
+  else if (a.cols <= 512)
+    fwd_rows<XT, YT, 32, 16>(a, s);
+  else if (a.cols <= 1024)
+    fwd_rows<XT, YT, 128, 8>(a, s);
+  else if (a.cols <= 2048)
+    fwd_rows<XT, YT, 128, 16>(a, s);
+  else if (a.cols <= 4096)
+    fwd_rows<XT, YT, 256, 16>(a, s);
+  else if (a.cols <= 8192)
+    fwd_rows<XT, YT, 512, 16>(a, s);
+  else
+    fwd_rows<XT, YT, 1024, 16>(a, s);
+}
+
+template <typename XT, typename YT, int TR, int NE>
+int ring_fwd_launch(const LnFwd& a, int sms, int device, cudaStream_t s) {
+  constexpr int RB = ln_ring_block(TR) / TR, kBlocks = ln_ring_blocks(TR);
+  static std::mutex mu;
+  static uint64_t done = 0;
+  auto* kernel = ln_fwd_ring_kernel<XT, YT, TR, NE>;
+  int* status = nullptr;
+  int rc;
+  if ((rc = raise_smem(kernel, device, mu, done)) != MMN_OK) return rc;
+  if ((rc = kernel_status_word(&status)) != MMN_OK) return rc;
+  const int64_t row = a.cols * (int64_t)sizeof(XT);
+  // more rows in flight than this cost bandwidth (16384 x 4096, 3 blocks an SM:
+  // 8 rows 51.2 us, 3 rows 48.6 us)
+  const int depth = (int)std::min<int64_t>(kFwdRing, (224 * 1024 / kBlocks - 4096) / (row * RB));
+  const int64_t grid = std::min<int64_t>((a.rows + RB - 1) / RB, (int64_t)sms * kBlocks);
+  kernel<<<(unsigned)grid, ln_ring_block(TR), depth * row * RB, s>>>(a, depth, status);
+  return MMN_OK;
+}
+
+template <typename XT, typename YT>
+int fwd_types(const LnFwd& a, bool vec, bool ring, int sms, int device, cudaStream_t s) {
+  if constexpr (sizeof(XT) == 2) {
+    if (ring) {
+      if (a.cols <= 512) return ring_fwd_launch<XT, YT, 32, 16>(a, sms, device, s);
+      if (a.cols <= 1024) return ring_fwd_launch<XT, YT, 32, 32>(a, sms, device, s);
+      if (a.cols <= 2048) return ring_fwd_launch<XT, YT, 64, 32>(a, sms, device, s);
+      if (a.cols <= 4096) return ring_fwd_launch<XT, YT, 128, 32>(a, sms, device, s);
+      if (a.cols <= 8192) return ring_fwd_launch<XT, YT, 256, 32>(a, sms, device, s);
+      return ring_fwd_launch<XT, YT, 512, 32>(a, sms, device, s);
+    }
+  }
   if (a.cols > kFwdMaxCols)
     ln_fwd_wide_kernel<XT, YT><<<(unsigned)a.rows, 512, 0, s>>>(a);
   else if (vec)
-    fwd_width<XT, YT, V>(a, s);
+    fwd_width<XT, YT>(a, s);
+  else if (a.cols <= 64)
+    fwd_scalar<XT, YT, 8, 8>(a, s);
+  else if (a.cols <= 256)
+    fwd_scalar<XT, YT, 32, 8>(a, s);
+  else if (a.cols <= 1024)
+    fwd_scalar<XT, YT, 128, 8>(a, s);
+  else if (a.cols <= 2048)
+    fwd_scalar<XT, YT, 128, 16>(a, s);
+  else if (a.cols <= 4096)
+    fwd_scalar<XT, YT, 256, 16>(a, s);
+  else if (a.cols <= 8192)
+    fwd_scalar<XT, YT, 512, 16>(a, s);
   else
-    fwd_width<XT, YT, 1>(a, s);
+    fwd_scalar<XT, YT, 512, 32>(a, s);
+  return MMN_OK;
 }
 
-// Threads per row of the backward kernel for a width.
+// Threads per row of the backward kernels for a width.
 int bwd_tr(int64_t cols) {
-  return cols <= 64 ? 8 : cols <= 512 ? 32 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
+  return cols <= 64 ? 8 : cols <= 256 ? 32 : cols <= 512 ? 64 : cols <= 2048 ? 128
+         : cols <= 4096 ? 256 : 512;
 }
 
 // Blocks of the backward kernel (partial sums to add): one per row group, at
-// most what the GPU holds at once. Wide rows: chunks of rows.
+// most what the GPU holds at once.
 int bwd_parts(int64_t rows, int64_t cols, int sms) {
   if (rows <= 0 || cols <= 0) return 0;
-  if (cols > kBwdMaxCols) return (int)std::min<int64_t>(rows, 64);
   const int tr = bwd_tr(cols), rb = ln_bwd_block(tr) / tr;
   return (int)std::min<int64_t>((rows + rb - 1) / rb, (int64_t)sms * ln_bwd_min_blocks(tr));
 }
@@ -461,7 +1011,9 @@ void bwd_width(const LnBwd& a, int parts, cudaStream_t s) {
     case 8:
       return bwd_launch<XT, DT, V, 8, 8>(a, parts, s);
     case 32:
-      return bwd_launch<XT, DT, V, 32, 16>(a, parts, s);
+      return bwd_launch<XT, DT, V, 32, 8>(a, parts, s);
+    case 64:
+      return bwd_launch<XT, DT, V, 64, 8>(a, parts, s);
     case 128:
       return bwd_launch<XT, DT, V, 128, 16>(a, parts, s);
     case 256:
@@ -471,9 +1023,50 @@ void bwd_width(const LnBwd& a, int parts, cudaStream_t s) {
   }
 }
 
+// Rows in flight per group with bulk copies: what an SM's 224 KB hold, shared by
+// the blocks on it.
 template <typename XT, typename DT>
-void bwd_types(const LnBwd& a, int parts, bool vec, cudaStream_t s) {
+int ring_depth(int64_t cols, int* smem) {
+  const int tr = bwd_tr(cols), rb = ln_bwd_block(tr) / tr;
+  const int64_t row = cols * (int64_t)(sizeof(XT) + sizeof(DT));
+  const int64_t gamma = cols > kBwdMaxCols ? cols * 4 : 0;
+  const int64_t budget = 224 * 1024 / ln_bwd_min_blocks(tr) - 4096 - gamma;
+  const int depth = (int)std::min<int64_t>(kRingMax, budget / (row * rb));
+  // (the closing sums of several groups use the same memory)
+  const int64_t acc = rb > 1 ? (int64_t)rb * tr * 8 * 4 : 0;
+  *smem = (int)std::max<int64_t>(gamma + depth * row * rb, acc);
+  return depth;
+}
+
+template <typename XT, typename DT, int V, int TR, int NE>
+int ring_launch(const LnBwd& a, int parts, int depth, int smem, int* status, int device,
+                cudaStream_t s) {
+  static std::mutex mu;
+  static uint64_t done = 0;
+  auto* kernel = ln_bwd_ring_kernel<XT, DT, V, TR, NE>;
+  const int rc = raise_smem(kernel, device, mu, done);
+  if (rc != MMN_OK) return rc;
+  kernel<<<parts, ln_bwd_block(TR), smem, s>>>(a, depth, status);
+  return MMN_OK;
+}
+
+template <typename XT, typename DT>
+int bwd_types(const LnBwd& a, int parts, bool vec, bool ring, int device, cudaStream_t s) {
   constexpr int V = sizeof(XT) == 2 && sizeof(DT) == 2 ? 8 : 4;
+  int smem = 0;
+  const int depth = ring && a.cols > 64 && a.cols <= kRingMaxCols ? ring_depth<XT, DT>(a.cols, &smem) : 0;
+  if (depth >= 2) {
+    int* status = nullptr;
+    const int rc = kernel_status_word(&status);
+    if (rc != MMN_OK) return rc;
+    if (a.cols <= 256) return ring_launch<XT, DT, V, 32, 8>(a, parts, depth, smem, status, device, s);
+    if (a.cols <= 512) return ring_launch<XT, DT, V, 64, 8>(a, parts, depth, smem, status, device, s);
+    if (a.cols <= 1024) return ring_launch<XT, DT, V, 128, 8>(a, parts, depth, smem, status, device, s);
+    if (a.cols <= 2048) return ring_launch<XT, DT, V, 128, 16>(a, parts, depth, smem, status, device, s);
+    if (a.cols <= 4096) return ring_launch<XT, DT, V, 256, 16>(a, parts, depth, smem, status, device, s);
+    if (a.cols <= 8192) return ring_launch<XT, DT, V, 512, 16>(a, parts, depth, smem, status, device, s);
+    return ring_launch<XT, DT, V, 512, 32>(a, parts, depth, smem, status, device, s);
+  }
   if (a.cols > kBwdMaxCols) {
     const int64_t chunk = (a.rows + parts - 1) / parts;
     ln_bwd_wide_cols_kernel<XT, DT>
@@ -484,6 +1077,7 @@ void bwd_types(const LnBwd& a, int parts, bool vec, cudaStream_t s) {
   } else {
     bwd_width<XT, DT, 1>(a, parts, s);
   }
+  return MMN_OK;
 }
 
 bool bad_dtype(int d) { return d != MMN_DTYPE_F32 && d != MMN_DTYPE_BF16; }
@@ -553,21 +1147,28 @@ extern "C" int mmn_layer_norm(const void* x, int64_t x_ld, int x_dtype, const vo
     if (q.p && (rc = check_device_elems(q.p, esize(q.dt), device, q.n)) != MMN_OK) return rc;
   LnFwd a{x, gamma, beta, y, mean, rstd, rows > 1 ? x_ld : cols, rows > 1 ? y_ld : cols, rows, cols,
           eps, param_dtype == MMN_DTYPE_BF16};
-  const int v = x_dtype == MMN_DTYPE_BF16 && y_dtype == MMN_DTYPE_BF16 ? 8 : 4;
+  const int v = 4;
   const bool vec = cols % v == 0 && vec_rows(x, a.x_ld, esize(x_dtype), v) &&
                    vec_rows(y, a.y_ld, esize(y_dtype), v) &&
                    vec_rows(gamma, cols, esize(param_dtype), v) &&
                    vec_rows(beta, cols, esize(param_dtype), v);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool xb = x_dtype == MMN_DTYPE_BF16, yb = y_dtype == MMN_DTYPE_BF16;
+  // (with fewer rows a block of its own per row is quicker)
+  const bool ring = xb && vec && cols > 64 && cols <= kFwdMaxCols && rows >= 8 * (int64_t)sms &&
+                    cols % 8 == 0 && vec_rows(x, a.x_ld, 2, 8) &&
+                    vec_rows(y, a.y_ld, esize(y_dtype), 8) &&
+                    vec_rows(gamma, cols, esize(param_dtype), 8) &&
+                    vec_rows(beta, cols, esize(param_dtype), 8);
   if (xb && yb)
-    fwd_types<__nv_bfloat16, __nv_bfloat16>(a, vec, s);
+    rc = fwd_types<__nv_bfloat16, __nv_bfloat16>(a, vec, ring, sms, device, s);
   else if (xb)
-    fwd_types<__nv_bfloat16, float>(a, vec, s);
+    rc = fwd_types<__nv_bfloat16, float>(a, vec, ring, sms, device, s);
   else if (yb)
-    fwd_types<float, __nv_bfloat16>(a, vec, s);
+    rc = fwd_types<float, __nv_bfloat16>(a, vec, ring, sms, device, s);
   else
-    fwd_types<float, float>(a, vec, s);
+    rc = fwd_types<float, float>(a, vec, ring, sms, device, s);
+  if (rc != MMN_OK) return rc;
   MMN_CUDA_TRY(cudaGetLastError());
   return MMN_OK;
 }
@@ -631,21 +1232,35 @@ extern "C" int mmn_layer_norm_backward(const void* dy, int64_t dy_ld, int dy_dty
                      vec_rows(dy, a.dy_ld, esize(dy_dtype), v) &&
                      vec_rows(dx, a.dx_ld, esize(x_dtype), v) &&
                      vec_rows(gamma, cols, esize(param_dtype), v);
+    // dx in place of an input that a later row still reads is no hazard: a row is
+    // read before its dx is written, and no other row is touched
+    const bool ring = vec && (cols * esize(x_dtype)) % 16 == 0 && (cols * esize(dy_dtype)) % 16 == 0 &&
+                      vec_rows(x, a.x_ld, esize(x_dtype), 16) &&
+                      vec_rows(dy, a.dy_ld, esize(dy_dtype), 16);
     const bool xb = x_dtype == MMN_DTYPE_BF16, db = dy_dtype == MMN_DTYPE_BF16;
     if (xb && db)
-      bwd_types<__nv_bfloat16, __nv_bfloat16>(a, parts, vec, s);
+      rc = bwd_types<__nv_bfloat16, __nv_bfloat16>(a, parts, vec, ring, device, s);
     else if (xb)
-      bwd_types<__nv_bfloat16, float>(a, parts, vec, s);
+      rc = bwd_types<__nv_bfloat16, float>(a, parts, vec, ring, device, s);
     else if (db)
-      bwd_types<float, __nv_bfloat16>(a, parts, vec, s);
+      rc = bwd_types<float, __nv_bfloat16>(a, parts, vec, ring, device, s);
     else
-      bwd_types<float, float>(a, parts, vec, s);
+      rc = bwd_types<float, float>(a, parts, vec, ring, device, s);
+    if (rc != MMN_OK) return rc;
     MMN_CUDA_TRY(cudaGetLastError());
   }
   if (parts == 0 && accumulate) return MMN_OK;  // no rows: the sums are zero
   LnSum su{static_cast<const float*>(workspace), dgamma, dbeta, cols, parts,
            grad_dtype == MMN_DTYPE_BF16, accumulate != 0};
-  ln_bwd_sum_kernel<<<dim3((unsigned)((cols + 31) / 32), 2), 256, 0, s>>>(su);
-  MMN_CUDA_TRY(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((cols + 31) / 32), 2, 1);
+  cfg.blockDim = dim3(1024, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, ln_bwd_sum_kernel, su));
   return MMN_OK;
 }

@@ -375,10 +375,6 @@ __global__ void __launch_bounds__(256) mx_zero_kernel(void* out, int64_t ld, int
   }
 }
 
-// A kernel of this file that gave up a bounded wait leaves its code here, per
-// device (mmn_kernel_status).
-__device__ int g_mx_status;
-
 // -------------------------------------------------------------------- host
 constexpr int64_t kMaxDim = int64_t(1) << 30;
 
@@ -486,11 +482,6 @@ int launch_quantize(const void* x, int64_t ld, int dtype, int64_t rows, int64_t 
   return MMN_OK;
 }
 
-int status_word(int** p) {
-  MMN_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(p), g_mx_status));
-  return MMN_OK;
-}
-
 template <int BN, bool TRANS>
 int launch_gemm(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, cudaStream_t s) {
   CUtensorMap ta, tb;
@@ -595,7 +586,7 @@ int product(const mmn_mxfp4* a, const mmn_mxfp4* b, void* out, int64_t ld, int d
   g.out_bf16 = dtype == MMN_DTYPE_BF16;
   g.accumulate = accumulate != 0;
   g.vec = vec_rows(out, ld, esize(dtype), 8);
-  int rc = status_word(&g.status);
+  int rc = kernel_status_word(&g.status);
   if (rc != MMN_OK) return rc;
   // Few rows: the other operand's rows fill the 128 lanes.
   if (a->rows <= 16) return launch_gemm<16, true>(b, a, g, s);
@@ -770,7 +761,7 @@ extern "C" int mmn_kernel_status(int device, void* stream) {
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
   DeviceGuard guard(device);
   int* word = nullptr;
-  if ((rc = status_word(&word)) != MMN_OK) return rc;
+  if ((rc = kernel_status_word(&word)) != MMN_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int st = 0;
   MMN_CUDA_TRY(cudaMemcpyAsync(&st, word, sizeof(int), cudaMemcpyDeviceToHost, s));

@@ -11,8 +11,8 @@ step of the output's type (2^-24 fp32, 2^-8 bf16 relative to the value):
   dx       r [3u|g| + (D + 4) u mean|g| + |h| ((D + 4) u mean|g h| + mean(|g| err h))
               + |c2| err(h) + 4u (|g| + |c1| + |h c2|)] + H |dx|
   dgamma   a sum over rows in which each passes through at most R additions (the
-           rows of one block, its 32 row groups, an eighth of the blocks' sums,
-           8): (R + 3) u sum|dy h| + sum |dy| err(h) + H |dgamma|
+           rows of one block, its 32 row groups, a part of the blocks' sums, the
+           parts): (R + 3) u sum|dy h| + sum |dy| err(h) + H |dgamma|
   dbeta    R u sum|dy| + H |dbeta|
 The backward pass takes mean and rstd as inputs: there err(h) is
 r u |x - mean| + 2 u |h|.
