@@ -27,21 +27,6 @@ namespace mmn {
 namespace {
 
 // -------------------------------------------------------------- conversions
-// Four e2m1 bytes from eight fp32 values (v[0] in the lowest four bits), to
-// nearest even, saturating.
-__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
-      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
-      : "=r"(r)
-      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
-  return r;
-}
-
 // The values of four 4-bit codes, through bf16, which holds them: the byte
 // permutation looks up the high and the low byte of 0, 1/2, 1, 3/2, 2, 3, 4, 6.
 __device__ __forceinline__ void e2m1x4_values(uint32_t w, float* v) {
@@ -56,18 +41,6 @@ __device__ __forceinline__ void e2m1x4_values(uint32_t w, float* v) {
   v[1] = __uint_as_float(p0 & 0xFFFF0000u);
   v[2] = __uint_as_float(p1 << 16);
   v[3] = __uint_as_float(p1 & 0xFFFF0000u);
-}
-
-// Scale byte of a block from the bits of its largest magnitude as fp32 (taken
-// as an integer maximum, so that a NaN is not lost in it).
-__device__ __forceinline__ uint32_t mx_scale(uint32_t amax_bits) {
-  const uint32_t e = amax_bits >> 23;
-  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
-}
-
-// 1 / scale (2^(127 - byte)); for a block without values any finite number.
-__device__ __forceinline__ float mx_inv_scale(uint32_t s) {
-  return s == 255u ? 1.0f : __uint_as_float((254u - s) << 23);
 }
 
 __device__ __forceinline__ float mx_scale_value(uint32_t s) {
@@ -431,6 +404,14 @@ Range scales_range(const mmn_mxfp4* q) {
   return {q->scales, q->cols ? scale_bytes(q->rows, q->cols) : 0};
 }
 
+template <int BN, int SRC>
+int split_setup() {
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_split_kernel<BN, SRC>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    MxSplit<BN, SRC>::kSmemBytes));
+  return MMN_OK;
+}
+
 // Shared memory of the kernels above 48 KB, once per device.
 int kernel_setup(int device) {
   static std::mutex mu;
@@ -439,11 +420,13 @@ int kernel_setup(int device) {
   if (device < 64 && (done >> device) & 1u) return MMN_OK;
   const auto smem = cudaFuncAttributeMaxDynamicSharedMemorySize;
   MMN_CUDA_TRY(cudaFuncSetAttribute(mx_quantize_kernel<float>, smem, MxTile<float>::kSmem));
-  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<16, true>, smem, MxShape<16>::kSmemBytes));
-  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<32, true>, smem, MxShape<32>::kSmemBytes));
-  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<64, true>, smem, MxShape<64>::kSmemBytes));
-  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<128, true>, smem, MxShape<128>::kSmemBytes));
-  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_kernel<128, false>, smem, MxShape<128>::kSmemBytes));
+  int rc;
+  if ((rc = split_setup<16, 0>()) != MMN_OK || (rc = split_setup<32, 0>()) != MMN_OK ||
+      (rc = split_setup<64, 0>()) != MMN_OK || (rc = split_setup<128, 0>()) != MMN_OK ||
+      (rc = split_setup<16, 1>()) != MMN_OK || (rc = split_setup<32, 1>()) != MMN_OK ||
+      (rc = split_setup<64, 1>()) != MMN_OK || (rc = split_setup<16, 2>()) != MMN_OK ||
+      (rc = split_setup<32, 2>()) != MMN_OK || (rc = split_setup<64, 2>()) != MMN_OK)
+    return rc;
   MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_pair_kernel, smem, MxPair::kSmemBytes));
   if (device < 64) done |= uint64_t(1) << device;
   return MMN_OK;
@@ -482,24 +465,43 @@ int launch_quantize(const void* x, int64_t ld, int dtype, int64_t rows, int64_t 
   return MMN_OK;
 }
 
-template <int BN, bool TRANS>
-int launch_gemm(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, cudaStream_t s) {
-  CUtensorMap ta, tb;
-  std::string err = encode_byte_rows(&ta, a->codes, code_pitch(a->cols), a->rows, 128);
-  if (err.empty()) err = encode_byte_rows(&tb, b->codes, code_pitch(b->cols), b->rows, BN);
+// out = A W^T with A's rows on the N side: A as 4-bit codes (SRC 0) or as rows to
+// round (SRC 1: bf16, 2: fp32).
+template <int BN, int SRC>
+int launch_split(const mmn_mxfp4* a, const MxRows& rows, const mmn_mxfp4* w, int64_t n,
+                 MxGemmArgs& g, int sms, cudaStream_t s) {
+  CUtensorMap tw, tx;
+  std::string err = encode_byte_rows(&tw, w->codes, code_pitch(w->cols), w->rows, 128);
+  if (SRC != 0)
+    tx = tw;
+  else if (err.empty())
+    err = encode_byte_rows(&tx, a->codes, code_pitch(a->cols), a->rows, BN);
   if (!err.empty()) return fail(MMN_E_CUDA, err);
-  g.sfa = static_cast<const uint8_t*>(a->scales);
-  g.sfb = static_cast<const uint8_t*>(b->scales);
-  g.ka = (int)scale_blocks(a->cols);
-  g.M = (int)a->rows;
-  g.N = (int)b->rows;
-  g.num_kb = (int)((a->cols + 255) / 256);
-  g.rt_b = (int)((b->rows + 127) / 128);
-  g.tiles_n = (int)((b->rows + BN - 1) / BN);
-  const int64_t tiles = (int64_t)((a->rows + 127) / 128) * g.tiles_n;
-  if (tiles > (int64_t(1) << 31) - 1) return fail(MMN_E_SHAPE, "product too large");
-  mx_gemm_kernel<BN, TRANS><<<(unsigned)tiles, 192, MxShape<BN>::kSmemBytes, s>>>(ta, tb, g);
-  MMN_CUDA_TRY(cudaGetLastError());
+  g.sfa = static_cast<const uint8_t*>(w->scales);
+  g.sfb = SRC == 0 ? static_cast<const uint8_t*>(a->scales) : nullptr;
+  g.ka = (int)scale_blocks(w->cols);
+  g.M = (int)w->rows;
+  g.N = (int)n;
+  g.num_kb = (int)((w->cols + 255) / 256);
+  g.tiles_n = (int)((n + BN - 1) / BN);
+  const int64_t tiles = (w->rows + 127) / 128 * g.tiles_n;
+  // Split K while a split leaves no CTA without an SM: a cluster of 2, 4 or 8 CTAs
+  // with at least one stage of K each.
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= sms && splits * 2 <= g.num_kb) splits *= 2;
+  if (tiles * splits > (int64_t(1) << 31) - 1) return fail(MMN_E_SHAPE, "product too large");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * splits), 1, 1);
+  cfg.blockDim = dim3(MxSplit<BN, SRC>::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = MxSplit<BN, SRC>::kSmemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_split_kernel<BN, SRC>, tw, tx, g, rows, splits));
   return MMN_OK;
 }
 
@@ -570,31 +572,52 @@ int launch_gemm_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int 
   return MMN_OK;
 }
 
+int zero_out(void* out, int64_t ld, int64_t rows, int64_t cols, int dtype, cudaStream_t s) {
+  mx_zero_kernel<<<256, 256, 0, s>>>(out, ld, rows, cols, dtype == MMN_DTYPE_BF16);
+  MMN_CUDA_TRY(cudaGetLastError());
+  return MMN_OK;
+}
+
+int gemm_out(MxGemmArgs* g, void* out, int64_t ld, int dtype, int accumulate) {
+  g->out = out;
+  g->ld = ld;
+  g->out_bf16 = dtype == MMN_DTYPE_BF16;
+  g->accumulate = accumulate != 0;
+  g->vec = vec_rows(out, ld, esize(dtype), 8);
+  return kernel_status_word(&g->status);
+}
+
 // out (a.rows x b.rows) = A B^T, on checked arguments.
 int product(const mmn_mxfp4* a, const mmn_mxfp4* b, void* out, int64_t ld, int dtype,
             int accumulate, int sms, cudaStream_t s) {
   if (a->rows == 0 || b->rows == 0) return MMN_OK;
-  if (a->cols == 0) {
-    if (accumulate) return MMN_OK;
-    mx_zero_kernel<<<256, 256, 0, s>>>(out, ld, a->rows, b->rows, dtype == MMN_DTYPE_BF16);
-    MMN_CUDA_TRY(cudaGetLastError());
-    return MMN_OK;
-  }
+  if (a->cols == 0) return accumulate ? MMN_OK : zero_out(out, ld, a->rows, b->rows, dtype, s);
   MxGemmArgs g{};
-  g.out = out;
-  g.ld = ld;
-  g.out_bf16 = dtype == MMN_DTYPE_BF16;
-  g.accumulate = accumulate != 0;
-  g.vec = vec_rows(out, ld, esize(dtype), 8);
-  int rc = kernel_status_word(&g.status);
+  int rc = gemm_out(&g, out, ld, dtype, accumulate);
   if (rc != MMN_OK) return rc;
-  // Few rows: the other operand's rows fill the 128 lanes.
-  if (a->rows <= 16) return launch_gemm<16, true>(b, a, g, s);
-  if (a->rows <= 32) return launch_gemm<32, true>(b, a, g, s);
-  if (a->rows <= 64) return launch_gemm<64, true>(b, a, g, s);
-  if (a->rows <= 128) return launch_gemm<128, true>(b, a, g, s);
   if (a->rows > 256 && b->rows > 256) return launch_gemm_pair(a, b, g, sms, s);
-  return launch_gemm<128, false>(a, b, g, s);
+  const MxRows none{};
+  if (a->rows <= 16) return launch_split<16, 0>(a, none, b, a->rows, g, sms, s);
+  if (a->rows <= 32) return launch_split<32, 0>(a, none, b, a->rows, g, sms, s);
+  if (a->rows <= 64) return launch_split<64, 0>(a, none, b, a->rows, g, sms, s);
+  return launch_split<128, 0>(a, none, b, a->rows, g, sms, s);
+}
+
+// out = q(x) W^T for at most MMN_MXFP4_DIRECT_ROWS rows of x, on checked arguments.
+int direct_linear(const void* x, int64_t ld, int dtype, int64_t rows, const mmn_mxfp4* w, void* out,
+                  int64_t out_ld, int out_dtype, int sms, cudaStream_t s) {
+  MxGemmArgs g{};
+  int rc = gemm_out(&g, out, out_ld, out_dtype, 0);
+  if (rc != MMN_OK) return rc;
+  const MxRows r{x, ld, (int)w->cols, vec_rows(x, ld, esize(dtype), 16)};
+  if (dtype == MMN_DTYPE_BF16) {
+    if (rows <= 16) return launch_split<16, 1>(nullptr, r, w, rows, g, sms, s);
+    if (rows <= 32) return launch_split<32, 1>(nullptr, r, w, rows, g, sms, s);
+    return launch_split<64, 1>(nullptr, r, w, rows, g, sms, s);
+  }
+  if (rows <= 16) return launch_split<16, 2>(nullptr, r, w, rows, g, sms, s);
+  if (rows <= 32) return launch_split<32, 2>(nullptr, r, w, rows, g, sms, s);
+  return launch_split<64, 2>(nullptr, r, w, rows, g, sms, s);
 }
 
 int check_out(const void* out, int64_t ld, int dtype, int64_t rows, int64_t cols,
@@ -723,19 +746,24 @@ extern "C" int mmn_mxfp4_matmul(const mmn_mxfp4* a, const mmn_mxfp4* b, void* ou
 extern "C" int mmn_mxfp4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t rows,
                                 const mmn_mxfp4* w, const mmn_mxfp4* xq, void* out, int64_t out_ld,
                                 int out_dtype, int device, void* stream) {
-  if (!w || !xq) return fail(MMN_E_INVALID, "null matrix");
+  if (!w) return fail(MMN_E_INVALID, "null matrix");
   if (bad_dtype(x_dtype) || bad_dtype(out_dtype)) return fail(MMN_E_INVALID, "unknown dtype");
   int rc, sms = 0;
   if ((rc = check_dims(rows, w->cols)) != MMN_OK) return rc;
-  if (xq->rows != rows || xq->cols != w->cols)
-    return fail(MMN_E_SHAPE, "xq is not a rows x w.cols matrix");
-  if ((rc = check_mx(w, "w")) != MMN_OK || (rc = check_mx(xq, "xq")) != MMN_OK) return rc;
   const int64_t cols = w->cols;
+  const bool direct = rows <= MMN_MXFP4_DIRECT_ROWS;
+  if (!direct && !xq) return fail(MMN_E_INVALID, "xq is needed for this many rows");
+  if (xq && (xq->rows != rows || xq->cols != cols))
+    return fail(MMN_E_SHAPE, "xq is not a rows x w.cols matrix");
+  if ((rc = check_mx(w, "w")) != MMN_OK) return rc;
+  if (xq && (rc = check_mx(xq, "xq")) != MMN_OK) return rc;
   const bool empty = rows == 0 || cols == 0;
   if (!empty && !x) return fail(MMN_E_INVALID, "null pointer");
   if (rows > 1 && x_ld < cols) return fail(MMN_E_INVALID, "a row pitch is smaller than cols");
+  const Range none{nullptr, 0};
   const Range in[] = {matrix_range(x, rows > 1 ? x_ld : cols, rows, cols, esize(x_dtype)),
-                      codes_range(w), scales_range(w), codes_range(xq), scales_range(xq)};
+                      codes_range(w), scales_range(w), xq ? codes_range(xq) : none,
+                      xq ? scales_range(xq) : none};
   for (int i = 0; i < 3; ++i)
     if (ranges_meet(in[i], in[3]) || ranges_meet(in[i], in[4]))
       return fail(MMN_E_INVALID, "xq overlaps an input");
@@ -746,14 +774,16 @@ extern "C" int mmn_mxfp4_linear(const void* x, int64_t x_ld, int x_dtype, int64_
   DeviceGuard guard(device);
   if (cols && (rc = check_device_elems(x, esize(x_dtype), device, "x")) != MMN_OK) return rc;
   if ((rc = check_mx_device(w, device, "w")) != MMN_OK) return rc;
-  if ((rc = check_mx_device(xq, device, "xq")) != MMN_OK) return rc;
+  if (!direct && (rc = check_mx_device(xq, device, "xq")) != MMN_OK) return rc;
   if ((rc = check_device_elems(out, esize(out_dtype), device, "out")) != MMN_OK) return rc;
   if ((rc = kernel_setup(device)) != MMN_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cols && (rc = launch_quantize(x, rows > 1 ? x_ld : cols, x_dtype, rows, cols, xq, nullptr,
-                                    s)) != MMN_OK)
-    return rc;
-  return product(xq, w, out, rows > 1 ? out_ld : w->rows, out_dtype, 0, sms, s);
+  const int64_t ld = rows > 1 ? x_ld : cols, old = rows > 1 ? out_ld : w->rows;
+  if (cols == 0) return zero_out(out, old, rows, w->rows, out_dtype, s);
+  if (direct)
+    return direct_linear(x, ld, x_dtype, rows, w, out, old, out_dtype, sms, s);
+  if ((rc = launch_quantize(x, ld, x_dtype, rows, cols, xq, nullptr, s)) != MMN_OK) return rc;
+  return product(xq, w, out, old, out_dtype, 0, sms, s);
 }
 
 extern "C" int mmn_kernel_status(int device, void* stream) {

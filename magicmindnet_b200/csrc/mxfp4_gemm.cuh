@@ -18,12 +18,11 @@
 namespace mmn {
 
 struct MxGemmArgs {
-  const uint8_t* sfa;  // scale blocks of the operand on the 128-row side
-  const uint8_t* sfb;  // scale blocks of the other operand
+  const uint8_t* sfa;  // split kernel: scale blocks of the operand on the 128 lanes
+  const uint8_t* sfb;  // ... and of the other one
   int ka;              // scale blocks along K of one 128-row tile (even)
-  int M, N;            // rows of the two operands (128-row side first)
+  int M, N;            // rows of the two operands (the one on the lanes first)
   int num_kb;          // stages of 256 along K
-  int rt_b;            // 128-row tiles of the second operand
   int tiles_n;
   void* out;
   long long ld;        // elements between rows of out
@@ -34,27 +33,371 @@ struct MxGemmArgs {
   int* status;
 };
 
-template <int BN>
-struct MxShape {
+// -------------------------------------------------------- block conversions
+// Four e2m1 bytes from eight fp32 values (v[0] in the lowest four bits), to
+// nearest even, saturating.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// Scale byte of a block from the bits of its largest magnitude as fp32 (taken
+// as an integer maximum, so that a NaN is not lost in it).
+__device__ __forceinline__ uint32_t mx_scale(uint32_t amax_bits) {
+  const uint32_t e = amax_bits >> 23;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+
+// 1 / scale (2^(127 - byte)); for a block without values any finite number.
+__device__ __forceinline__ float mx_inv_scale(uint32_t s) {
+  return s == 255u ? 1.0f : __uint_as_float((254u - s) << 23);
+}
+
+// The codes of one block of 32 values; its scale byte in *scale.
+__device__ __forceinline__ uint4 mx_block(const float (&w)[32], uint32_t* scale) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(w[i]) & 0x7FFFFFFFu);
+  const uint32_t s = mx_scale(m);
+  const float inv = mx_inv_scale(s);
+  uint32_t q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = w[i * 8 + k] * inv;
+    q[i] = e2m1x8(v);
+  }
+  *scale = s;
+  return make_uint4(q[0], q[1], q[2], q[3]);
+}
+
+// ------------------------------------------------------ few rows, split along K
+// out^T tiles: 128 rows of B (columns of out) on the TMEM lanes, BN rows of A
+// (rows of out) as the N side. With few tiles the GPU would idle and the weight
+// stream would be short of loads in flight, so a cluster of up to 8 CTAs shares a
+// tile, each taking a part of K; the partial tiles are added in rank order
+// through distributed shared memory (the same result in every run).
+//
+// SRC = 0: A comes as 4-bit codes by TMA. SRC = 1 / 2: A is bf16 / fp32 and each CTA
+// rounds its part of K to 4 bits in shared memory while the weights' first
+// stages are on their way: a token costs one launch, and no scratch. BN below 128
+// takes one tile of A's rows (its scales then start at a block's first row).
+template <int BN, int SRC>
+struct MxSplit {
   static constexpr int kABytes = 128 * 128;
   static constexpr int kBBytes = BN * 128;
-  static constexpr int kTileBytes = kABytes + kBBytes;
-  static constexpr int kSfbTiles = (BN + 127) / 128;
-  static constexpr int kSfBytes = 1024 * (1 + kSfbTiles);
+  static constexpr int kTileBytes = kABytes + (SRC == 0 ? kBBytes : 0);
+  static constexpr int kSfBytes = SRC == 0 ? 2048 : 1024;
   static constexpr int kStageBytes = kTileBytes + kSfBytes;
-  static constexpr int kStagesMax = 220000 / kStageBytes;
-  static constexpr int kStages = kStagesMax < 8 ? kStagesMax : 8;
+  static constexpr int kStages = 212000 / kStageBytes < 8 ? 212000 / kStageBytes : 8;
+  // k blocks of A rounded at a time (SRC != 0)
+  static constexpr int kChunk = SRC == 0 ? 0 : (BN <= 32 ? 16 : 8);
+  static constexpr int kQBytes = kChunk * (kBBytes + 1024);
   static constexpr int kAccCols = BN < 32 ? 32 : BN;
-  static constexpr int kSfCols = 8 * (1 + kSfbTiles);  // TMEM columns of one stage's scales
-  static constexpr int kColsUsed = kAccCols + kStages * kSfCols;
-  static constexpr int kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128
-                                   : kColsUsed <= 256 ? 256 : 512;
-  static constexpr int kEpiBytes = 4 * 32 * 33 * 4;
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 512 + kEpiBytes;
-  static_assert(kColsUsed <= 512, "TMEM has 512 columns");
+  static constexpr int kColsUsed = kAccCols + kStages * 16;
+  static constexpr int kTmemCols = kColsUsed <= 128 ? 128 : 256;
+  static constexpr int kThreads = 64 + 256;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kQBytes + 512;
+  static_assert(kColsUsed <= 256, "TMEM columns");
   static_assert(kSmemBytes <= 232448, "shared memory per CTA");
-  static_assert(kStages >= 3, "pipeline depth");
+  static_assert(kStages * kTileBytes >= BN * 128 * 4, "the partial tile takes the stages' place");
 };
+
+struct MxRows {
+  const void* x;  // SRC != 0: the rows to round
+  long long ld;
+  int cols;
+  int vec;        // rows are 16-byte aligned
+};
+
+template <int BN, int SRC>
+__global__ void __launch_bounds__(320, 1)
+    mx_split_kernel(const __grid_constant__ CUtensorMap tm_w,
+                    const __grid_constant__ CUtensorMap tm_x, const MxGemmArgs args,
+                    const MxRows rows, int splits) {
+  using S = MxSplit<BN, SRC>;
+  constexpr int STAGES = S::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* tiles = smem;
+  uint8_t* qb = smem + STAGES * S::kTileBytes;   // rounded A: [chunk][BN x 128 B], swizzled
+  uint8_t* qs = qb + S::kChunk * S::kBBytes;     // its scales: [chunk][1024]
+  uint8_t* sfs = qs + S::kChunk * 1024;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sfs + STAGES * S::kSfBytes);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = full + 2 * STAGES;
+  uint64_t* bready = tfull + 1;  // a chunk of A is rounded
+  uint64_t* bfree = tfull + 2;   // its MMAs are done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 3);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tfull + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
+  const int tm = tile / args.tiles_n, tn = tile % args.tiles_n;
+  const int kb0 = (int)((long long)args.num_kb * rank / splits);
+  const int nkb = (int)((long long)args.num_kb * (rank + 1) / splits) - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    mbar_init(bready, 256);
+    mbar_init(bfree, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_w);
+    if (SRC == 0) tma_prefetch_desc(&tm_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, S::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    const bool one = elect_one();
+    uint32_t last = 0, issued = 0;  // parity of each stage's last load, stages used
+    for (int i = 0; i < nkb; ++i) {
+      const int s = i % STAGES;
+      const uint32_t ph = (i / STAGES) & 1;
+      if (!mbar_wait_warp(&empty[s], ph ^ 1u, abort_flag)) break;
+      if (one) {
+        const int kb = kb0 + i;
+        mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+        uint8_t* t = tiles + s * S::kTileBytes;
+        uint8_t* f = sfs + s * S::kSfBytes;
+        tma_load_3d(t, &tm_w, &full[s], kb * 128, tm * 128, 0);
+        bulk_load(f, args.sfa + ((long long)tm * args.ka + kb * 2) * 512, 1024, &full[s]);
+        if constexpr (SRC == 0) {
+          tma_load_3d(t + S::kABytes, &tm_x, &full[s], kb * 128, tn * BN, 0);
+          bulk_load(f + 1024, args.sfb + ((long long)(tn * BN / 128) * args.ka + kb * 2) * 512,
+                    1024, &full[s]);
+        }
+      }
+      issued |= 1u << s;
+      last = (last & ~(1u << s)) | (ph << s);
+    }
+    // every load lands before the CTA may exit
+    for (int s = 0; s < STAGES; ++s)
+      if (issued & (1u << s)) {
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(&full[s], (last >> s) & 1u))
+          if (global_timer_ns() - t0 > kWaitLimitNs) {
+            *abort_flag = 1;
+            break;
+          }
+      }
+  } else if (warp == 1) {
+    const bool one = elect_one();
+    bool ok = true;
+    for (int i = 0; i < nkb; ++i) {
+      const int s = i % STAGES;
+      if constexpr (SRC != 0) {
+        if (i % S::kChunk == 0 &&
+            !mbar_wait_warp(bready, (i / S::kChunk) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+      }
+      if (!mbar_wait_warp(&full[s], (i / STAGES) & 1, abort_flag)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (one) {
+        const uint32_t t = smem_u32(tiles + s * S::kTileBytes);
+        const uint32_t f = smem_u32(sfs + s * S::kSfBytes);
+        const int qi = SRC == 0 ? 0 : i % S::kChunk;
+        const uint32_t bt = SRC == 0 ? t + S::kABytes : smem_u32(qb + qi * S::kBBytes);
+        const uint32_t bf = SRC == 0 ? f + 1024 : smem_u32(qs + qi * 1024);
+        const uint32_t sa = tmem_base + S::kAccCols + s * 16, sb = sa + 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tc_cp_scales(sa + 4 * h, umma_desc_scales(f + 512 * h));
+          tc_cp_scales(sb + 4 * h, umma_desc_scales(bf + 512 * h));
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          constexpr uint32_t id0 = umma_idesc_mxf4(128, BN, 0), id1 = umma_idesc_mxf4(128, BN, 1);
+          const int h = kk >> 1;
+          tc_mma_mxf4(tmem_base, umma_desc_sw128(t + kk * 32, 16, 1024),
+                      umma_desc_sw128(bt + kk * 32, 16, 1024), (kk & 1) ? id1 : id0, sa + 4 * h,
+                      sb + 4 * h, (i | kk) != 0);
+        }
+        tc_commit(&empty[s]);
+        if (SRC != 0 && (i + 1) % (S::kChunk ? S::kChunk : 1) == 0) tc_commit(bfree);
+      }
+      __syncwarp();
+    }
+    if (one) {
+      tc_commit(tfull);  // after a time-out too: what was issued ends before TMEM is freed
+      if (!ok) {
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(tfull, 0))
+          if (global_timer_ns() - t0 > kWaitLimitNs) break;
+      }
+    }
+    __syncwarp();
+  } else {
+    const int et = threadIdx.x - 64;
+    if constexpr (SRC != 0) {
+      for (int c0 = 0; c0 < nkb; c0 += S::kChunk) {
+        const int nk = min(S::kChunk, nkb - c0);
+        if (c0 > 0) mbar_wait(bfree, (c0 / S::kChunk - 1) & 1, abort_flag);
+        // one block of 32 per turn; consecutive threads take consecutive blocks
+        for (int id = et; id < BN * nk * 8; id += 256) {
+          const int n = id / (nk * 8), b = id - n * (nk * 8), q = b >> 3, j = b & 7;
+          const int row = tn * BN + n, col = (kb0 + c0) * 256 + b * 32;
+          float w[32];
+          const int have = row < args.N ? min(32, rows.cols - col) : 0;
+          if constexpr (SRC == 1) {
+            const __nv_bfloat16* p =
+                static_cast<const __nv_bfloat16*>(rows.x) + (long long)row * rows.ld + col;
+            if (have == 32 && rows.vec) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+                const uint32_t e[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  w[i * 8 + 2 * k] = __uint_as_float(e[k] << 16);
+                  w[i * 8 + 2 * k + 1] = __uint_as_float(e[k] & 0xFFFF0000u);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) w[i] = i < have ? __bfloat162float(p[i]) : 0.0f;
+            }
+          } else {
+            const float* p = static_cast<const float*>(rows.x) + (long long)row * rows.ld + col;
+            if (have == 32 && rows.vec) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 u = reinterpret_cast<const float4*>(p)[i];
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) w[i] = i < have ? p[i] : 0.0f;
+            }
+          }
+          uint32_t sc;
+          const uint4 u = mx_block(w, &sc);
+          *reinterpret_cast<uint4*>(qb + q * S::kBBytes + n * 128 + ((j ^ (n & 7)) << 4)) = u;
+          qs[q * 1024 + (j >> 2) * 512 + (n & 31) * 16 + (n >> 5) * 4 + (j & 3)] = (uint8_t)sc;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(bready);
+      }
+    }
+    // the partial tile, [row of out][column of out], into the stages' place
+    const int sub = warp & 3, half = (warp - 2) >> 2;
+    const bool ready = mbar_wait(tfull, 0, abort_flag);
+    if (__all_sync(0xffffffffu, ready)) {  // tcgen05.ld is warp-collective
+      tc_fence_after();
+      float* part = reinterpret_cast<float*>(tiles);
+#pragma unroll 1
+      for (int ch = half; ch < (BN + 31) / 32; ch += 2) {
+        float v[32];
+        tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(sub * 32) << 16) + ch * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (BN >= 32 || j < BN) part[(ch * 32 + j) * 128 + sub * 32 + lane] = v[j];
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (splits > 1) cluster_sync_all();
+  {
+    // four consecutive columns of out per thread, the ranks' partials in order
+    const uint32_t part = smem_u32(tiles);
+    const int total = BN * 32, per = (total + splits - 1) / splits;
+    const int e1 = min(total, (rank + 1) * per);
+    for (int e = rank * per + threadIdx.x; e < e1; e += 320) {
+      const int j = e >> 5, r = (e & 31) * 4;
+      const int row = tn * BN + j, col = tm * 128 + r;
+      if (row >= args.N || col >= args.M) continue;
+      float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int k = 0; k < splits; ++k) {
+        const uint32_t addr = part + (j * 128 + r) * 4;
+        const float4 g = splits > 1 ? ld_cluster_f32x4(mapa_shared(addr, k))
+                                    : *reinterpret_cast<const float4*>(tiles + (j * 128 + r) * 4);
+        f.x += g.x;
+        f.y += g.y;
+        f.z += g.z;
+        f.w += g.w;
+      }
+      const long long i = (long long)row * args.ld + col;
+      const float v[4] = {f.x, f.y, f.z, f.w};
+      if (args.vec && col + 4 <= args.M) {
+        if (args.out_bf16) {
+          uint2* p = reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(args.out) + i);
+          float o[4] = {v[0], v[1], v[2], v[3]};
+          if (args.accumulate) {
+            const uint2 old = *p;
+            o[0] += __uint_as_float(old.x << 16);
+            o[1] += __uint_as_float(old.x & 0xFFFF0000u);
+            o[2] += __uint_as_float(old.y << 16);
+            o[3] += __uint_as_float(old.y & 0xFFFF0000u);
+          }
+          uint2 u;
+          *reinterpret_cast<__nv_bfloat162*>(&u.x) = __floats2bfloat162_rn(o[0], o[1]);
+          *reinterpret_cast<__nv_bfloat162*>(&u.y) = __floats2bfloat162_rn(o[2], o[3]);
+          *p = u;
+        } else {
+          float4* p = reinterpret_cast<float4*>(static_cast<float*>(args.out) + i);
+          if (args.accumulate) {
+            const float4 old = *p;
+            f.x += old.x;
+            f.y += old.y;
+            f.z += old.z;
+            f.w += old.w;
+          }
+          *p = f;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (col + k < args.M) {
+            if (args.out_bf16) {
+              __nv_bfloat16* p = static_cast<__nv_bfloat16*>(args.out) + i + k;
+              *p = __float2bfloat16_rn(args.accumulate ? v[k] + __bfloat162float(*p) : v[k]);
+            } else {
+              float* p = static_cast<float*>(args.out) + i + k;
+              *p = args.accumulate ? *p + v[k] : v[k];
+            }
+          }
+      }
+    }
+  }
+  if (splits > 1) {
+    __syncthreads();
+    cluster_sync_all();  // every rank has read this one's partial
+  }
+  if (*abort_flag && threadIdx.x == 0) atomicExch(args.status, kDevWaitTimeout);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, S::kTmemCols);
+  }
+}
 
 // Writes (or adds) a 32 x 32 block held one row per lane (v[j] = column j) to
 // out rows r0.., columns c0.., through the warp's 32 x 33 stage.
@@ -129,171 +472,6 @@ __device__ __forceinline__ void mx_store_block(const MxGemmArgs& a, long long r0
     }
   }
   __syncwarp();
-}
-
-// One 128 x BN tile per CTA. TRANS: the 128-row operand's rows are out's
-// columns. Warp 0 loads, warp 1 issues the copies and MMAs, warps 2-5 store.
-template <int BN, bool TRANS>
-__global__ void __launch_bounds__(192, 1)
-    mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_a,
-                   const __grid_constant__ CUtensorMap tm_b, const MxGemmArgs args) {
-  using S = MxShape<BN>;
-  constexpr int STAGES = S::kStages;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* tiles = smem;
-  uint8_t* sfs = smem + STAGES * S::kTileBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sfs + STAGES * S::kSfBytes);
-  uint64_t* empty = full + STAGES;
-  uint64_t* tfull = full + 2 * STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tfull + 2);
-  float* epi = reinterpret_cast<float*>(sfs + STAGES * S::kSfBytes + 512);
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tm = blockIdx.x / args.tiles_n, tn = blockIdx.x % args.tiles_n;
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    mbar_init(tfull, 1);
-    *abort_flag = 0;
-    fence_barrier_init();
-    tma_prefetch_desc(&tm_a);
-    tma_prefetch_desc(&tm_b);
-  }
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, S::kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-
-  if (warp == 0) {
-    if (lane == 0) {
-      const int row0 = tm * 128, col0 = tn * BN;
-      uint32_t last = 0, issued = 0;  // parity of each stage's last load, stages used
-      for (int kb = 0; kb < args.num_kb; ++kb) {
-        const int s = kb % STAGES;
-        const uint32_t ph = (kb / STAGES) & 1;
-        if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag)) break;
-        mbar_arrive_expect_tx(&full[s], S::kStageBytes);
-        uint8_t* t = tiles + s * S::kTileBytes;
-        tma_load_3d(t, &tm_a, &full[s], kb * 128, row0, 0);
-        tma_load_3d(t + S::kABytes, &tm_b, &full[s], kb * 128, col0, 0);
-        uint8_t* f = sfs + s * S::kSfBytes;
-        bulk_load(f, args.sfa + ((long long)tm * args.ka + kb * 2) * 512, 1024, &full[s]);
-#pragma unroll
-        for (int g = 0; g < S::kSfbTiles; ++g) {
-          // (a tile beyond the operand's last takes that one's scales: its
-          // elements are zero and its columns are not stored)
-          const int rt = min(col0 / 128 + g, args.rt_b - 1);
-          bulk_load(f + 1024 * (1 + g), args.sfb + ((long long)rt * args.ka + kb * 2) * 512, 1024,
-                    &full[s]);
-        }
-        issued |= 1u << s;
-        last = (last & ~(1u << s)) | (ph << s);
-      }
-      // every load lands before the CTA may exit
-      for (int s = 0; s < STAGES; ++s)
-        if (issued & (1u << s)) {
-          const uint64_t t0 = global_timer_ns();
-          while (!mbar_try_wait(&full[s], (last >> s) & 1u))
-            if (global_timer_ns() - t0 > kWaitLimitNs) {
-              *abort_flag = 1;
-              break;
-            }
-        }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int kb = 0; ok && kb < args.num_kb; ++kb) {
-        const int s = kb % STAGES;
-        if (!mbar_wait(&full[s], (kb / STAGES) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t t = smem_u32(tiles + s * S::kTileBytes);
-        const uint32_t f = smem_u32(sfs + s * S::kSfBytes);
-        // scale columns of the stage: [K half][4], then [K half][row group][4]
-        const uint32_t sa = tmem_base + S::kAccCols + s * S::kSfCols;
-        const uint32_t sb = sa + 8;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          tc_cp_scales(sa + 4 * h, umma_desc_scales(f + 512 * h));
-#pragma unroll
-          for (int g = 0; g < S::kSfbTiles; ++g)
-            tc_cp_scales(sb + (h * S::kSfbTiles + g) * 4,
-                         umma_desc_scales(f + 1024 * (1 + g) + 512 * h));
-        }
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          constexpr uint32_t id0 = umma_idesc_mxf4(128, BN, 0), id1 = umma_idesc_mxf4(128, BN, 1);
-          const int h = kk >> 1;
-          tc_mma_mxf4(tmem_base, umma_desc_sw128(t + kk * 32, 16, 1024),
-                      umma_desc_sw128(t + S::kABytes + kk * 32, 16, 1024), (kk & 1) ? id1 : id0,
-                      sa + 4 * h, sb + h * S::kSfbTiles * 4, (kb | kk) != 0);
-        }
-        tc_commit(&empty[s]);
-      }
-      tc_commit(tfull);  // also on the way out after a time-out: what was issued ends first
-      if (!ok) {
-        const uint64_t t0 = global_timer_ns();
-        while (!mbar_try_wait(tfull, 0))
-          if (global_timer_ns() - t0 > kWaitLimitNs) break;
-      }
-    }
-  } else {
-    const int sub = warp & 3;
-    const bool ready = mbar_wait(tfull, 0, abort_flag);
-    if (__all_sync(0xffffffffu, ready)) {  // tcgen05.ld is warp-collective
-      tc_fence_after();
-      float* tst = epi + (warp - 2) * 32 * 33;
-      const int m0 = tm * 128 + sub * 32;
-#pragma unroll 1
-      for (int ch = 0; ch < (BN + 31) / 32; ++ch) {
-        const int n0 = tn * BN + ch * 32;
-        float v[32];
-        tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(sub * 32) << 16) + ch * 32, v);
-        tmem_ld_wait();
-        const int mr = min(32, args.M - m0), nr = min(32, min(args.N, (tn + 1) * BN) - n0);
-        if (mr <= 0 || nr <= 0) continue;
-        if constexpr (TRANS) {
-          if (lane < mr) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < nr) {
-                const long long i = (long long)(n0 + j) * args.ld + m0 + lane;
-                if (args.out_bf16) {
-                  __nv_bfloat16* p = static_cast<__nv_bfloat16*>(args.out) + i;
-                  *p = __float2bfloat16_rn(args.accumulate ? v[j] + __bfloat162float(*p) : v[j]);
-                } else {
-                  float* p = static_cast<float*>(args.out) + i;
-                  *p = args.accumulate ? *p + v[j] : v[j];
-                }
-              }
-          }
-        } else {
-          mx_store_block(args, m0, n0, mr, nr, v, tst);
-        }
-      }
-      tc_fence_before();
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (*abort_flag && threadIdx.x == 0) atomicExch(args.status, kDevWaitTimeout);
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, S::kTmemCols);
-  }
 }
 
 // ---------------------------------------------------------------- CTA pairs

@@ -149,10 +149,10 @@ def mxfp4_linear(x, w, out=None, out_dtype=None):
         old = shape[-1]
     else:
         old = _out_pitch(out, shape, out_dtype, dev)
-    xq = Mxfp4Matrix(rows, cols, dev)
+    xq = None if rows <= N.MXFP4_DIRECT_ROWS else Mxfp4Matrix(rows, cols, dev)
     N.check(N.lib().mmn_mxfp4_linear(x.data_ptr(), ld, _dtype(x, "x"), rows, ctypes.byref(w._c),
-                                     ctypes.byref(xq._c), out.data_ptr(), old,
-                                     _dtype(out, "out"), dev.index, _stream(dev)))
+                                     None if xq is None else ctypes.byref(xq._c), out.data_ptr(),
+                                     old, _dtype(out, "out"), dev.index, _stream(dev)))
     return out
 
 

@@ -186,7 +186,8 @@ def test_non_finite_blocks(mmn, dtype):
 PRODUCTS = [(1, 1, 1), (1, 128, 256), (3, 300, 100), (16, 129, 64), (17, 517, 1030),
             (32, 128, 2048), (33, 1000, 96), (64, 77, 4096), (100, 640, 333), (128, 128, 256),
             (129, 1, 512), (200, 300, 31), (256, 256, 1024), (300, 513, 2500), (513, 257, 4128),
-            (1000, 31, 700), (2048, 16, 8192), (5, 2000, 14336), (777, 1030, 1999)]
+            (1000, 31, 700), (2048, 16, 8192), (5, 2000, 14336), (777, 1030, 1999),
+            (512, 512, 256), (520, 264, 1000), (2304, 2560, 300)]
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
@@ -198,6 +199,10 @@ def test_matmul(mmn, m, n, k, out):
     qa, qb = mmn.mxfp4_quantize(a), mmn.mxfp4_quantize(b)
     va, vb = plain_values(a), plain_values(b)
     check_product(mmn.mxfp4_matmul(qa, qb, out_dtype=T(out)), va, vb)
+    # added to what an aligned buffer holds
+    base = torch.randn(m, n, device="cuda").to(T(out))
+    got = mmn.mxfp4_matmul(qa, qb, out=base.clone(), accumulate=True)
+    check_product(got, va, vb, base)
     # into a slice of a wider buffer at an odd place, then added to it
     buf = torch.full((m, n + 11), 7.0, device="cuda", dtype=T(out))
     view = buf[:, 3:3 + n]
@@ -211,7 +216,9 @@ def test_matmul(mmn, m, n, k, out):
 
 @pytest.mark.parametrize("dtype,out", list(itertools.product(["f32", "bf16"], repeat=2)))
 @pytest.mark.parametrize("m,n,k", [(1, 256, 512), (1, 8192, 2048), (7, 100, 70), (48, 513, 1056),
-                                   (100, 77, 512), (300, 520, 1030), (640, 1024, 2048)])
+                                   (100, 77, 512), (300, 520, 1030), (640, 1024, 2048),
+                                   (16, 200, 9000), (17, 130, 33000), (33, 128, 17000),
+                                   (64, 19200, 2500), (20, 19001, 5000)])
 def test_linear(mmn, m, n, k, dtype, out):
     import torch
 

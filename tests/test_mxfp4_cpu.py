@@ -108,12 +108,23 @@ def test_linear_refusals(N):
 
     assert f() == gate(N)
     assert f(x=None) == bad and f(ld=63) == bad and f(xd=4) == bad and f(od=4) == bad
-    assert f(w=None) == bad and f(xq=None) == bad and f(out=None) == bad and f(old=7) == bad
+    assert f(w=None) == bad and f(out=None) == bad and f(old=7) == bad
+    assert f(xq=None) == gate(N) and N.MXFP4_DIRECT_ROWS == 64  # few rows need no room
+    assert f(rows=64, xq=None) == gate(N) and f(rows=65, xq=None) == bad
     assert f(rows=5) == N.MMN_E_SHAPE
     assert f(xq=mx(N, 4, 96, 0x1000000000)) == N.MMN_E_SHAPE
     assert f(xq=mx(N, 4, 64, 0x2000000000)) == bad  # the room lies over the weight
     assert f(xq=mx(N, 4, 64, 0x7000000000)) == bad  # ... over x
     assert f(out=vp(0x7000000000)) == bad           # out over x
+
+
+def test_direct_rows_constant_agrees(N):
+    import os
+    import re
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = open(os.path.join(root, "include", "mmn_optim.h")).read()
+    assert re.findall(r"#define MMN_MXFP4_DIRECT_ROWS (\d+)", text) == [str(N.MXFP4_DIRECT_ROWS)]
 
 
 def test_wrappers_refuse_what_is_not_theirs():
