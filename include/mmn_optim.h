@@ -530,7 +530,7 @@ int mmn_mxfp4_matmul(const mmn_mxfp4 *a, const mmn_mxfp4 *b, void *out, int64_t 
  * bf16) is rounded to 4 bits and multiplied: out (rows x w.rows) = q(x) W^T. xq
  * (rows x w.cols) gives room for the rounded x, its contents afterwards are
  * unspecified; up to MMN_MXFP4_DIRECT_ROWS rows need none (NULL). */
-#define MMN_MXFP4_DIRECT_ROWS 64
+#define MMN_MXFP4_DIRECT_ROWS 16
 int mmn_mxfp4_linear(const void *x, int64_t x_ld, int x_dtype, int64_t rows, const mmn_mxfp4 *w,
                      const mmn_mxfp4 *xq, void *out, int64_t out_ld, int out_dtype, int device,
                      void *stream);

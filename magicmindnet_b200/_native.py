@@ -18,7 +18,7 @@ MEM_HOST, MEM_DEVICE = 0, 1
 DTYPE_F32, DTYPE_BF16 = 0, 1
 ROUTE_AUTO, ROUTE_MUON, ROUTE_ADAMW = 0, 1, 2
 NS_REFERENCE, NS_BF16, NS_TF32, NS_FP32 = 0, 1, 2, 3
-MXFP4_DIRECT_ROWS = 64
+MXFP4_DIRECT_ROWS = 16
 
 
 class MmnError(RuntimeError):

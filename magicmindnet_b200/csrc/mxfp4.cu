@@ -87,6 +87,8 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
   uint8_t* sf_row = sm + 128 * kPitch;
   uint8_t* sf_col = sf_row + 512;
   const int tid = threadIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();  // a product's setup overlaps this kernel's end
   const int ct = blockIdx.x % a.nct, rt = blockIdx.x / a.nct;
   const int c0 = ct * 128, r0 = rt * 128;
   const bool in_c = c0 < a.cols, in_r = r0 < a.rows;
@@ -423,9 +425,7 @@ int kernel_setup(int device) {
   int rc;
   if ((rc = split_setup<16, 0>()) != MMN_OK || (rc = split_setup<32, 0>()) != MMN_OK ||
       (rc = split_setup<64, 0>()) != MMN_OK || (rc = split_setup<128, 0>()) != MMN_OK ||
-      (rc = split_setup<16, 1>()) != MMN_OK || (rc = split_setup<32, 1>()) != MMN_OK ||
-      (rc = split_setup<64, 1>()) != MMN_OK || (rc = split_setup<16, 2>()) != MMN_OK ||
-      (rc = split_setup<32, 2>()) != MMN_OK || (rc = split_setup<64, 2>()) != MMN_OK)
+      (rc = split_setup<16, 1>()) != MMN_OK || (rc = split_setup<16, 2>()) != MMN_OK)
     return rc;
   MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_pair_kernel, smem, MxPair::kSmemBytes));
   if (device < 64) done |= uint64_t(1) << device;
@@ -456,12 +456,21 @@ int launch_quantize(const void* x, int64_t ld, int dtype, int64_t rows, int64_t 
   a.vec = vec_rows(x, ld, esize(dtype), 16);
   const int64_t blocks = nrt * a.nct;
   if (blocks > (int64_t(1) << 31) - 1) return fail(MMN_E_SHAPE, "matrix too large");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.dynamicSmemBytes =
+      dtype == MMN_DTYPE_BF16 ? MxTile<__nv_bfloat16>::kSmem : MxTile<float>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   if (dtype == MMN_DTYPE_BF16)
-    mx_quantize_kernel<__nv_bfloat16>
-        <<<(unsigned)blocks, 256, MxTile<__nv_bfloat16>::kSmem, s>>>(a);
+    MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_quantize_kernel<__nv_bfloat16>, a));
   else
-    mx_quantize_kernel<float><<<(unsigned)blocks, 256, MxTile<float>::kSmem, s>>>(a);
-  MMN_CUDA_TRY(cudaGetLastError());
+    MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_quantize_kernel<float>, a));
   return MMN_OK;
 }
 
@@ -495,12 +504,14 @@ int launch_split(const mmn_mxfp4* a, const MxRows& rows, const mmn_mxfp4* w, int
   cfg.blockDim = dim3(MxSplit<BN, SRC>::kThreads, 1, 1);
   cfg.dynamicSmemBytes = MxSplit<BN, SRC>::kSmemBytes;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_split_kernel<BN, SRC>, tw, tx, g, rows, splits));
   return MMN_OK;
 }
@@ -561,12 +572,14 @@ int launch_gemm_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int 
   cfg.blockDim = dim3(MxPair::kThreads, 1, 1);
   cfg.dynamicSmemBytes = MxPair::kSmemBytes;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel, ta, tb, tsa, tsb, to, g,
                                   (int)tiles_m, (int)tiles));
   return MMN_OK;
@@ -587,15 +600,22 @@ int gemm_out(MxGemmArgs* g, void* out, int64_t ld, int dtype, int accumulate) {
   return kernel_status_word(&g->status);
 }
 
-// out (a.rows x b.rows) = A B^T, on checked arguments.
+// out (a.rows x b.rows) = A B^T, on checked arguments. early_w: B was complete
+// before the stream's previous kernel, one of this file, began.
 int product(const mmn_mxfp4* a, const mmn_mxfp4* b, void* out, int64_t ld, int dtype,
-            int accumulate, int sms, cudaStream_t s) {
+            int accumulate, int early_w, int sms, cudaStream_t s) {
   if (a->rows == 0 || b->rows == 0) return MMN_OK;
   if (a->cols == 0) return accumulate ? MMN_OK : zero_out(out, ld, a->rows, b->rows, dtype, s);
   MxGemmArgs g{};
   int rc = gemm_out(&g, out, ld, dtype, accumulate);
   if (rc != MMN_OK) return rc;
-  if (a->rows > 256 && b->rows > 256) return launch_gemm_pair(a, b, g, sms, s);
+  g.early_w = early_w;
+  // 256 x 256 tiles on CTA pairs once 128 x 128 ones fill two thirds of the SMs
+  // (512 x 4096 x 4096, 128 of them: 11.6 us against 12.0; 256 x 4096 x 4096, 64:
+  // 11.1 against 10.0; 1000 x 1030 x 4096, 72: 18.8 against 10.3).
+  const int64_t tiles = (a->rows + 127) / 128 * ((b->rows + 127) / 128);
+  if (a->rows > 128 && tiles * 3 > (int64_t)sms * 2)
+    return launch_gemm_pair(a, b, g, sms, s);
   const MxRows none{};
   if (a->rows <= 16) return launch_split<16, 0>(a, none, b, a->rows, g, sms, s);
   if (a->rows <= 32) return launch_split<32, 0>(a, none, b, a->rows, g, sms, s);
@@ -610,14 +630,8 @@ int direct_linear(const void* x, int64_t ld, int dtype, int64_t rows, const mmn_
   int rc = gemm_out(&g, out, out_ld, out_dtype, 0);
   if (rc != MMN_OK) return rc;
   const MxRows r{x, ld, (int)w->cols, vec_rows(x, ld, esize(dtype), 16)};
-  if (dtype == MMN_DTYPE_BF16) {
-    if (rows <= 16) return launch_split<16, 1>(nullptr, r, w, rows, g, sms, s);
-    if (rows <= 32) return launch_split<32, 1>(nullptr, r, w, rows, g, sms, s);
-    return launch_split<64, 1>(nullptr, r, w, rows, g, sms, s);
-  }
-  if (rows <= 16) return launch_split<16, 2>(nullptr, r, w, rows, g, sms, s);
-  if (rows <= 32) return launch_split<32, 2>(nullptr, r, w, rows, g, sms, s);
-  return launch_split<64, 2>(nullptr, r, w, rows, g, sms, s);
+  return dtype == MMN_DTYPE_BF16 ? launch_split<16, 1>(nullptr, r, w, rows, g, sms, s)
+                                 : launch_split<16, 2>(nullptr, r, w, rows, g, sms, s);
 }
 
 int check_out(const void* out, int64_t ld, int dtype, int64_t rows, int64_t cols,
@@ -739,8 +753,8 @@ extern "C" int mmn_mxfp4_matmul(const mmn_mxfp4* a, const mmn_mxfp4* b, void* ou
   if ((rc = check_mx_device(b, device, "b")) != MMN_OK) return rc;
   if ((rc = check_device_elems(out, esize(dtype), device, "out")) != MMN_OK) return rc;
   if ((rc = kernel_setup(device)) != MMN_OK) return rc;
-  return product(a, b, out, a->rows > 1 ? out_ld : b->rows, dtype, accumulate, sms,
-                 static_cast<cudaStream_t>(stream));
+  return product(a, b, out, a->rows > 1 ? out_ld : b->rows, dtype, accumulate, 0,
+                 sms, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mmn_mxfp4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t rows,
@@ -783,7 +797,7 @@ extern "C" int mmn_mxfp4_linear(const void* x, int64_t x_ld, int x_dtype, int64_
   if (direct)
     return direct_linear(x, ld, x_dtype, rows, w, out, old, out_dtype, sms, s);
   if ((rc = launch_quantize(x, ld, x_dtype, rows, cols, xq, nullptr, s)) != MMN_OK) return rc;
-  return product(xq, w, out, old, out_dtype, 0, sms, s);
+  return product(xq, w, out, old, out_dtype, 0, 1, sms, s);
 }
 
 extern "C" int mmn_kernel_status(int device, void* stream) {

@@ -30,6 +30,7 @@ struct MxGemmArgs {
   int accumulate;
   int vec;             // out and ld are aligned for 16-byte accesses
   int tma_out;         // the pair kernel stores through its tensor map
+  int early_w;         // split kernel: the lanes' operand was complete before the previous kernel
   int* status;
 };
 
@@ -100,7 +101,7 @@ struct MxSplit {
   static constexpr int kStageBytes = kTileBytes + kSfBytes;
   static constexpr int kStages = 212000 / kStageBytes < 8 ? 212000 / kStageBytes : 8;
   // k blocks of A rounded at a time (SRC != 0)
-  static constexpr int kChunk = SRC == 0 ? 0 : (BN <= 32 ? 16 : 8);
+  static constexpr int kChunk = SRC == 0 ? 0 : 16;
   static constexpr int kQBytes = kChunk * (kBBytes + 1024);
   static constexpr int kAccCols = BN < 32 ? 32 : BN;
   static constexpr int kColsUsed = kAccCols + kStages * 16;
@@ -147,23 +148,102 @@ __global__ void __launch_bounds__(320, 1)
   const int kb0 = (int)((long long)args.num_kb * rank / splits);
   const int nkb = (int)((long long)args.num_kb * (rank + 1) / splits) - kb0;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+  // The loads of a stage: the lanes' operand, then (SRC = 0) the rows.
+  auto load_w = [&](int i) {
+    const int s = i % STAGES, kb = kb0 + i;
+    mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+    tma_load_3d(tiles + s * S::kTileBytes, &tm_w, &full[s], kb * 128, tm * 128, 0);
+    bulk_load(sfs + s * S::kSfBytes, args.sfa + ((long long)tm * args.ka + kb * 2) * 512, 1024,
+              &full[s]);
+  };
+  auto load_x = [&](int i) {
+    const int s = i % STAGES, kb = kb0 + i;
+    tma_load_3d(tiles + s * S::kTileBytes + S::kABytes, &tm_x, &full[s], kb * 128, tn * BN, 0);
+    bulk_load(sfs + s * S::kSfBytes + 1024,
+              args.sfb + ((long long)(tn * BN / 128) * args.ka + kb * 2) * 512, 1024, &full[s]);
+  };
+  // The rounding of k blocks c0 .. c0 + nk - 1 of the rows, one block of 32 per turn;
+  // consecutive threads take consecutive blocks.
+  auto round_rows = [&](int et, int c0, int nk) {
+    for (int id = et; id < BN * nk * 8; id += 256) {
+      const int n = id / (nk * 8), b = id - n * (nk * 8), q = b >> 3, j = b & 7;
+      const int row = tn * BN + n, col = (kb0 + c0) * 256 + b * 32;
+      float w[32];
+      const int have = row < args.N ? min(32, rows.cols - col) : 0;
+      if constexpr (SRC == 1) {
+        const __nv_bfloat16* p =
+            static_cast<const __nv_bfloat16*>(rows.x) + (long long)row * rows.ld + col;
+        if (have == 32 && rows.vec) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+            const uint32_t e[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              w[i * 8 + 2 * k] = __uint_as_float(e[k] << 16);
+              w[i * 8 + 2 * k + 1] = __uint_as_float(e[k] & 0xFFFF0000u);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) w[i] = i < have ? __bfloat162float(p[i]) : 0.0f;
+        }
+      } else {
+        const float* p = static_cast<const float*>(rows.x) + (long long)row * rows.ld + col;
+        if (have == 32 && rows.vec) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 u = reinterpret_cast<const float4*>(p)[i];
+            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) w[i] = i < have ? p[i] : 0.0f;
+        }
+      }
+      uint32_t sc;
+      const uint4 u = mx_block(w, &sc);
+      *reinterpret_cast<uint4*>(qb + q * S::kBBytes + n * 128 + ((j ^ (n & 7)) << 4)) = u;
+      qs[q * 1024 + (j >> 2) * 512 + (n & 31) * 16 + (n >> 5) * 4 + (j & 3)] = (uint8_t)sc;
     }
-    mbar_init(tfull, 1);
-    mbar_init(bready, 256);
-    mbar_init(bfree, 1);
-    *abort_flag = 0;
-    fence_barrier_init();
-    tma_prefetch_desc(&tm_w);
-    if (SRC == 0) tma_prefetch_desc(&tm_x);
-  }
-  if (warp == 1) {
+    fence_proxy_async_smem();
+  };
+
+  // Launched as a programmatic dependent: barriers and TMEM are set up while the
+  // previous kernel ends. Nothing it may have written is read before the wait;
+  // early_w says that the lanes' operand is older than it. The first stages are
+  // on their way, and the first rows rounded, before the block first meets.
+  uint32_t last = 0, issued = 0;  // parity of each stage's last load, stages used
+  const int ahead = nkb < STAGES ? nkb : STAGES;
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&tm_w);
+      if (SRC == 0) tma_prefetch_desc(&tm_x);
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&full[s], 1);
+        mbar_init(&empty[s], 1);
+      }
+      mbar_init(tfull, 1);
+      mbar_init(bready, 256);
+      mbar_init(bfree, 1);
+      *abort_flag = 0;
+      fence_barrier_init();
+      if (!args.early_w) griddep_wait();
+      for (int i = 0; i < ahead; ++i) load_w(i);
+      if (args.early_w) griddep_wait();
+      if (SRC == 0)
+        for (int i = 0; i < ahead; ++i) load_x(i);
+    }
+    __syncwarp();
+    issued = (1u << ahead) - 1;
+  } else if (warp == 1) {
     tmem_alloc(tmem_slot, S::kTmemCols);
     tmem_relinquish();
+  } else {
+    griddep_wait();
+    if (SRC != 0) round_rows(threadIdx.x - 64, 0, min(S::kChunk, nkb));
   }
+  griddep_launch_dependents();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -171,25 +251,14 @@ __global__ void __launch_bounds__(320, 1)
 
   if (warp == 0) {
     const bool one = elect_one();
-    uint32_t last = 0, issued = 0;  // parity of each stage's last load, stages used
-    for (int i = 0; i < nkb; ++i) {
+    for (int i = ahead; i < nkb; ++i) {
       const int s = i % STAGES;
       const uint32_t ph = (i / STAGES) & 1;
       if (!mbar_wait_warp(&empty[s], ph ^ 1u, abort_flag)) break;
       if (one) {
-        const int kb = kb0 + i;
-        mbar_arrive_expect_tx(&full[s], S::kStageBytes);
-        uint8_t* t = tiles + s * S::kTileBytes;
-        uint8_t* f = sfs + s * S::kSfBytes;
-        tma_load_3d(t, &tm_w, &full[s], kb * 128, tm * 128, 0);
-        bulk_load(f, args.sfa + ((long long)tm * args.ka + kb * 2) * 512, 1024, &full[s]);
-        if constexpr (SRC == 0) {
-          tma_load_3d(t + S::kABytes, &tm_x, &full[s], kb * 128, tn * BN, 0);
-          bulk_load(f + 1024, args.sfb + ((long long)(tn * BN / 128) * args.ka + kb * 2) * 512,
-                    1024, &full[s]);
-        }
+        load_w(i);
+        if (SRC == 0) load_x(i);
       }
-      issued |= 1u << s;
       last = (last & ~(1u << s)) | (ph << s);
     }
     // every load lands before the CTA may exit
@@ -208,8 +277,8 @@ __global__ void __launch_bounds__(320, 1)
     for (int i = 0; i < nkb; ++i) {
       const int s = i % STAGES;
       if constexpr (SRC != 0) {
-        if (i % S::kChunk == 0 &&
-            !mbar_wait_warp(bready, (i / S::kChunk) & 1, abort_flag)) {
+        if (i > 0 && i % S::kChunk == 0 &&
+            !mbar_wait_warp(bready, (i / S::kChunk - 1) & 1, abort_flag)) {
           ok = false;
           break;
         }
@@ -256,52 +325,9 @@ __global__ void __launch_bounds__(320, 1)
   } else {
     const int et = threadIdx.x - 64;
     if constexpr (SRC != 0) {
-      for (int c0 = 0; c0 < nkb; c0 += S::kChunk) {
-        const int nk = min(S::kChunk, nkb - c0);
-        if (c0 > 0) mbar_wait(bfree, (c0 / S::kChunk - 1) & 1, abort_flag);
-        // one block of 32 per turn; consecutive threads take consecutive blocks
-        for (int id = et; id < BN * nk * 8; id += 256) {
-          const int n = id / (nk * 8), b = id - n * (nk * 8), q = b >> 3, j = b & 7;
-          const int row = tn * BN + n, col = (kb0 + c0) * 256 + b * 32;
-          float w[32];
-          const int have = row < args.N ? min(32, rows.cols - col) : 0;
-          if constexpr (SRC == 1) {
-            const __nv_bfloat16* p =
-                static_cast<const __nv_bfloat16*>(rows.x) + (long long)row * rows.ld + col;
-            if (have == 32 && rows.vec) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-                const uint32_t e[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  w[i * 8 + 2 * k] = __uint_as_float(e[k] << 16);
-                  w[i * 8 + 2 * k + 1] = __uint_as_float(e[k] & 0xFFFF0000u);
-                }
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) w[i] = i < have ? __bfloat162float(p[i]) : 0.0f;
-            }
-          } else {
-            const float* p = static_cast<const float*>(rows.x) + (long long)row * rows.ld + col;
-            if (have == 32 && rows.vec) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 u = reinterpret_cast<const float4*>(p)[i];
-                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) w[i] = i < have ? p[i] : 0.0f;
-            }
-          }
-          uint32_t sc;
-          const uint4 u = mx_block(w, &sc);
-          *reinterpret_cast<uint4*>(qb + q * S::kBBytes + n * 128 + ((j ^ (n & 7)) << 4)) = u;
-          qs[q * 1024 + (j >> 2) * 512 + (n & 31) * 16 + (n >> 5) * 4 + (j & 3)] = (uint8_t)sc;
-        }
-        fence_proxy_async_smem();
+      for (int c0 = S::kChunk; c0 < nkb; c0 += S::kChunk) {
+        mbar_wait(bfree, (c0 / S::kChunk - 1) & 1, abort_flag);
+        round_rows(et, c0, min(S::kChunk, nkb - c0));
         mbar_arrive(bready);
       }
     }
@@ -458,17 +484,29 @@ __device__ __forceinline__ void mx_store_block(const MxGemmArgs& a, long long r0
       }
     }
   } else if (lane < cols) {
-    for (int r = 0; r < rows && r < 32; ++r) {
-      float f = tst[r * 33 + lane];
-      const long long i = (r0 + r) * a.ld + c0 + lane;
-      if (a.out_bf16) {
-        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out) + i;
-        if (a.accumulate) f += __bfloat162float(*p);
-        *p = __float2bfloat16_rn(f);
-      } else {
-        float* p = static_cast<float*>(a.out) + i;
-        *p = a.accumulate ? *p + f : f;
+    // a row per turn, one column per lane; loads of eight rows before their stores
+    const long long i0 = r0 * a.ld + c0 + lane;
+#pragma unroll 1
+    for (int r = 0; r < rows; r += 8) {
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        f[k] = tst[(r + k) * 33 + lane];
+        if (a.accumulate && r + k < rows) {
+          const long long i = i0 + (r + k) * a.ld;
+          f[k] += a.out_bf16 ? __bfloat162float(static_cast<__nv_bfloat16*>(a.out)[i])
+                             : static_cast<float*>(a.out)[i];
+        }
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (r + k < rows) {
+          const long long i = i0 + (r + k) * a.ld;
+          if (a.out_bf16)
+            static_cast<__nv_bfloat16*>(a.out)[i] = __float2bfloat16_rn(f[k]);
+          else
+            static_cast<float*>(a.out)[i] = f[k];
+        }
     }
   }
   __syncwarp();
@@ -609,6 +647,10 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
   cluster_sync_all();  // the peer's barriers are initialised, both TMEM allocations done
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // Launched as a programmatic dependent: only the setup above overlaps the
+  // previous kernel.
+  griddep_wait();
+  griddep_launch_dependents();
 
   // The loading and the issuing warp stay converged: all lanes wait, one elected
   // lane issues. (With the waits inside a one-lane branch the scale copies did

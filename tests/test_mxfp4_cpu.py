@@ -109,8 +109,9 @@ def test_linear_refusals(N):
     assert f() == gate(N)
     assert f(x=None) == bad and f(ld=63) == bad and f(xd=4) == bad and f(od=4) == bad
     assert f(w=None) == bad and f(out=None) == bad and f(old=7) == bad
-    assert f(xq=None) == gate(N) and N.MXFP4_DIRECT_ROWS == 64  # few rows need no room
-    assert f(rows=64, xq=None) == gate(N) and f(rows=65, xq=None) == bad
+    few = N.MXFP4_DIRECT_ROWS
+    assert f(xq=None) == gate(N)  # few rows need no room
+    assert f(rows=few, xq=None) == gate(N) and f(rows=few + 1, xq=None) == bad
     assert f(rows=5) == N.MMN_E_SHAPE
     assert f(xq=mx(N, 4, 96, 0x1000000000)) == N.MMN_E_SHAPE
     assert f(xq=mx(N, 4, 64, 0x2000000000)) == bad  # the room lies over the weight
