@@ -100,15 +100,15 @@ struct MxSplit {
   static constexpr int kSfBytes = SRC == 0 ? 2048 : 1024;
   static constexpr int kStageBytes = kTileBytes + kSfBytes;
   static constexpr int kStages = 212000 / kStageBytes < 8 ? 212000 / kStageBytes : 8;
-  // k blocks of A rounded at a time (SRC != 0)
-  static constexpr int kChunk = SRC == 0 ? 0 : 16;
-  static constexpr int kQBytes = kChunk * (kBBytes + 1024);
+  static constexpr int kPairs = SRC == 0 ? 0 : 8;  // pairs of rounded k blocks (SRC != 0)
+  static constexpr int kQBytes = 2 * kPairs * (kBBytes + 1024);
   static constexpr int kAccCols = BN < 32 ? 32 : BN;
   static constexpr int kColsUsed = kAccCols + kStages * 16;
   static constexpr int kTmemCols = kColsUsed <= 128 ? 128 : 256;
   static constexpr int kThreads = 64 + 256;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kQBytes + 512;
   static_assert(kColsUsed <= 256, "TMEM columns");
+  static_assert(SRC == 0 || BN == 16, "a thread per block of a pair of k blocks");
   static_assert(kSmemBytes <= 232448, "shared memory per CTA");
   static_assert(kStages * kTileBytes >= BN * 128 * 4, "the partial tile takes the stages' place");
 };
@@ -118,6 +118,52 @@ struct MxRows {
   long long ld;
   int cols;
   int vec;        // rows are 16-byte aligned
+};
+
+// A block of 32 values of a row on its way: bf16 (SRC 1) or fp32 (2) as loaded.
+template <int SRC>
+struct MxRaw {
+  uint4 u[SRC == 2 ? 8 : 4];
+  // `have` values exist from (row, col) on; the rest of the block is zero
+  __device__ __forceinline__ void load(const MxRows& r, int row, int col, int have) {
+    constexpr int kPer = SRC == 2 ? 4 : 8;  // values per 16 bytes
+    const char* p = static_cast<const char*>(r.x) + ((long long)row * r.ld + col) * (16 / kPer);
+    if (have == 32 && r.vec) {
+#pragma unroll
+      for (int i = 0; i < 32 / kPer; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32 / kPer; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (SRC == 2) {
+            w[k] = i * 4 + k < have ? reinterpret_cast<const uint32_t*>(p)[i * 4 + k] : 0u;
+          } else {
+            const int e = i * 8 + 2 * k;
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+            w[k] = (e < have ? (uint32_t)h[e] : 0u) | (e + 1 < have ? (uint32_t)h[e + 1] << 16 : 0u);
+          }
+        }
+        u[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  __device__ __forceinline__ void values(float (&w)[32]) const {
+#pragma unroll
+    for (int i = 0; i < (SRC == 2 ? 8 : 4); ++i) {
+      const uint32_t e[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (SRC == 2) {
+          w[i * 4 + k] = __uint_as_float(e[k]);
+        } else {
+          w[i * 8 + 2 * k] = __uint_as_float(e[k] << 16);
+          w[i * 8 + 2 * k + 1] = __uint_as_float(e[k] & 0xFFFF0000u);
+        }
+      }
+    }
+  }
 };
 
 template <int BN, int SRC>
@@ -131,16 +177,16 @@ __global__ void __launch_bounds__(320, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* tiles = smem;
-  uint8_t* qb = smem + STAGES * S::kTileBytes;   // rounded A: [chunk][BN x 128 B], swizzled
-  uint8_t* qs = qb + S::kChunk * S::kBBytes;     // its scales: [chunk][1024]
-  uint8_t* sfs = qs + S::kChunk * 1024;
+  uint8_t* qb = smem + STAGES * S::kTileBytes;    // rounded A: [k block][BN x 128 B], swizzled
+  uint8_t* qs = qb + 2 * S::kPairs * S::kBBytes;  // its scales: [k block][1024]
+  uint8_t* sfs = qs + 2 * S::kPairs * 1024;
   uint64_t* full = reinterpret_cast<uint64_t*>(sfs + STAGES * S::kSfBytes);
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = full + 2 * STAGES;
-  uint64_t* bready = tfull + 1;  // a chunk of A is rounded
-  uint64_t* bfree = tfull + 2;   // its MMAs are done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 3);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tfull + 4);
+  uint64_t* bready = tfull + 1;           // a pair of k blocks of A is rounded
+  uint64_t* bfree = bready + S::kPairs;   // its MMAs are done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bfree + S::kPairs);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bfree + S::kPairs + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
@@ -162,51 +208,14 @@ __global__ void __launch_bounds__(320, 1)
     bulk_load(sfs + s * S::kSfBytes + 1024,
               args.sfb + ((long long)(tn * BN / 128) * args.ka + kb * 2) * 512, 1024, &full[s]);
   };
-  // The rounding of k blocks c0 .. c0 + nk - 1 of the rows, one block of 32 per turn;
-  // consecutive threads take consecutive blocks.
-  auto round_rows = [&](int et, int c0, int nk) {
-    for (int id = et; id < BN * nk * 8; id += 256) {
-      const int n = id / (nk * 8), b = id - n * (nk * 8), q = b >> 3, j = b & 7;
-      const int row = tn * BN + n, col = (kb0 + c0) * 256 + b * 32;
-      float w[32];
-      const int have = row < args.N ? min(32, rows.cols - col) : 0;
-      if constexpr (SRC == 1) {
-        const __nv_bfloat16* p =
-            static_cast<const __nv_bfloat16*>(rows.x) + (long long)row * rows.ld + col;
-        if (have == 32 && rows.vec) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-            const uint32_t e[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              w[i * 8 + 2 * k] = __uint_as_float(e[k] << 16);
-              w[i * 8 + 2 * k + 1] = __uint_as_float(e[k] & 0xFFFF0000u);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) w[i] = i < have ? __bfloat162float(p[i]) : 0.0f;
-        }
-      } else {
-        const float* p = static_cast<const float*>(rows.x) + (long long)row * rows.ld + col;
-        if (have == 32 && rows.vec) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 u = reinterpret_cast<const float4*>(p)[i];
-            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) w[i] = i < have ? p[i] : 0.0f;
-        }
-      }
-      uint32_t sc;
-      const uint4 u = mx_block(w, &sc);
-      *reinterpret_cast<uint4*>(qb + q * S::kBBytes + n * 128 + ((j ^ (n & 7)) << 4)) = u;
-      qs[q * 1024 + (j >> 2) * 512 + (n & 31) * 16 + (n >> 5) * 4 + (j & 3)] = (uint8_t)sc;
-    }
-    fence_proxy_async_smem();
+  // SRC != 0: a thread rounds one block of 32 of each pair of k blocks (16 rows x 16
+  // blocks), its next one already on the way. Pairs go round a ring of kPairs.
+  const int et = threadIdx.x - 64, qn = et >> 4, qj = et & 15;
+  const int npairs = (nkb + 1) / 2;
+  MxRaw<SRC> raw;
+  auto fetch = [&](int p) {
+    const int row = tn * BN + qn, col = (kb0 + 2 * p) * 256 + qj * 32;
+    raw.load(rows, row, col, row < args.N && 2 * p + (qj >> 3) < nkb ? min(32, rows.cols - col) : 0);
   };
 
   // Launched as a programmatic dependent: barriers and TMEM are set up while the
@@ -224,8 +233,10 @@ __global__ void __launch_bounds__(320, 1)
         mbar_init(&empty[s], 1);
       }
       mbar_init(tfull, 1);
-      mbar_init(bready, 256);
-      mbar_init(bfree, 1);
+      for (int p = 0; p < S::kPairs; ++p) {
+        mbar_init(&bready[p], 256);
+        mbar_init(&bfree[p], 1);
+      }
       *abort_flag = 0;
       fence_barrier_init();
       if (!args.early_w) griddep_wait();
@@ -241,7 +252,7 @@ __global__ void __launch_bounds__(320, 1)
     tmem_relinquish();
   } else {
     griddep_wait();
-    if (SRC != 0) round_rows(threadIdx.x - 64, 0, min(S::kChunk, nkb));
+    if constexpr (SRC != 0) fetch(0);
   }
   griddep_launch_dependents();
   tc_fence_before();
@@ -277,8 +288,8 @@ __global__ void __launch_bounds__(320, 1)
     for (int i = 0; i < nkb; ++i) {
       const int s = i % STAGES;
       if constexpr (SRC != 0) {
-        if (i > 0 && i % S::kChunk == 0 &&
-            !mbar_wait_warp(bready, (i / S::kChunk - 1) & 1, abort_flag)) {
+        const int p = i >> 1;
+        if (!(i & 1) && !mbar_wait_warp(&bready[p % S::kPairs], (p / S::kPairs) & 1, abort_flag)) {
           ok = false;
           break;
         }
@@ -291,7 +302,7 @@ __global__ void __launch_bounds__(320, 1)
       if (one) {
         const uint32_t t = smem_u32(tiles + s * S::kTileBytes);
         const uint32_t f = smem_u32(sfs + s * S::kSfBytes);
-        const int qi = SRC == 0 ? 0 : i % S::kChunk;
+        const int qi = SRC == 0 ? 0 : i % (2 * S::kPairs);
         const uint32_t bt = SRC == 0 ? t + S::kABytes : smem_u32(qb + qi * S::kBBytes);
         const uint32_t bf = SRC == 0 ? f + 1024 : smem_u32(qs + qi * 1024);
         const uint32_t sa = tmem_base + S::kAccCols + s * 16, sb = sa + 8;
@@ -309,7 +320,7 @@ __global__ void __launch_bounds__(320, 1)
                       sb + 4 * h, (i | kk) != 0);
         }
         tc_commit(&empty[s]);
-        if (SRC != 0 && (i + 1) % (S::kChunk ? S::kChunk : 1) == 0) tc_commit(bfree);
+        if (SRC != 0 && (i & 1)) tc_commit(&bfree[(i >> 1) % S::kPairs]);
       }
       __syncwarp();
     }
@@ -323,12 +334,19 @@ __global__ void __launch_bounds__(320, 1)
     }
     __syncwarp();
   } else {
-    const int et = threadIdx.x - 64;
     if constexpr (SRC != 0) {
-      for (int c0 = S::kChunk; c0 < nkb; c0 += S::kChunk) {
-        mbar_wait(bfree, (c0 / S::kChunk - 1) & 1, abort_flag);
-        round_rows(et, c0, min(S::kChunk, nkb - c0));
-        mbar_arrive(bready);
+      for (int p = 0; p < npairs; ++p) {
+        const int slot = p % S::kPairs, q = 2 * slot + (qj >> 3), j = qj & 7;
+        if (p >= S::kPairs) mbar_wait(&bfree[slot], (p / S::kPairs - 1) & 1, abort_flag);
+        float w[32];
+        raw.values(w);
+        if (p + 1 < npairs) fetch(p + 1);
+        uint32_t sc;
+        const uint4 u = mx_block(w, &sc);
+        *reinterpret_cast<uint4*>(qb + q * S::kBBytes + qn * 128 + ((j ^ (qn & 7)) << 4)) = u;
+        qs[q * 1024 + (j >> 2) * 512 + qn * 16 + (j & 3)] = (uint8_t)sc;
+        fence_proxy_async_smem();
+        mbar_arrive(&bready[slot]);
       }
     }
     // the partial tile, [row of out][column of out], into the stages' place
