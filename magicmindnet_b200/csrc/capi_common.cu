@@ -1,5 +1,6 @@
 // Shared pieces of the C ABI: error reporting, device contexts, the AdamW
 // bias-correction table and the environment entry points.
+#include <atomic>
 #include <cmath>
 #include <cstring>
 
@@ -162,8 +163,15 @@ int check_device_ptr(const void* p, int device, const char* what) {
 // device (mmn_kernel_status).
 __device__ int g_kernel_status;
 
-int kernel_status_word(int** p) {
-  MMN_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(p), g_kernel_status));
+int kernel_status_word(int device, int** p) {
+  // the address is fixed per device: asked for once (any thread writes the same)
+  static std::atomic<int*> known[64];
+  int* k = device < 64 ? known[device].load(std::memory_order_relaxed) : nullptr;
+  if (!k) {
+    MMN_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(&k), g_kernel_status));
+    if (device < 64) known[device].store(k, std::memory_order_relaxed);
+  }
+  *p = k;
   return MMN_OK;
 }
 

@@ -28,6 +28,10 @@ struct DeviceGuard {
   int prev = -1;
   explicit DeviceGuard(int dev) {
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev == dev) {
+      prev = -1;  // nothing to change or restore
+      return;
+    }
     cudaSetDevice(dev);
   }
   ~DeviceGuard() {
@@ -80,8 +84,9 @@ int check_device_ptr(const void* p, int device, const char* what);
 // check_device_ptr, and `p` is aligned to its elements of `esize` bytes.
 int check_device_elems(const void* p, size_t esize, int device, const char* what);
 
-// The current device's status word of the caller-buffer kernels (mmn_kernel_status).
-int kernel_status_word(int** p);
+// The status word of the caller-buffer kernels (mmn_kernel_status) on `device`,
+// which is current.
+int kernel_status_word(int device, int** p);
 
 // The device checks of the caller-buffer entry points: a usable sm_100 GPU,
 // whose SM count goes to *sms.

@@ -943,7 +943,7 @@ int ring_fwd_launch(const LnFwd& a, int sms, int device, cudaStream_t s) {
   int* status = nullptr;
   int rc;
   if ((rc = raise_smem(kernel, device, mu, done)) != MMN_OK) return rc;
-  if ((rc = kernel_status_word(&status)) != MMN_OK) return rc;
+  if ((rc = kernel_status_word(device, &status)) != MMN_OK) return rc;
   const int64_t row = a.cols * (int64_t)sizeof(XT);
   // more rows in flight than this cost bandwidth (16384 x 4096, 3 blocks an SM:
   // 8 rows 51.2 us, 3 rows 48.6 us)
@@ -1057,7 +1057,7 @@ int bwd_types(const LnBwd& a, int parts, bool vec, bool ring, int device, cudaSt
   const int depth = ring && a.cols > 64 && a.cols <= kRingMaxCols ? ring_depth<XT, DT>(a.cols, &smem) : 0;
   if (depth >= 2) {
     int* status = nullptr;
-    const int rc = kernel_status_word(&status);
+    const int rc = kernel_status_word(device, &status);
     if (rc != MMN_OK) return rc;
     if (a.cols <= 256) return ring_launch<XT, DT, V, 32, 8>(a, parts, depth, smem, status, device, s);
     if (a.cols <= 512) return ring_launch<XT, DT, V, 64, 8>(a, parts, depth, smem, status, device, s);

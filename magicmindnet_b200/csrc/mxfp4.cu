@@ -591,23 +591,23 @@ int zero_out(void* out, int64_t ld, int64_t rows, int64_t cols, int dtype, cudaS
   return MMN_OK;
 }
 
-int gemm_out(MxGemmArgs* g, void* out, int64_t ld, int dtype, int accumulate) {
+int gemm_out(MxGemmArgs* g, void* out, int64_t ld, int dtype, int accumulate, int device) {
   g->out = out;
   g->ld = ld;
   g->out_bf16 = dtype == MMN_DTYPE_BF16;
   g->accumulate = accumulate != 0;
   g->vec = vec_rows(out, ld, esize(dtype), 8);
-  return kernel_status_word(&g->status);
+  return kernel_status_word(device, &g->status);
 }
 
 // out (a.rows x b.rows) = A B^T, on checked arguments. early_w: B was complete
 // before the stream's previous kernel, one of this file, began.
 int product(const mmn_mxfp4* a, const mmn_mxfp4* b, void* out, int64_t ld, int dtype,
-            int accumulate, int early_w, int sms, cudaStream_t s) {
+            int accumulate, int early_w, int sms, int device, cudaStream_t s) {
   if (a->rows == 0 || b->rows == 0) return MMN_OK;
   if (a->cols == 0) return accumulate ? MMN_OK : zero_out(out, ld, a->rows, b->rows, dtype, s);
   MxGemmArgs g{};
-  int rc = gemm_out(&g, out, ld, dtype, accumulate);
+  int rc = gemm_out(&g, out, ld, dtype, accumulate, device);
   if (rc != MMN_OK) return rc;
   g.early_w = early_w;
   // 256 x 256 tiles on CTA pairs once 128 x 128 ones fill two thirds of the SMs
@@ -625,9 +625,9 @@ int product(const mmn_mxfp4* a, const mmn_mxfp4* b, void* out, int64_t ld, int d
 
 // out = q(x) W^T for at most MMN_MXFP4_DIRECT_ROWS rows of x, on checked arguments.
 int direct_linear(const void* x, int64_t ld, int dtype, int64_t rows, const mmn_mxfp4* w, void* out,
-                  int64_t out_ld, int out_dtype, int sms, cudaStream_t s) {
+                  int64_t out_ld, int out_dtype, int sms, int device, cudaStream_t s) {
   MxGemmArgs g{};
-  int rc = gemm_out(&g, out, out_ld, out_dtype, 0);
+  int rc = gemm_out(&g, out, out_ld, out_dtype, 0, device);
   if (rc != MMN_OK) return rc;
   const MxRows r{x, ld, (int)w->cols, vec_rows(x, ld, esize(dtype), 16)};
   return dtype == MMN_DTYPE_BF16 ? launch_split<16, 1>(nullptr, r, w, rows, g, sms, s)
@@ -754,7 +754,7 @@ extern "C" int mmn_mxfp4_matmul(const mmn_mxfp4* a, const mmn_mxfp4* b, void* ou
   if ((rc = check_device_elems(out, esize(dtype), device, "out")) != MMN_OK) return rc;
   if ((rc = kernel_setup(device)) != MMN_OK) return rc;
   return product(a, b, out, a->rows > 1 ? out_ld : b->rows, dtype, accumulate, 0,
-                 sms, static_cast<cudaStream_t>(stream));
+                 sms, device, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mmn_mxfp4_linear(const void* x, int64_t x_ld, int x_dtype, int64_t rows,
@@ -795,9 +795,9 @@ extern "C" int mmn_mxfp4_linear(const void* x, int64_t x_ld, int x_dtype, int64_
   const int64_t ld = rows > 1 ? x_ld : cols, old = rows > 1 ? out_ld : w->rows;
   if (cols == 0) return zero_out(out, old, rows, w->rows, out_dtype, s);
   if (direct)
-    return direct_linear(x, ld, x_dtype, rows, w, out, old, out_dtype, sms, s);
+    return direct_linear(x, ld, x_dtype, rows, w, out, old, out_dtype, sms, device, s);
   if ((rc = launch_quantize(x, ld, x_dtype, rows, cols, xq, nullptr, s)) != MMN_OK) return rc;
-  return product(xq, w, out, old, out_dtype, 0, 1, sms, s);
+  return product(xq, w, out, old, out_dtype, 0, 1, sms, device, s);
 }
 
 extern "C" int mmn_kernel_status(int device, void* stream) {
@@ -805,7 +805,7 @@ extern "C" int mmn_kernel_status(int device, void* stream) {
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
   DeviceGuard guard(device);
   int* word = nullptr;
-  if ((rc = kernel_status_word(&word)) != MMN_OK) return rc;
+  if ((rc = kernel_status_word(device, &word)) != MMN_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int st = 0;
   MMN_CUDA_TRY(cudaMemcpyAsync(&st, word, sizeof(int), cudaMemcpyDeviceToHost, s));

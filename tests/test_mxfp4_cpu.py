@@ -44,6 +44,17 @@ def test_sizes(N):
     assert N.lib().mmn_mxfp4_size(1, 1, None, ctypes.byref(s)) == N.MMN_E_INVALID
 
 
+def test_python_matrix_has_the_c_sizes(N):
+    import magicmindnet_b200 as mmn
+
+    c, s = ctypes.c_int64(), ctypes.c_int64()
+    for r, k in ((1, 1), (5, 33), (128, 256), (129, 257), (300, 1030), (0, 64), (7, 0)):
+        N.check(N.lib().mmn_mxfp4_size(r, k, ctypes.byref(c), ctypes.byref(s)))
+        m = mmn.Mxfp4Matrix(r, k, "cpu")
+        assert m.codes.numel() == c.value and m.scales.numel() == s.value
+        assert m.codes.shape == (r, (k + 31) // 32 * 16)
+
+
 def quant(N, x=vp(0x7000000000), ld=64, dt=F32, rows=4, cols=64, q="q", qt="qt"):
     q = mx(N, 4, 64, 0x1000000000) if q == "q" else q
     qt = mx(N, 64, 4, 0x2000000000) if qt == "qt" else qt
