@@ -61,6 +61,17 @@ struct MxQuantArgs {
   int vec;                      // rows of x are 16-byte aligned
 };
 
+// The larger magnitudes of two pairs of bf16 (m >= 0); a NaN stays one.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t x) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\t"
+      "abs.bf16x2 t, %2;\n\t"
+      "max.NaN.bf16x2 %0, %1, t;\n\t}"
+      : "=r"(r)
+      : "r"(m), "r"(x));
+  return r;
+}
+
 template <typename T>
 struct MxTile {
   static constexpr int kPitch = 128 * sizeof(T) + 16;  // bytes; the skew spreads a column over banks
@@ -138,8 +149,8 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           u[q] = *reinterpret_cast<const uint4*>(sm + r * kPitch + k4 * 64 + q * 16);
-          mm = __vmaxu2(mm, __vmaxu2(__vmaxu2(u[q].x & 0x7FFF7FFFu, u[q].y & 0x7FFF7FFFu),
-                                     __vmaxu2(u[q].z & 0x7FFF7FFFu, u[q].w & 0x7FFF7FFFu)));
+          mm = max_abs2(max_abs2(mm, u[q].x), u[q].y);
+          mm = max_abs2(max_abs2(mm, u[q].z), u[q].w);
         }
         s = mx_scale(max(mm & 0xFFFFu, mm >> 16) << 16);
         const float inv = mx_inv_scale(s);
@@ -192,7 +203,7 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         w[i] = *reinterpret_cast<const uint32_t*>(sm + (rb * 32 + i) * kPitch + cp * 4);
-        mm = __vmaxu2(mm, w[i] & 0x7FFF7FFFu);
+        mm = max_abs2(mm, w[i]);
       }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
