@@ -181,6 +181,31 @@ int check_device_elems(const void* p, size_t esize, int device, const char* what
   return check_device_ptr(p, device, what);
 }
 
+bool matrices_overlap(const MatrixIn& a, const MatrixIn& b) {
+  if (a.rows == 0 || a.cols == 0 || b.rows == 0 || b.cols == 0) return false;
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.p), b0 = reinterpret_cast<uintptr_t>(b.p);
+  const uintptr_t aw = (uintptr_t)a.cols * a.esz, bw = (uintptr_t)b.cols * b.esz;
+  const uintptr_t as = (uintptr_t)a.ld * a.esz, bs = (uintptr_t)b.ld * b.esz;
+  const uintptr_t a1 = a0 + (uintptr_t)(a.rows - 1) * as + aw;
+  const uintptr_t b1 = b0 + (uintptr_t)(b.rows - 1) * bs + bw;
+  if (a1 <= b0 || b1 <= a0) return false;
+  // one row against rows of a pitch counts as that pitch
+  const uintptr_t s = a.rows == 1 ? bs : as;
+  if ((a.rows > 1 && b.rows > 1 && as != bs) || (a.rows == 1 && b.rows == 1) || s == 0) return true;
+  // same pitch: column slices of one buffer may interleave
+  const uintptr_t d = b0 >= a0 ? (b0 - a0) % s : (s - (a0 - b0) % s) % s;
+  return !(d >= aw && d + bw <= s);
+}
+
+int check_out_overlap(const MatrixIn& out, const char* what, const MatrixIn& in) {
+  if (out.p == in.p && out.ld == in.ld && out.esz == in.esz && out.rows == in.rows &&
+      out.cols == in.cols)
+    return MMN_OK;
+  if (matrices_overlap(out, in))
+    return fail(MMN_E_INVALID, std::string(what) + " overlaps an input it does not equal");
+  return MMN_OK;
+}
+
 // The device checks of the caller-buffer entry points: a usable sm_100 GPU.
 int percall_device(int device, int* sms) {
   int count = 0;

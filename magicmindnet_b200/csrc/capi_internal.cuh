@@ -92,11 +92,19 @@ int kernel_status_word(int device, int** p);
 // whose SM count goes to *sms.
 int percall_device(int device, int* sms);
 
-// An output matrix (rows x cols, row pitch in elements) may be one input (same
-// place, pitch and element size) or share no element with it; column slices
-// of one buffer share none. Else MMN_E_INVALID naming `what`.
-int check_out_overlap(const void* out, int64_t out_ld, size_t out_esz, const char* what,
-                      const void* in, int64_t in_ld, size_t in_esz, int64_t rows, int64_t cols);
+// A matrix of the caller: rows x cols elements of esz bytes, ld elements apart.
+struct MatrixIn {
+  const void* p;
+  int64_t ld, rows, cols;
+  size_t esz;
+};
+
+// Whether two matrices share bytes; column slices of one buffer do not.
+bool matrices_overlap(const MatrixIn& a, const MatrixIn& b);
+
+// An output matrix may be one input (same place, pitch and element size) or share
+// no element with it. Else MMN_E_INVALID naming `what`.
+int check_out_overlap(const MatrixIn& out, const char* what, const MatrixIn& in);
 
 // Rows of a matrix (pitch ld, esz-byte elements) can be read v elements at a
 // time: base and pitch are multiples of that access, 16 bytes at most.

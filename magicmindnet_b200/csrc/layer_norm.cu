@@ -1092,31 +1092,6 @@ int check_extent(int64_t rows, int64_t cols) {
 
 }  // namespace
 
-// A rows x cols matrix in memory, for the overlap rule of the caller-buffer calls.
-bool matrices_overlap(const void* p, int64_t ld, size_t esz, const void* q, int64_t qld,
-                      size_t qesz, int64_t rows, int64_t cols) {
-  const uintptr_t p0 = reinterpret_cast<uintptr_t>(p), q0 = reinterpret_cast<uintptr_t>(q);
-  const uintptr_t pw = (uintptr_t)cols * esz, qw = (uintptr_t)cols * qesz;
-  const uintptr_t ps = (uintptr_t)ld * esz, qs = (uintptr_t)qld * qesz;
-  const uintptr_t p1 = p0 + (uintptr_t)(rows - 1) * ps + pw, q1 = q0 + (uintptr_t)(rows - 1) * qs + qw;
-  if (p1 <= q0 || q1 <= p0) return false;
-  if (ps != qs || ps == 0) return true;
-  // same row pitch: column slices of one buffer may interleave
-  const uintptr_t d = q0 >= p0 ? (q0 - p0) % ps : (ps - (p0 - q0) % ps) % ps;
-  return !(d >= pw && d + qw <= ps);
-}
-
-// An output matrix may be one input (same place, pitch and element size) or
-// share no element with it.
-int check_out_overlap(const void* out, int64_t out_ld, size_t out_esz, const char* what,
-                      const void* in, int64_t in_ld, size_t in_esz, int64_t rows, int64_t cols) {
-  if (rows == 0 || cols == 0) return MMN_OK;
-  if (out == in && out_ld == in_ld && out_esz == in_esz) return MMN_OK;
-  if (matrices_overlap(out, out_ld, out_esz, in, in_ld, in_esz, rows, cols))
-    return fail(MMN_E_INVALID, std::string(what) + " overlaps an input it does not equal");
-  return MMN_OK;
-}
-
 }  // namespace mmn
 
 using namespace mmn;
@@ -1134,8 +1109,10 @@ extern "C" int mmn_layer_norm(const void* x, int64_t x_ld, int x_dtype, const vo
   if (!empty && (!x || !gamma || !beta || !y)) return fail(MMN_E_INVALID, "null pointer");
   if (rows > 1 && (x_ld < cols || y_ld < cols))
     return fail(MMN_E_INVALID, "a row pitch is smaller than cols");
-  if (!empty && (rc = check_out_overlap(y, y_ld, esize(y_dtype), "y", x, x_ld, esize(x_dtype),
-                                        rows, cols)) != MMN_OK)
+  if (mean && mean == rstd) return fail(MMN_E_INVALID, "mean and rstd are one buffer");
+  if (!empty && (rc = check_out_overlap({y, rows > 1 ? y_ld : cols, rows, cols, esize(y_dtype)},
+                                        "y", {x, rows > 1 ? x_ld : cols, rows, cols,
+                                              esize(x_dtype)})) != MMN_OK)
     return rc;
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
   if (empty) return MMN_OK;
@@ -1201,12 +1178,14 @@ extern "C" int mmn_layer_norm_backward(const void* dy, int64_t dy_ld, int dy_dty
   if (rows > 1 && (x_ld < cols || dy_ld < cols || dx_ld < cols))
     return fail(MMN_E_INVALID, "a row pitch is smaller than cols");
   if (dgamma == dbeta && cols > 0) return fail(MMN_E_INVALID, "dgamma and dbeta are one buffer");
-  if (!empty &&
-      ((rc = check_out_overlap(dx, dx_ld, esize(x_dtype), "dx", x, x_ld, esize(x_dtype), rows,
-                               cols)) != MMN_OK ||
-       (rc = check_out_overlap(dx, dx_ld, esize(x_dtype), "dx", dy, dy_ld, esize(dy_dtype), rows,
-                               cols)) != MMN_OK))
-    return rc;
+  if (!empty) {
+    const MatrixIn mdx{dx, rows > 1 ? dx_ld : cols, rows, cols, esize(x_dtype)};
+    if ((rc = check_out_overlap(mdx, "dx", {x, rows > 1 ? x_ld : cols, rows, cols,
+                                            esize(x_dtype)})) != MMN_OK ||
+        (rc = check_out_overlap(mdx, "dx", {dy, rows > 1 ? dy_ld : cols, rows, cols,
+                                            esize(dy_dtype)})) != MMN_OK)
+      return rc;
+  }
   if (!empty && reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(MMN_E_INVALID, "workspace is not 16-byte aligned");
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;

@@ -793,7 +793,11 @@ extern "C" int mmn_mxfp4_linear(const void* x, int64_t x_ld, int x_dtype, int64_
     if (ranges_meet(in[i], in[3]) || ranges_meet(in[i], in[4]))
       return fail(MMN_E_INVALID, "xq overlaps an input");
   if (ranges_meet(in[3], in[4])) return fail(MMN_E_INVALID, "xq's codes and scales overlap");
-  if ((rc = check_out(out, out_ld, out_dtype, rows, w->rows, in, 5)) != MMN_OK) return rc;
+  if ((rc = check_out(out, out_ld, out_dtype, rows, w->rows, in + 1, 4)) != MMN_OK) return rc;
+  // (x and out may be column slices of one buffer)
+  if (matrices_overlap({out, rows > 1 ? out_ld : w->rows, rows, w->rows, esize(out_dtype)},
+                       {x, rows > 1 ? x_ld : cols, rows, cols, esize(x_dtype)}))
+    return fail(MMN_E_INVALID, "the output overlaps x");
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
   if (rows == 0 || w->rows == 0) return MMN_OK;
   DeviceGuard guard(device);

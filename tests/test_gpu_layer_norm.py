@@ -250,6 +250,24 @@ def test_strided_unaligned_and_in_place(mmn, cols):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("rows,cols", [(270000, 8192), (70000, 32768)])
+def test_offsets_beyond_32_bits(mmn, rows, cols):
+    """More than 2^31 elements: the last rows, and the sums over all of them."""
+    import torch
+
+    x = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+    tail, gamma, beta, dyt = make(5, cols, "bf16", "bf16", seed=8)
+    x[-5:] = tail
+    y, mean, rstd = mmn.layer_norm(x, gamma, beta)
+    check_forward(y[-5:], mean[-5:], rstd[-5:], tail, gamma, beta, 1e-5)
+    assert torch.equal(y[0], beta.bfloat16()) and torch.equal(y[rows // 2], beta.bfloat16())
+    y.zero_()
+    y[-5:] = dyt  # now dy: nothing but in the last rows
+    out = mmn.layer_norm_backward(y, x, gamma, mean, rstd)
+    check_backward(out[0][-5:], out[1], out[2], dyt, tail, gamma, mean[-5:], rstd[-5:])
+    assert not out[0][:-5].any()
+
+
 def test_gradients_against_differences(mmn):
     """The directional derivative of sum(dy * layer_norm(x)) in 64 bits, central
     differences of step 1e-6 (their own error is about 1e-10), against the

@@ -161,3 +161,86 @@ def test_state_and_shape_errors(mmn):
     with pytest.raises(mmn.ShapeError):
         lin.backward(torch.zeros(4, D, device="cuda"))
     step.close()
+
+
+FIRST_CALLS = """
+import sys
+sys.path.insert(0, %r)
+import torch
+import magicmindnet_b200 as mmn
+x = torch.randn(300, 512, device="cuda").bfloat16()
+dy = torch.randn(300, 512, device="cuda").bfloat16()
+g, w = torch.ones(512, device="cuda"), torch.randn(512, 512, device="cuda")
+
+def block():
+    y, mean, rstd = mmn.layer_norm(x, g, g)
+    q, qt = mmn.mxfp4_quantize(w, "both")
+    z = mmn.mxfp4_linear(y, q)
+    z1 = mmn.mxfp4_linear(y[:1], q)
+    dq, dt = mmn.mxfp4_quantize(dy, "both")
+    dz = mmn.mxfp4_matmul(dq, qt)
+    dw = mmn.mxfp4_matmul(dt, mmn.mxfp4_quantize(y, "cols"), out_dtype=torch.float32)
+    return (z, z1, dw, q.dequantize()) + mmn.layer_norm_backward(dz, x, g, mean, rstd)
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):  # the very first calls of this process
+    got = block()
+for it in range(3):
+    x.copy_(torch.randn_like(x)); dy.copy_(torch.randn_like(dy))
+    graph.replay()
+    for a, b in zip(got, block()):
+        assert torch.equal(a, b)
+mmn.kernel_status()
+print("captured")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are being captured: nothing is allocated or set
+    up in a way that a capture forbids."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS % root], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+def test_two_graphs_at_once(mmn):
+    """Two captured passes over different data, replayed together on two streams:
+    each keeps its own workspaces."""
+    import torch
+
+    w = data(512, 384, "f32", 1, 0.5)
+    q, qt = mmn.mxfp4_quantize(w, "both")
+    g = torch.ones(384, device="cuda")
+
+    def passes(x, dy):
+        y, mean, rstd = mmn.layer_norm(x, g, g)
+        dq, dt = mmn.mxfp4_quantize(dy, "both")
+        dz = mmn.mxfp4_matmul(dq, qt)
+        dw = mmn.mxfp4_matmul(dt, mmn.mxfp4_quantize(y, "cols"), out_dtype=torch.float32)
+        return (mmn.mxfp4_linear(y, q), dw) + mmn.layer_norm_backward(dz, x, g, mean, rstd)
+
+    runs = []
+    for s in (1, 2):
+        x, dy = data(2000, 384, "bf16", s, 0.3), data(2000, 512, "bf16", s + 5, 0.3)
+        want = passes(x, dy)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = passes(x, dy)
+        # (x and dy stay: a graph keeps the addresses of its inputs, not the tensors)
+        runs.append((graph, got, want, torch.cuda.Stream(), x, dy))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, _, _, s, _, _ in runs:
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, got, want, _, _, _ in runs:
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    mmn.kernel_status()

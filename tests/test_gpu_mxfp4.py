@@ -262,6 +262,42 @@ def test_strided_and_unaligned_inputs(mmn):
         assert not out[:, :2].any() and not out[:, 2 + x.shape[1]:].any()
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("m,n,k", [(700, 1112, 512), (2000, 1304, 300), (40, 264, 512)])
+def test_aligned_slices_leave_their_neighbours(mmn, m, n, k, accumulate, out):
+    """Aligned column slices of a wider buffer (the widest stores) whose last tile
+    ends inside the slice: rows and columns around it stay as they were."""
+    import torch
+
+    a, b = data(m, k, "f32", 1, 1.0), data(n, k, "f32", 2, 1.0)
+    buf = torch.randn(m + 2, n + 24, device="cuda").to(T(out))
+    keep = buf.clone()
+    view = buf[1:1 + m, 8:8 + n]
+    mmn.mxfp4_matmul(mmn.mxfp4_quantize(a), mmn.mxfp4_quantize(b), out=view, accumulate=accumulate)
+    check_product(view, plain_values(a), plain_values(b),
+                  keep[1:1 + m, 8:8 + n] if accumulate else None)
+    outside = torch.ones_like(buf, dtype=torch.bool)
+    outside[1:1 + m, 8:8 + n] = False
+    assert torch.equal(buf[outside], keep[outside])
+
+
+@pytest.mark.parametrize("m", [3, 200])
+def test_linear_within_one_buffer(mmn, m):
+    """x and the result as column slices of one buffer; slices that meet are refused."""
+    import torch
+
+    w = data(96, 64, "f32", 6, 0.5)
+    q = mmn.mxfp4_quantize(w)
+    buf = data(m, 200, "bf16", 3, 1.0)
+    x, out = buf[:, :64], buf[:, 100:196]
+    want = mmn.mxfp4_linear(x.clone(), q)
+    assert mmn.mxfp4_linear(x, q, out=out) is out
+    assert torch.equal(out, want)
+    with pytest.raises(mmn.MmnError):
+        mmn.mxfp4_linear(x, q, out=buf[:, 63:159])
+
+
 def test_refill_in_place(mmn):
     import torch
 
