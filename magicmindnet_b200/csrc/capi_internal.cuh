@@ -106,6 +106,25 @@ bool matrices_overlap(const MatrixIn& a, const MatrixIn& b);
 // no element with it. Else MMN_E_INVALID naming `what`.
 int check_out_overlap(const MatrixIn& out, const char* what, const MatrixIn& in);
 
+// Launches a kernel as a programmatic dependent of the stream's previous one: it may
+// be scheduled while that one ends, and begins with griddep_wait, before which it
+// reads and writes nothing in global memory.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int block, size_t smem,
+                             cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Rows of a matrix (pitch ld, esz-byte elements) can be read v elements at a
 // time: base and pitch are multiples of that access, 16 bytes at most.
 inline bool vec_rows(const void* p, int64_t ld, size_t esz, int v) {

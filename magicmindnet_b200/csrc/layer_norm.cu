@@ -109,6 +109,8 @@ template <typename XT, typename YT, int V, int TR, int NE>
 __global__ void __launch_bounds__(TR <= 32 ? 128 : TR) ln_fwd_kernel(const LnFwd a) {
   constexpr int kBlock = TR <= 32 ? 128 : TR, RB = kBlock / TR, NC = NE / V;
   __shared__ float2 red[2][32];
+  griddep_wait();
+  griddep_launch_dependents();
   const int t = threadIdx.x % TR;
   const int64_t row = (int64_t)blockIdx.x * RB + threadIdx.x / TR;
   const bool ok = row < a.rows;
@@ -170,6 +172,8 @@ __global__ void __launch_bounds__(TR <= 32 ? 128 : TR) ln_fwd_kernel(const LnFwd
 template <typename XT, typename YT>
 __global__ void __launch_bounds__(512) ln_fwd_wide_kernel(const LnFwd a) {
   __shared__ float2 red[2][32];
+  griddep_wait();
+  griddep_launch_dependents();
   const int64_t row = blockIdx.x;
   const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
   YT* y = static_cast<YT*>(a.y) + row * a.y_ld;
@@ -337,6 +341,8 @@ __global__ void __launch_bounds__(ln_rows_block(TR), ln_rows_block(TR) > 512 ? 1
   const bool ok = row < a.rows;
   const int cols = ok ? (int)a.cols : 0;
   const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
+  griddep_wait();
+  griddep_launch_dependents();
   f2 v[NE / 2];
   f2 s = 0;
 #pragma unroll
@@ -423,6 +429,8 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR))
     mbar_arrive_expect_tx(&bars[sub][slot], rb);
     bulk_load(ring + slot * rb, x + k * step * a.x_ld, rb, &bars[sub][slot]);
   };
+  griddep_wait();
+  griddep_launch_dependents();
   if (t == 0)
     for (int k = 0; k < depth && k < mine; ++k) issue(k, k);
   f2 ga[NE / 2], be[NE / 2];
@@ -511,6 +519,8 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
     ln_bwd_kernel(const LnBwd a) {
   constexpr int kBlock = ln_bwd_block(TR), RB = kBlock / TR, NC = NE / V;
   __shared__ float2 red[2][32];
+  griddep_wait();
+  griddep_launch_dependents();
   const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
   const float inv_n = 1.0f / (float)a.cols;
   float sg[NE], sb[NE];  // dgamma, dbeta of this thread's columns
@@ -651,6 +661,7 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
   const int64_t mine = first < a.rows ? (a.rows - first + step - 1) / step : 0;
   const int64_t first0 = (int64_t)blockIdx.x * RB;
   const int64_t trips = first0 < a.rows ? (a.rows - first0 + step - 1) / step : 0;
+  griddep_wait();
   if (t == 0)
     for (int k = 0; k < depth && k < mine; ++k) issue(k, k);
   f2 ga[kReread ? 1 : NE / 2];
@@ -795,6 +806,8 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
 // or x), then dx row by row.
 template <typename XT, typename DT>
 __global__ void __launch_bounds__(128) ln_bwd_wide_cols_kernel(const LnBwd a, int64_t chunk) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int64_t c = (int64_t)blockIdx.x * 128 + threadIdx.x;
   if (c >= a.cols) return;
   const int64_t r0 = (int64_t)blockIdx.y * chunk, r1 = min(a.rows, r0 + chunk);
@@ -814,6 +827,8 @@ __global__ void __launch_bounds__(128) ln_bwd_wide_cols_kernel(const LnBwd a, in
 template <typename XT, typename DT>
 __global__ void __launch_bounds__(512) ln_bwd_wide_rows_kernel(const LnBwd a) {
   __shared__ float2 red[32];
+  griddep_wait();
+  griddep_launch_dependents();
   const int64_t row = blockIdx.x;
   const XT* x = static_cast<const XT*>(a.x) + row * a.x_ld;
   const DT* dy = static_cast<const DT*>(a.dy) + row * a.dy_ld;
@@ -892,14 +907,16 @@ constexpr int64_t kRingMaxCols = 16384;  // rows through shared memory
 template <typename XT, typename YT, int TR, int NE>
 void fwd_scalar(const LnFwd& a, cudaStream_t s) {
   constexpr int kBlock = TR <= 32 ? 128 : TR, RB = kBlock / TR;
-  ln_fwd_kernel<XT, YT, 1, TR, NE><<<(unsigned)((a.rows + RB - 1) / RB), kBlock, 0, s>>>(a);
+  launch_dependent(ln_fwd_kernel<XT, YT, 1, TR, NE>,
+                          dim3((unsigned)((a.rows + RB - 1) / RB)), kBlock, 0, s, a);
 }
 
 template <typename XT, typename YT, int TR, int NE>
 void fwd_rows(const LnFwd& a, cudaStream_t s) {
   constexpr int64_t kRows = ln_rows_block(TR) / TR;
-  ln_fwd_rows_kernel<XT, YT, TR, NE>
-      <<<(unsigned)((a.rows + kRows - 1) / kRows), ln_rows_block(TR), 0, s>>>(a);
+  launch_dependent(ln_fwd_rows_kernel<XT, YT, TR, NE>,
+                          dim3((unsigned)((a.rows + kRows - 1) / kRows)), ln_rows_block(TR), 0, s,
+                          a);
 }
 
 // Shared memory above 48 KB for a kernel, once per device (`done`: the devices
@@ -949,7 +966,8 @@ int ring_fwd_launch(const LnFwd& a, int sms, int device, cudaStream_t s) {
   // 8 rows 51.2 us, 3 rows 48.6 us)
   const int depth = (int)std::min<int64_t>(kFwdRing, (224 * 1024 / kBlocks - 4096) / (row * RB));
   const int64_t grid = std::min<int64_t>((a.rows + RB - 1) / RB, (int64_t)sms * kBlocks);
-  kernel<<<(unsigned)grid, ln_ring_block(TR), depth * row * RB, s>>>(a, depth, status);
+  launch_dependent(kernel, dim3((unsigned)grid), ln_ring_block(TR), depth * row * RB, s, a, depth,
+                   status);
   return MMN_OK;
 }
 
@@ -966,7 +984,7 @@ int fwd_types(const LnFwd& a, bool vec, bool ring, int sms, int device, cudaStre
     }
   }
   if (a.cols > kFwdMaxCols)
-    ln_fwd_wide_kernel<XT, YT><<<(unsigned)a.rows, 512, 0, s>>>(a);
+    launch_dependent(ln_fwd_wide_kernel<XT, YT>, dim3((unsigned)a.rows), 512, 0, s, a);
   else if (vec)
     fwd_width<XT, YT>(a, s);
   else if (a.cols <= 64)
@@ -1002,7 +1020,7 @@ int bwd_parts(int64_t rows, int64_t cols, int sms) {
 
 template <typename XT, typename DT, int V, int TR, int NE>
 void bwd_launch(const LnBwd& a, int parts, cudaStream_t s) {
-  ln_bwd_kernel<XT, DT, V, TR, NE><<<parts, ln_bwd_block(TR), 0, s>>>(a);
+  launch_dependent(ln_bwd_kernel<XT, DT, V, TR, NE>, dim3(parts), ln_bwd_block(TR), 0, s, a);
 }
 
 template <typename XT, typename DT, int V>
@@ -1046,7 +1064,7 @@ int ring_launch(const LnBwd& a, int parts, int depth, int smem, int* status, int
   auto* kernel = ln_bwd_ring_kernel<XT, DT, V, TR, NE>;
   const int rc = raise_smem(kernel, device, mu, done);
   if (rc != MMN_OK) return rc;
-  kernel<<<parts, ln_bwd_block(TR), smem, s>>>(a, depth, status);
+  launch_dependent(kernel, dim3(parts), ln_bwd_block(TR), smem, s, a, depth, status);
   return MMN_OK;
 }
 
@@ -1069,9 +1087,9 @@ int bwd_types(const LnBwd& a, int parts, bool vec, bool ring, int device, cudaSt
   }
   if (a.cols > kBwdMaxCols) {
     const int64_t chunk = (a.rows + parts - 1) / parts;
-    ln_bwd_wide_cols_kernel<XT, DT>
-        <<<dim3((unsigned)((a.cols + 127) / 128), (unsigned)parts), 128, 0, s>>>(a, chunk);
-    ln_bwd_wide_rows_kernel<XT, DT><<<(unsigned)a.rows, 512, 0, s>>>(a);
+    launch_dependent(ln_bwd_wide_cols_kernel<XT, DT>,
+                     dim3((unsigned)((a.cols + 127) / 128), (unsigned)parts), 128, 0, s, a, chunk);
+    launch_dependent(ln_bwd_wide_rows_kernel<XT, DT>, dim3((unsigned)a.rows), 512, 0, s, a);
   } else if (vec) {
     bwd_width<XT, DT, V>(a, parts, s);
   } else {
@@ -1231,15 +1249,7 @@ extern "C" int mmn_layer_norm_backward(const void* dy, int64_t dy_ld, int dy_dty
   if (parts == 0 && accumulate) return MMN_OK;  // no rows: the sums are zero
   LnSum su{static_cast<const float*>(workspace), dgamma, dbeta, cols, parts,
            grad_dtype == MMN_DTYPE_BF16, accumulate != 0};
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((cols + 31) / 32), 2, 1);
-  cfg.blockDim = dim3(1024, 1, 1);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, ln_bwd_sum_kernel, su));
+  MMN_CUDA_TRY(launch_dependent(ln_bwd_sum_kernel, dim3((unsigned)((cols + 31) / 32), 2), 1024, 0, s,
+                                su));
   return MMN_OK;
 }

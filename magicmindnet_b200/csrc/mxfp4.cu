@@ -291,6 +291,8 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const MxDequantArgs 
   constexpr int V = 16 / sizeof(T), NH = 256 / (32 * V), NR = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ct = blockIdx.x % a.nct, rt = blockIdx.x / a.nct;
+  griddep_wait();
+  griddep_launch_dependents();
   uint32_t w[NH][NR], s[NH][NR];
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
@@ -467,21 +469,12 @@ int launch_quantize(const void* x, int64_t ld, int dtype, int64_t rows, int64_t 
   a.vec = vec_rows(x, ld, esize(dtype), 16);
   const int64_t blocks = nrt * a.nct;
   if (blocks > (int64_t(1) << 31) - 1) return fail(MMN_E_SHAPE, "matrix too large");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.dynamicSmemBytes =
-      dtype == MMN_DTYPE_BF16 ? MxTile<__nv_bfloat16>::kSmem : MxTile<float>::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  const dim3 grid((unsigned)blocks);
   if (dtype == MMN_DTYPE_BF16)
-    MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_quantize_kernel<__nv_bfloat16>, a));
+    MMN_CUDA_TRY(launch_dependent(mx_quantize_kernel<__nv_bfloat16>, grid, 256,
+                                  MxTile<__nv_bfloat16>::kSmem, s, a));
   else
-    MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_quantize_kernel<float>, a));
+    MMN_CUDA_TRY(launch_dependent(mx_quantize_kernel<float>, grid, 256, MxTile<float>::kSmem, s, a));
   return MMN_OK;
 }
 
@@ -740,10 +733,9 @@ extern "C" int mmn_mxfp4_dequantize(const mmn_mxfp4* q, void* out, int64_t out_l
   const unsigned grid = (unsigned)blocks;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MMN_DTYPE_BF16)
-    mx_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+    MMN_CUDA_TRY(launch_dependent(mx_dequantize_kernel<__nv_bfloat16>, dim3(grid), 256, 0, s, a));
   else
-    mx_dequantize_kernel<float><<<grid, 256, 0, s>>>(a);
-  MMN_CUDA_TRY(cudaGetLastError());
+    MMN_CUDA_TRY(launch_dependent(mx_dequantize_kernel<float>, dim3(grid), 256, 0, s, a));
   return MMN_OK;
 }
 
