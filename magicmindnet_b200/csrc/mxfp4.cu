@@ -440,7 +440,8 @@ int kernel_setup(int device) {
       (rc = split_setup<64, 0>()) != MMN_OK || (rc = split_setup<128, 0>()) != MMN_OK ||
       (rc = split_setup<16, 1>()) != MMN_OK || (rc = split_setup<16, 2>()) != MMN_OK)
     return rc;
-  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_pair_kernel, smem, MxPair::kSmemBytes));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_pair_kernel<192>, smem, MxPair<192>::kSmemBytes));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_gemm_pair_kernel<256>, smem, MxPair<256>::kSmemBytes));
   if (device < 64) done |= uint64_t(1) << device;
   return MMN_OK;
 }
@@ -522,6 +523,7 @@ int launch_split(const mmn_mxfp4* a, const MxRows& rows, const mmn_mxfp4* w, int
 
 // The CTA pairs that fit on the GPU at once (a persistent grid must not exceed
 // them: a pair scheduled late would run its whole tile list after the others).
+// One CTA fills an SM, so both tile widths have the same number.
 int max_pairs(int sms, int* out) {
   static std::mutex mu;
   static int known_sms = 0, pairs = 0;  // every sm_100 device gives the same for its SM count
@@ -529,8 +531,8 @@ int max_pairs(int sms, int* out) {
   if (known_sms != sms) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (sms / 2), 1, 1);
-    cfg.blockDim = dim3(MxPair::kThreads, 1, 1);
-    cfg.dynamicSmemBytes = MxPair::kSmemBytes;
+    cfg.blockDim = dim3(MxPair<256>::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = MxPair<256>::kSmemBytes;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
@@ -538,7 +540,7 @@ int max_pairs(int sms, int* out) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    MMN_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, mx_gemm_pair_kernel, &cfg));
+    MMN_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, mx_gemm_pair_kernel<256>, &cfg));
     if (n <= 0) return fail(MMN_E_CUDA, "no CTA pair fits on the device");
     pairs = n < sms / 2 ? n : sms / 2;
     known_sms = sms;
@@ -547,16 +549,18 @@ int max_pairs(int sms, int* out) {
   return MMN_OK;
 }
 
-int launch_gemm_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int sms,
-                     cudaStream_t s) {
+template <int BN>
+int launch_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int pairs, cudaStream_t s) {
   CUtensorMap ta, tb, tsa, tsb, to;
   const int64_t runs = scale_blocks(a->cols) / 2;
   std::string err = encode_byte_rows(&ta, a->codes, code_pitch(a->cols), a->rows, 128);
-  if (err.empty()) err = encode_byte_rows(&tb, b->codes, code_pitch(b->cols), b->rows, 128);
+  if (err.empty()) err = encode_byte_rows(&tb, b->codes, code_pitch(b->cols), b->rows, BN / 2);
   if (err.empty()) err = encode_scale_runs(&tsa, a->scales, runs, (a->rows + 127) / 128, 1);
   if (err.empty()) err = encode_scale_runs(&tsb, b->scales, runs, (b->rows + 127) / 128, 2);
-  // bf16 values are added in the epilogue's registers: a TMA addition would round
-  // the product to bf16 before the sum
+  // Stores and fp32 additions go through the tensor map where the rows are aligned
+  // (TMA additions flush values below 2^-126 to zero). bf16 values are added in
+  // the epilogue's registers: a TMA addition would round the product to bf16
+  // before the sum.
   g.tma_out = g.vec && !(g.out_bf16 && g.accumulate);
   if (!g.tma_out)
     to = ta;
@@ -566,15 +570,13 @@ int launch_gemm_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int 
   g.M = (int)a->rows;
   g.N = (int)b->rows;
   g.num_kb = (int)((a->cols + 255) / 256);
-  g.tiles_n = (int)((b->rows + 255) / 256);
+  g.tiles_n = (int)((b->rows + BN - 1) / BN);
   const int64_t tiles_m = (a->rows + 255) / 256, tiles = tiles_m * g.tiles_n;
   if (tiles > (int64_t(1) << 30)) return fail(MMN_E_SHAPE, "product too large");
-  int pairs = 0, rc = max_pairs(sms, &pairs);
-  if (rc != MMN_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * (unsigned)(tiles < pairs ? tiles : pairs), 1, 1);
-  cfg.blockDim = dim3(MxPair::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = MxPair::kSmemBytes;
+  cfg.blockDim = dim3(MxPair<BN>::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = MxPair<BN>::kSmemBytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -584,9 +586,23 @@ int launch_gemm_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel, ta, tb, tsa, tsb, to, g,
+  MMN_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel<BN>, ta, tb, tsa, tsb, to, g,
                                   (int)tiles_m, (int)tiles));
   return MMN_OK;
+}
+
+int launch_gemm_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int sms,
+                     cudaStream_t s) {
+  int pairs = 0, rc = max_pairs(sms, &pairs);
+  if (rc != MMN_OK) return rc;
+  // The tile width whose whole waves take fewer clocks (the measured costs of a k
+  // block and of a tile, mxfp4_gemm.cuh): 4096 x 14336 x 4096 165.9 thousand clocks
+  // with 192 and 173.4 with 256, 4096 x 2048 x 8192 65.2 and 57.5.
+  const int64_t tm = (a->rows + 255) / 256, kb = (a->cols + 255) / 256;
+  const int64_t w192 = (tm * ((b->rows + 191) / 192) + pairs - 1) / pairs;
+  const int64_t w256 = (tm * ((b->rows + 255) / 256) + pairs - 1) / pairs;
+  return w192 * (464 * kb + 2000) < w256 * (591 * kb + 3100) ? launch_pair<192>(a, b, g, pairs, s)
+                                                             : launch_pair<256>(a, b, g, pairs, s);
 }
 
 int zero_out(void* out, int64_t ld, int64_t rows, int64_t cols, int dtype, cudaStream_t s) {

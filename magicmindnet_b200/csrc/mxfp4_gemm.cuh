@@ -531,31 +531,41 @@ __device__ __forceinline__ void mx_store_block(const MxGemmArgs& a, long long r0
 }
 
 // ---------------------------------------------------------------- CTA pairs
-// 256 x 256 tiles on CTA pairs, persistent: each CTA loads its 128 rows of A and
-// half of B's rows, and the scales of its rows of A and of all of B's.
-//
-// TMEM (512 columns): two accumulators of 256 columns that overlap by 120, and a
-// set of 24 columns of scales per stage (a stage that has been loaded again has
-// had its MMAs completed, so its scale columns are free too). The epilogue
-// drains the overlapping columns first and releases them, so the next tile's
-// MMAs start while the rest is still being stored.
+// 256 x BN tiles on CTA pairs, persistent: each CTA loads its 128 rows of A and half
+// of B's rows, and the scales of its rows of A and of all of B's. TMEM (512
+// columns) holds two accumulators and a set of 24 columns of scales per stage (a
+// stage that has been loaded again has had its MMAs completed, so its scale
+// columns are free too).
+//   BN = 192: the accumulators are apart, and no tile's MMAs wait for the epilogue
+//             of the one before.
+//   BN = 256: they overlap by 120 columns. The epilogue drains the shared columns
+//             first and releases them before it stores anything; the wait costs
+//             about 1900 clocks a tile, but a stage's operands serve a third more.
+// Measured (clocks): a k block 464 and 591, and 2000 and 3100 a tile, for 192 and
+// 256; launch_gemm_pair takes the cheaper for the number of waves. What bounds
+// them: a stage's operands cross shared memory at nearly its bandwidth (67 KB in
+// 512 tensor clocks for 256) and L2 delivers them at 0.85 of the rate measured
+// without MMAs; the SM clock settles at 1.65 GHz under the power cap.
+template <int BN>
 struct MxPair {
   static constexpr int kABytes = 128 * 128;
-  static constexpr int kBBytes = 128 * 128;
+  static constexpr int kBBytes = BN / 2 * 128;
   static constexpr int kTileBytes = kABytes + kBBytes;
   static constexpr int kSfBytes = 3 * 1024;
   static constexpr int kStageBytes = kTileBytes + kSfBytes;
   static constexpr int kStages = 5;
   static constexpr int kSfCols = 24;
   static constexpr int kSfCol = 512 - kStages * kSfCols;  // first column of the scales
-  static constexpr int kAcc1 = kSfCol - 256;  // first column of the second accumulator
+  static constexpr bool kOverlap = 2 * BN > kSfCol;
+  static constexpr int kAcc1 = kOverlap ? kSfCol - BN : BN;  // the second accumulator's first column
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kEpiWarpBytes = 4608;  // two 2 KB store boxes, or a 32 x 33 fp32 tile
   static constexpr int kEpiBytes = kEpiWarps * kEpiWarpBytes;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + 512 + kEpiBytes;
+  static_assert(BN == 192 || BN == 256, "tile widths");
   static_assert(kEpiWarpBytes >= 32 * 33 * 4 && kEpiWarpBytes % 512 == 0, "epilogue stage");
-  static_assert(256 - kAcc1 <= 128, "the epilogue releases four chunks of 32 columns first");
+  static_assert(!kOverlap || BN - kAcc1 <= 128, "the epilogue releases four chunks of 32 first");
   static_assert(kSmemBytes <= 232448, "shared memory per CTA");
 };
 
@@ -612,14 +622,15 @@ __device__ __forceinline__ void mx_store_tma(const CUtensorMap* map, uint8_t* st
   }
 }
 
-__global__ void __launch_bounds__(MxPair::kThreads, 1)
+template <int BN>
+__global__ void __launch_bounds__(MxPair<BN>::kThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
                         const __grid_constant__ CUtensorMap tm_b,
                         const __grid_constant__ CUtensorMap tm_sfa,
                         const __grid_constant__ CUtensorMap tm_sfb,
                         const __grid_constant__ CUtensorMap tm_out, const MxGemmArgs args,
                         int tiles_m, int num_tiles) {
-  using S = MxPair;
+  using S = MxPair<BN>;
   constexpr int STAGES = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -628,11 +639,11 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
   uint8_t* sfs = smem + STAGES * S::kTileBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(sfs + STAGES * S::kSfBytes);
   uint64_t* empty = full + STAGES;
-  uint64_t* tfull = full + 2 * STAGES;       // [2]
-  uint64_t* tempty = full + 2 * STAGES + 2;  // one phase per tile
-  uint64_t* drain = full + 2 * STAGES + 3;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + 2 * STAGES + 4);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(full + 2 * STAGES + 5);
+  uint64_t* tfull = full + 2 * STAGES;       // [2] MMA -> epilogue
+  uint64_t* tempty = full + 2 * STAGES + 2;  // [2] epilogue -> MMA
+  uint64_t* drain = full + 2 * STAGES + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + 2 * STAGES + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(full + 2 * STAGES + 6);
   uint8_t* epi = sfs + STAGES * S::kSfBytes + 512;  // 512-byte aligned, as the swizzle needs
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -647,7 +658,8 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
     }
     mbar_init(&tfull[0], 1);
     mbar_init(&tfull[1], 1);
-    mbar_init(tempty, 2 * S::kEpiWarps);  // one lane of every epilogue warp of the pair
+    for (int b = 0; b < 2; ++b)
+      mbar_init(&tempty[b], 2 * S::kEpiWarps);  // one lane of every epilogue warp of the pair
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -692,9 +704,10 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
           uint8_t* t = tiles + stage * S::kTileBytes;
           uint8_t* f = sfs + stage * S::kSfBytes;
           tma_load_3d_pair(t, &tm_a, fb, kb * 128, tm * 256 + (int)rank * 128, 0);
-          tma_load_3d_pair(t + S::kABytes, &tm_b, fb, kb * 128, tn * 256 + (int)rank * 128, 0);
+          tma_load_3d_pair(t + S::kABytes, &tm_b, fb, kb * 128, tn * BN + (int)rank * (BN / 2), 0);
           tma_load_3d_pair(f, &tm_sfa, fb, 0, kb, tm * 2 + (int)rank);
-          tma_load_3d_pair(f + 1024, &tm_sfb, fb, 0, kb, tn * 2);
+          // (two 128-row blocks of scales; an odd tile of 192 starts in the first one's middle)
+          tma_load_3d_pair(f + 1024, &tm_sfb, fb, 0, kb, tn * BN / 128);
         }
         issued |= 1u << stage;
         last = (last & ~(1u << stage)) | (phase << stage);
@@ -719,12 +732,20 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
   } else if (warp == 1) {
     if (leader) {
       const bool one = elect_one();
-      constexpr uint32_t id0 = umma_idesc_mxf4(256, 256, 0), id1 = umma_idesc_mxf4(256, 256, 1);
+      constexpr uint32_t id0 = umma_idesc_mxf4(256, BN, 0),
+                         id1 = umma_idesc_mxf4(256, BN, 1);
       int stage = 0, it = 0;  // it: tiles so far
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = group; ok && tile < num_tiles; tile += groups, ++it) {
-        const uint32_t acc = tmem_base + ((it & 1) ? S::kAcc1 : 0);
+        // apart: the accumulator's last tile has been read out of TMEM
+        if (!S::kOverlap && it > 1 && !mbar_wait_warp(&tempty[it & 1], ((it >> 1) - 1) & 1, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t acc = tmem_base + (it & 1) * S::kAcc1;
+        int tm, tn;
+        mx_tile(tile, tiles_m, args.tiles_n, tm, tn);
+        // (an odd tile of 192 starts 64 rows, two columns, into its scales)
+        const uint32_t sfb_row = BN == 192 && (tn & 1) ? 2 : 0;
         for (int kb = 0; kb < args.num_kb; ++kb) {
           if (!mbar_wait_warp(&full[stage], phase, abort_flag)) {
             ok = false;
@@ -744,10 +765,10 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
               tc_cp_scales_pair(sb + 8 * h + 4, umma_desc_scales(f + 2048 + 512 * h));
             }
           }
-          __syncwarp();
-          if (kb == 0 && it > 0) {
+          if (S::kOverlap && kb == 0 && it > 0) {
             // the columns that the previous tile's accumulator shares with this one
-            if (!mbar_wait_warp(tempty, (it - 1) & 1, abort_flag)) {
+            __syncwarp();
+            if (!mbar_wait_warp(&tempty[0], (it - 1) & 1, abort_flag)) {
               ok = false;
               break;
             }
@@ -759,7 +780,8 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
               const int h = kk >> 1;
               tc_mma_mxf4_pair(acc, umma_desc_sw128(t + kk * 32, 16, 1024),
                                umma_desc_sw128(t + S::kABytes + kk * 32, 16, 1024),
-                               (kk & 1) ? id1 : id0, sa + 4 * h, sb + 8 * h, (kb | kk) != 0);
+                               (kk & 1) ? id1 : id0, sa + 4 * h, sb + 8 * h + sfb_row,
+                               (kb | kk) != 0);
             }
             tc_commit_pair_mc(&empty[stage], 0x3);
           }
@@ -794,39 +816,52 @@ __global__ void __launch_bounds__(MxPair::kThreads, 1)
       const bool ready = mbar_wait(&tfull[it & 1], (it >> 1) & 1, abort_flag);
       if (!__all_sync(0xffffffffu, ready)) break;  // tcgen05.ld is warp-collective
       tc_fence_after();
-      const uint32_t acc = tmem_base + ((uint32_t)(sub * 32) << 16) + ((it & 1) ? S::kAcc1 : 0);
+      const uint32_t acc = tmem_base + ((uint32_t)(sub * 32) << 16) + (it & 1) * S::kAcc1;
       const int m0 = tm * 256 + (int)rank * 128 + sub * 32;
       const int mr = min(32, args.M - m0);
-      // The first accumulator shares its last columns with the second, that one
-      // its first: the outermost four of the eight 32-column chunks are read
-      // first, two a warp, and released before anything is stored.
-#pragma unroll 1
-      for (int i = 0; i < 4; i += 2) {
-        const int o0 = 2 * i + half, o1 = o0 + 2;
-        const int ch0 = (it & 1) ? o0 : 7 - o0, ch1 = (it & 1) ? o1 : 7 - o1;
-        float v[32], w[32];
-        tmem_ld_32x32b_x32(acc + ch0 * 32, v);
-        tmem_ld_32x32b_x32(acc + ch1 * 32, w);
-        tmem_ld_wait();
-        if (i == 0) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(tempty_leader);
+      auto store = [&](int ch, const float (&x)[32]) {
+        const int n0 = tn * BN + ch * 32, nr = min(32, args.N - n0);
+        if (mr <= 0 || nr <= 0) return;
+        if (args.tma_out) {
+          if (args.out_bf16)
+            mx_store_tma<true>(&tm_out, stg, n0, m0, false, x, buf);
+          else
+            mx_store_tma<false>(&tm_out, stg, n0, m0, args.accumulate, x, buf);
+        } else {
+          mx_store_block(args, m0, n0, mr, nr, x, reinterpret_cast<float*>(stg));
         }
-        auto store = [&](int ch, const float (&x)[32]) {
-          const int n0 = tn * 256 + ch * 32, nr = min(32, args.N - n0);
-          if (mr <= 0 || nr <= 0) return;
-          if (args.tma_out) {
-            if (args.out_bf16)
-              mx_store_tma<true>(&tm_out, stg, n0, m0, false, x, buf);
-            else
-              mx_store_tma<false>(&tm_out, stg, n0, m0, args.accumulate, x, buf);
-          } else {
-            mx_store_block(args, m0, n0, mr, nr, x, reinterpret_cast<float*>(stg));
-          }
-        };
-        store(ch0, v);
-        store(ch1, w);
+      };
+      auto release = [&](int b) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tempty_leader + b * 8);
+      };
+      if constexpr (S::kOverlap) {
+        // The first accumulator shares its last columns with the second, that one
+        // its first: the outermost four of the eight 32-column chunks are read
+        // first, two a warp, and released.
+#pragma unroll 1
+        for (int i = 0; i < 4; i += 2) {
+          const int o0 = 2 * i + half, o1 = o0 + 2;
+          const int ch0 = (it & 1) ? o0 : 7 - o0, ch1 = (it & 1) ? o1 : 7 - o1;
+          float v[32], w[32];
+          tmem_ld_32x32b_x32(acc + ch0 * 32, v);
+          tmem_ld_32x32b_x32(acc + ch1 * 32, w);
+          tmem_ld_wait();
+          if (i == 0) release(0);
+          store(ch0, v);
+          store(ch1, w);
+        }
+      } else {
+        constexpr int kChunks = BN / 32 / 2;  // 32-column chunks of a warp
+#pragma unroll 1
+        for (int i = 0; i < kChunks; ++i) {
+          float v[32];
+          tmem_ld_32x32b_x32(acc + (half * kChunks + i) * 32, v);
+          tmem_ld_wait();
+          if (i == kChunks - 1) release(it & 1);
+          store(half * kChunks + i, v);
+        }
       }
       tc_fence_before();
     }

@@ -187,7 +187,9 @@ PRODUCTS = [(1, 1, 1), (1, 128, 256), (3, 300, 100), (16, 129, 64), (17, 517, 10
             (32, 128, 2048), (33, 1000, 96), (64, 77, 4096), (100, 640, 333), (128, 128, 256),
             (129, 1, 512), (200, 300, 31), (256, 256, 1024), (300, 513, 2500), (513, 257, 4128),
             (1000, 31, 700), (2048, 16, 8192), (5, 2000, 14336), (777, 1030, 1999),
-            (512, 512, 256), (520, 264, 1000), (2304, 2560, 300)]
+            (512, 512, 256), (520, 264, 1000), (2304, 2560, 300),
+            # wide tiles of either width, one and several a CTA pair
+            (2304, 2048, 700), (2100, 2001, 520), (4100, 2000, 1000), (5000, 3001, 300)]
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
