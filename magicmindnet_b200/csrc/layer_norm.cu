@@ -8,10 +8,26 @@
 //   g = dy gamma, c1 = sum g / d, c2 = sum g h / d, dx = r (g - c1 - h c2)
 //   dgamma = sum over rows of dy h, dbeta = sum over rows of dy
 //
-// Bound by memory: a row is read once into registers, both sums of the
-// variance run over the registers (the second about the mean, so that a row
-// whose mean is large against its spread loses nothing), and the row is written
-// once. All statistics and sums are fp32; y and dx are rounded once.
+// Bound by memory: a row is read once, into registers or shared memory, the
+// squares are summed about the mean there (so that a row whose mean is large
+// against its spread loses nothing), and the row is written once. All statistics
+// and sums are fp32; y and dx are rounded once.
+//
+// Which kernel takes a call (measured on one B200, fractions of the 6.53 TB/s a
+// copy reaches):
+//   forward   ln_fwd_ring_kernel  bf16 rows, many and aligned: 16384 x 4096 in
+//                                 43.2 us (0.95), 70.6 us a row per block
+//             ln_fwd_rows_kernel  the rest of the rows that can be read four at a
+//                                 time: 16384 x 2048 fp32 to bf16 in 31.6 us (0.97)
+//             ln_fwd_kernel       rows at any alignment, one element at a time:
+//                                 3001 x 1013 fp32 in 7.4 us (0.50)
+//             ln_fwd_wide_kernel  rows beyond 16384
+//   backward  ln_bwd_ring_kernel  aligned rows of 65 to 16384: 16384 x 4096 bf16 in
+//                                 72.9 us (0.85) with the closing sums, 113 us with
+//                                 the rows loaded into registers
+//             ln_bwd_kernel       narrow rows and rows at any alignment up to 8192:
+//                                 3001 x 1013 fp32 in 19.7 us (0.28)
+//             ln_bwd_wide_*       the rest
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -104,10 +120,11 @@ struct LnBwd {
 };
 
 // ------------------------------------------------------------------- forward
-// TR threads hold one row, NE elements each, in chunks of V.
-template <typename XT, typename YT, int V, int TR, int NE>
+// Rows at any alignment: TR threads hold one row, NE elements each, taken one at a
+// time.
+template <typename XT, typename YT, int TR, int NE>
 __global__ void __launch_bounds__(TR <= 32 ? 128 : TR) ln_fwd_kernel(const LnFwd a) {
-  constexpr int kBlock = TR <= 32 ? 128 : TR, RB = kBlock / TR, NC = NE / V;
+  constexpr int kBlock = TR <= 32 ? 128 : TR, RB = kBlock / TR;
   __shared__ float2 red[2][32];
   griddep_wait();
   griddep_launch_dependents();
@@ -115,33 +132,21 @@ __global__ void __launch_bounds__(TR <= 32 ? 128 : TR) ln_fwd_kernel(const LnFwd
   const int64_t row = (int64_t)blockIdx.x * RB + threadIdx.x / TR;
   const bool ok = row < a.rows;
   const XT* x = static_cast<const XT*>(a.x) + (ok ? row : 0) * a.x_ld;
-  float v[NE];
+  float v[NE], s = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int64_t c = (int64_t)(i * TR + t) * V;
-    if (ok && c < a.cols) {
-      const Vec<XT, V> u = load_vec<XT, V>(x + c);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i * V + j] = to_f32(u.e[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i * V + j] = 0.0f;
-    }
+  for (int i = 0; i < NE; ++i) {
+    const int c = i * TR + t;
+    v[i] = ok && c < a.cols ? to_f32(x[c]) : 0.0f;
+    s += v[i];
   }
   const float n = (float)a.cols;
-  float s = 0.0f;
-#pragma unroll
-  for (int k = 0; k < NE; ++k) s += v[k];
   const float mean = row_sum<TR>(make_float2(s, 0.0f), red[0]).x / n;
   float q = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NC; ++i)
-    if ((int64_t)(i * TR + t) * V < a.cols) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = v[i * V + j] - mean;
-        q += d * d;
-      }
+  for (int i = 0; i < NE; ++i)
+    if (i * TR + t < a.cols) {
+      const float d = v[i] - mean;
+      q += d * d;
     }
   const float var = row_sum<TR>(make_float2(q, 0.0f), red[1]).x / n;
   const float rstd = 1.0f / sqrtf(var + a.eps);
@@ -152,17 +157,13 @@ __global__ void __launch_bounds__(TR <= 32 ? 128 : TR) ln_fwd_kernel(const LnFwd
   }
   YT* y = static_cast<YT*>(a.y) + row * a.y_ld;
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int64_t c = (int64_t)(i * TR + t) * V;
+  for (int i = 0; i < NE; ++i) {
+    const int c = i * TR + t;
     if (c < a.cols) {
-      float ga[V], be[V];
-      load_param<V>(a.gamma, a.param_bf16, c, ga);
-      load_param<V>(a.beta, a.param_bf16, c, be);
-      Vec<YT, V> o;
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        from_f32(o.e[j], (v[i * V + j] - mean) * rstd * ga[j] + be[j]);
-      *reinterpret_cast<Vec<YT, V>*>(y + c) = o;
+      float ga[1], be[1];
+      load_param<1>(a.gamma, a.param_bf16, c, ga);
+      load_param<1>(a.beta, a.param_bf16, c, be);
+      from_f32(y[c], (v[i] - mean) * rstd * ga[0] + be[0]);
     }
   }
 }
@@ -320,15 +321,16 @@ __device__ __forceinline__ float2 ring_sum2(float x, float y, float2* red) {
   }
 }
 
-constexpr int kRingMax = 4;  // rows in flight per row group, at most (more gained nothing)
+constexpr int kRingMax = 4;  // rows in flight per row group, at most (8 gained nothing)
 constexpr int kFwdRing = 2;  // ... in the forward kernel
 
 // The forward kernel for rows that can be read four elements at a time: TR threads
 // hold one row, NE columns each, a block a row (or a few short ones). Chunks of
 // four keep every access, the fp32 parameters' too, to whole consecutive lines
 // per warp. A block lives 2 to 3 us, most of it waiting, so what is in flight is
-// what the blocks on the GPU hold: enough for fp32 rows (16384 x 4096 in 80.6
-// us, 6.66 TB/s) and not for bf16 ones (64 us, 4.2 TB/s; ln_fwd_ring_kernel).
+// what the blocks on the GPU hold: enough for fp32 rows (16384 x 4096 in 79.3
+// us, 6.77 TB/s; 86 us with a third fewer blocks an SM) and not for bf16 ones (64
+// us, 4.2 TB/s; ln_fwd_ring_kernel).
 __host__ __device__ constexpr int ln_rows_block(int tr) { return tr <= 32 ? 128 : tr; }
 
 template <typename XT, typename YT, int TR, int NE>
@@ -898,8 +900,8 @@ __global__ void __launch_bounds__(1024) ln_bwd_sum_kernel(const LnSum a) {
 }
 
 // ------------------------------------------------------------------ dispatch
-// How a row is spread: the threads of a row by its width, so that a thread
-// holds 8 or 16 elements of a row.
+// How a row is spread: the threads of a row by its width, so that a thread holds 8
+// to 32 elements of it.
 constexpr int64_t kFwdMaxCols = 16384;
 constexpr int64_t kBwdMaxCols = 8192;    // rows in registers
 constexpr int64_t kRingMaxCols = 16384;  // rows through shared memory
@@ -907,16 +909,15 @@ constexpr int64_t kRingMaxCols = 16384;  // rows through shared memory
 template <typename XT, typename YT, int TR, int NE>
 void fwd_scalar(const LnFwd& a, cudaStream_t s) {
   constexpr int kBlock = TR <= 32 ? 128 : TR, RB = kBlock / TR;
-  launch_dependent(ln_fwd_kernel<XT, YT, 1, TR, NE>,
-                          dim3((unsigned)((a.rows + RB - 1) / RB)), kBlock, 0, s, a);
+  launch_dependent(ln_fwd_kernel<XT, YT, TR, NE>, dim3((unsigned)((a.rows + RB - 1) / RB)), kBlock,
+                   0, s, a);
 }
 
 template <typename XT, typename YT, int TR, int NE>
 void fwd_rows(const LnFwd& a, cudaStream_t s) {
   constexpr int64_t kRows = ln_rows_block(TR) / TR;
   launch_dependent(ln_fwd_rows_kernel<XT, YT, TR, NE>,
-                          dim3((unsigned)((a.rows + kRows - 1) / kRows)), ln_rows_block(TR), 0, s,
-                          a);
+                   dim3((unsigned)((a.rows + kRows - 1) / kRows)), ln_rows_block(TR), 0, s, a);
 }
 
 // Shared memory above 48 KB for a kernel, once per device (`done`: the devices
@@ -962,8 +963,8 @@ int ring_fwd_launch(const LnFwd& a, int sms, int device, cudaStream_t s) {
   if ((rc = raise_smem(kernel, device, mu, done)) != MMN_OK) return rc;
   if ((rc = kernel_status_word(device, &status)) != MMN_OK) return rc;
   const int64_t row = a.cols * (int64_t)sizeof(XT);
-  // more rows in flight than this cost bandwidth (16384 x 4096, 3 blocks an SM:
-  // 8 rows 51.2 us, 3 rows 48.6 us)
+  // more rows in flight cost bandwidth (16384 x 4096: 43.6 us with 2, 45.6 with 3,
+  // 47.2 with 4)
   const int depth = (int)std::min<int64_t>(kFwdRing, (224 * 1024 / kBlocks - 4096) / (row * RB));
   const int64_t grid = std::min<int64_t>((a.rows + RB - 1) / RB, (int64_t)sms * kBlocks);
   launch_dependent(kernel, dim3((unsigned)grid), ln_ring_block(TR), depth * row * RB, s, a, depth,

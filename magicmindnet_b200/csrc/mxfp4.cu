@@ -89,6 +89,10 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes
 // blocks of 32 along the rows, then down the columns, whose bytes are collected
 // in shared memory so that global memory sees 64 consecutive bytes per row of
 // codes. A tile gives exactly one 512-byte block of scales in each direction.
+// 8192 x 4096 bf16: rows 15.8 us, columns 15.8, both 21.7 (0.82, 0.82 and 0.73 of
+// a copy's rate); 16384 x 8192: 52, 53 and 74 us (1.0, 0.98, 0.85). What holds
+// "both" back are its instructions, 14 an element: issue slots 69% busy, the
+// shared-memory pipe 62%.
 template <typename T>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
   constexpr int kPitch = MxTile<T>::kPitch;
@@ -286,6 +290,7 @@ struct MxDequantArgs {
 // 32 rows x 256 columns per block. A lane turns four bytes into eight bf16, or two
 // bytes into four fp32 (in two halves of the columns), so that every store of a
 // warp is 512 consecutive bytes; the loads of a lane's rows are issued first.
+// 8192 x 4096: 16.6 us to bf16 (5.1 TB/s), 26.1 to fp32 (5.8 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const MxDequantArgs a) {
   constexpr int V = 16 / sizeof(T), NH = 256 / (32 * V), NR = 4;
