@@ -1128,11 +1128,15 @@ extern "C" int mmn_layer_norm(const void* x, int64_t x_ld, int x_dtype, const vo
   if (!empty && (!x || !gamma || !beta || !y)) return fail(MMN_E_INVALID, "null pointer");
   if (rows > 1 && (x_ld < cols || y_ld < cols))
     return fail(MMN_E_INVALID, "a row pitch is smaller than cols");
-  if (mean && mean == rstd) return fail(MMN_E_INVALID, "mean and rstd are one buffer");
-  if (!empty && (rc = check_out_overlap({y, rows > 1 ? y_ld : cols, rows, cols, esize(y_dtype)},
-                                        "y", {x, rows > 1 ? x_ld : cols, rows, cols,
-                                              esize(x_dtype)})) != MMN_OK)
-    return rc;
+  if (!empty) {
+    const MatrixIn mx{x, rows > 1 ? x_ld : cols, rows, cols, esize(x_dtype)};
+    const MatrixIn my{y, rows > 1 ? y_ld : cols, rows, cols, esize(y_dtype)};
+    const MatrixIn mm{mean, rows, mean ? 1 : 0, rows, 4}, mr{rstd, rows, rstd ? 1 : 0, rows, 4};
+    if ((rc = check_out_overlap(my, "y", mx)) != MMN_OK) return rc;
+    if (matrices_overlap(mm, mr) || matrices_overlap(mm, my) || matrices_overlap(mr, my) ||
+        matrices_overlap(mm, mx) || matrices_overlap(mr, mx))
+      return fail(MMN_E_INVALID, "mean or rstd overlaps another buffer");
+  }
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
   if (empty) return MMN_OK;
   DeviceGuard guard(device);
@@ -1196,7 +1200,9 @@ extern "C" int mmn_layer_norm_backward(const void* dy, int64_t dy_ld, int dy_dty
     return fail(MMN_E_INVALID, "null pointer");
   if (rows > 1 && (x_ld < cols || dy_ld < cols || dx_ld < cols))
     return fail(MMN_E_INVALID, "a row pitch is smaller than cols");
-  if (dgamma == dbeta && cols > 0) return fail(MMN_E_INVALID, "dgamma and dbeta are one buffer");
+  const MatrixIn mg{dgamma, cols, 1, cols, esize(grad_dtype)};
+  const MatrixIn mb{dbeta, cols, 1, cols, esize(grad_dtype)};
+  if (matrices_overlap(mg, mb)) return fail(MMN_E_INVALID, "dgamma and dbeta overlap");
   if (!empty) {
     const MatrixIn mdx{dx, rows > 1 ? dx_ld : cols, rows, cols, esize(x_dtype)};
     if ((rc = check_out_overlap(mdx, "dx", {x, rows > 1 ? x_ld : cols, rows, cols,
@@ -1204,6 +1210,8 @@ extern "C" int mmn_layer_norm_backward(const void* dy, int64_t dy_ld, int dy_dty
         (rc = check_out_overlap(mdx, "dx", {dy, rows > 1 ? dy_ld : cols, rows, cols,
                                             esize(dy_dtype)})) != MMN_OK)
       return rc;
+    if (matrices_overlap(mg, mdx) || matrices_overlap(mb, mdx))
+      return fail(MMN_E_INVALID, "dgamma or dbeta overlaps dx");
   }
   if (!empty && reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(MMN_E_INVALID, "workspace is not 16-byte aligned");
@@ -1212,6 +1220,16 @@ extern "C" int mmn_layer_norm_backward(const void* dy, int64_t dy_ld, int dy_dty
   if (workspace_bytes < (int64_t)parts * 2 * cols * 4)
     return fail(MMN_E_INVALID, "workspace is smaller than mmn_layer_norm_backward_workspace gives");
   if (cols == 0) return MMN_OK;
+  if (!empty) {
+    const MatrixIn mw{workspace, 2 * cols, parts, 2 * cols, 4};
+    const MatrixIn others[] = {mg, mb, {dx, rows > 1 ? dx_ld : cols, rows, cols, esize(x_dtype)},
+                               {x, rows > 1 ? x_ld : cols, rows, cols, esize(x_dtype)},
+                               {dy, rows > 1 ? dy_ld : cols, rows, cols, esize(dy_dtype)},
+                               {gamma, cols, 1, cols, esize(param_dtype)},
+                               {mean, rows, 1, rows, 4}, {rstd, rows, 1, rows, 4}};
+    for (const MatrixIn& m : others)
+      if (matrices_overlap(mw, m)) return fail(MMN_E_INVALID, "workspace overlaps another buffer");
+  }
   DeviceGuard guard(device);
   const struct { const void* p; int dt; const char* n; } ptrs[] = {
       {dy, dy_dtype, "dy"}, {x, x_dtype, "x"}, {gamma, param_dtype, "gamma"},

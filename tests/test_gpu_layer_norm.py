@@ -374,3 +374,9 @@ def test_refusals(mmn):
         torch.zeros_like(x).data_ptr(), 8, ws.data_ptr(), ws[8:].data_ptr(), 0, 0, ws.data_ptr(), 4,
         0, None)
     assert rc == N.MMN_E_INVALID  # workspace too small
+    big = torch.zeros(1 << 16, device="cuda")
+    rc = N.lib().mmn_layer_norm_backward(
+        x.data_ptr(), 8, 0, x.data_ptr(), 8, 0, g.data_ptr(), 0, m.data_ptr(), r.data_ptr(), 4, 8,
+        torch.zeros_like(x).data_ptr(), 8, big.data_ptr(), ws.data_ptr(), 0, 0, big.data_ptr(),
+        big.numel() * 4, 0, None)
+    assert rc == N.MMN_E_INVALID  # the workspace is also dgamma

@@ -17,9 +17,9 @@ def N():
 
 
 def fwd(N, x=X, x_ld=64, xd=F32, gamma=G, beta=B, pd=F32, eps=1e-5, rows=4, cols=64, y=Y, y_ld=64,
-        yd=F32, device=0):
-    return N.lib().mmn_layer_norm(x, x_ld, xd, gamma, beta, pd, eps, rows, cols, y, y_ld, yd, M, R,
-                                  device, None)
+        yd=F32, mean=M, rstd=R, device=0):
+    return N.lib().mmn_layer_norm(x, x_ld, xd, gamma, beta, pd, eps, rows, cols, y, y_ld, yd, mean,
+                                  rstd, device, None)
 
 
 def bwd(N, dy=Y, dy_ld=64, dd=F32, x=X, x_ld=64, xd=F32, gamma=G, pd=F32, mean=M, rstd=R, rows=4,
@@ -44,6 +44,7 @@ def gate(N):
     dict(y=X, yd=BF16),                     # in place, but of another element size
     dict(y=X, y_ld=128, x_ld=64),           # in place, but of another pitch
     dict(x_ld=100, y_ld=100, y=vp(0x100000 + 4 * 63)),  # slices that share a column
+    dict(mean=R), dict(mean=vp(0x600000 + 12)), dict(rstd=vp(0x200000 + 64)), dict(mean=X),
 ])
 def test_forward_refusals(N, kw):
     assert fwd(N, **kw) == N.MMN_E_INVALID
@@ -58,6 +59,7 @@ def test_forward_too_large_is_a_shape_error(N):
 @pytest.mark.parametrize("kw", [
     dict(), dict(y=X), dict(x_ld=128, y_ld=128, y=vp(0x100000 + 4 * 64)),  # slices side by side
     dict(rows=1, x_ld=0, y_ld=-5),  # the pitch of a single row is not read
+    dict(mean=None), dict(rstd=None), dict(mean=None, rstd=None), dict(mean=vp(0x600000 + 16)),
 ])
 def test_forward_allowed_up_to_the_device(N, kw):
     assert fwd(N, **kw) == gate(N)
@@ -69,6 +71,7 @@ def test_forward_allowed_up_to_the_device(N, kw):
     dict(dgamma=None), dict(dbeta=None), dict(ws=None), dict(ws=vp(0xC00004)), dict(x_ld=63),
     dict(dy_ld=63), dict(dx_ld=63), dict(dgamma=vp(0xB00000)),
     dict(dx=vp(0x100000 + 4)), dict(dx=Y, dd=BF16),
+    dict(dgamma=vp(0xB00000 + 4 * 63)), dict(dbeta=vp(0x900000 + 8)), dict(dgamma=vp(0x900000)),
 ])
 def test_backward_refusals(N, kw):
     assert bwd(N, **kw) == N.MMN_E_INVALID
