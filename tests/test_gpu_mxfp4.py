@@ -78,7 +78,9 @@ def check_product(out, a, b, base=None):
 
 
 SHAPES = [(1, 1), (1, 32), (2, 33), (31, 31), (32, 64), (33, 95), (127, 129), (128, 128),
-          (129, 257), (256, 512), (300, 520), (1000, 1030), (1, 5000), (5000, 1), (70, 2048)]
+          (129, 257), (256, 512), (300, 520), (1000, 1030), (1, 5000), (5000, 1), (70, 2048),
+          # more tiles than the GPU takes at once, an odd and an even number each way
+          (2890, 2888), (3000, 3208), (100000, 72), (5, 100000)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -142,6 +144,20 @@ def test_rounding_of_every_midpoint(mmn):
         same(mmn.mxfp4_quantize(y).dequantize(), plain_values(y), e)
         yt = y.t().contiguous()
         same(mmn.mxfp4_quantize(yt, "cols").dequantize(), plain_values(y), e)
+
+
+def test_non_finite_and_strided_in_many_tiles(mmn):
+    """The walk over many tiles: a slice of a wider buffer, Inf and NaN in its
+    corners and edges."""
+    import torch
+
+    buf = data(2900, 3100, "bf16", 4, 1.0)
+    x = buf[10:2890, 16:3072]
+    x[0, 0], x[-1, -1], x[128, 127], x[1500, 3055] = (float("nan"), float("inf"), -float("inf"),
+                                                      float("nan"))
+    q, qt = mmn.mxfp4_quantize(x, "both")
+    same(q.dequantize(), plain_values(x))
+    same(qt.dequantize(torch.bfloat16), plain_values(x.t()))
 
 
 def test_smallest_and_largest_magnitudes(mmn):
