@@ -90,9 +90,9 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes
 // in shared memory so that global memory sees 64 consecutive bytes per row of
 // codes. A tile gives exactly one 512-byte block of scales in each direction.
 // 8192 x 4096 bf16: rows 15.8 us, columns 15.8, both 21.7 (0.82, 0.82 and 0.73 of
-// a copy's rate); 16384 x 8192: 52, 53 and 74 us (1.0, 0.98, 0.85). What holds
-// "both" back are its instructions, 14 an element: issue slots 69% busy, the
-// shared-memory pipe 62%.
+// a copy's rate); 16384 x 8192: 52, 53 and 74 us (1.0, 0.98, 0.85). With few waves
+// of blocks their loads and their work fall together; within a block "both" is 14
+// instructions an element (issue slots 69% busy, the shared-memory pipe 62%).
 template <typename T>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
   constexpr int kPitch = MxTile<T>::kPitch;
