@@ -34,11 +34,11 @@ class Mxfp4Matrix:
         code_bytes = rows * ((cols + 31) // 32 * 16)
         total = code_bytes + ((rows + 127) // 128 * ((cols + 255) // 256) * 1024)
         self.shape = (rows, cols)
-        self._buf = torch.empty(total, dtype=torch.uint8, device=device)
-        self.device = self._buf.device
-        self._index = self._buf.get_device()
+        self._buf = buf = torch.empty(total, dtype=torch.uint8, device=device)
+        self.device = buf.device
+        self._index = buf.get_device()
         self._code_bytes = code_bytes
-        ptr = self._buf.data_ptr()
+        ptr = buf.data_ptr()
         self._c = N.Mxfp4C(ptr, ptr + code_bytes, rows, cols)
 
     @property

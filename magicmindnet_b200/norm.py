@@ -65,6 +65,8 @@ def _rows_view(t, what: str):
     if not shape:
         raise ValueError(f"{what}: expected at least one axis")
     cols = shape[-1]
+    if cols and t.is_contiguous():
+        return t.numel() // cols, cols, cols
     rows = 1
     for n in shape[:-1]:
         rows *= n
@@ -90,10 +92,11 @@ def _rows_view(t, what: str):
 
 def _vector(t, n: int, what: str, index: int) -> int:
     """dtype of a contiguous vector of n elements on a GPU."""
+    if isinstance(t, _t.Tensor) and t.get_device() == index and t.dim() == 1 \
+            and t.numel() == n and t.is_contiguous():
+        return _dtypes.get(t.dtype) or _dtype(t, what)
     _on_gpu(t, what, index)
-    if t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous vector of {n} elements")
-    return _dtype(t, what)
+    raise ValueError(f"{what}: expected a contiguous vector of {n} elements")
 
 
 def layer_norm(x, gamma, beta, eps: float = 1e-5, out_dtype=None, out=None):
@@ -118,7 +121,11 @@ def layer_norm(x, gamma, beta, eps: float = 1e-5, out_dtype=None, out=None):
         if out.shape != x.shape or (out_dtype is not None and out.dtype != out_dtype):
             raise N.ShapeError(N.MMN_E_SHAPE, "out must have x's shape (and out_dtype)")
         old = _rows_view(out, "out")[2]
-    mean, rstd = _t.empty(2, *x.shape[:-1], dtype=_t.float32, device=x.device).unbind(0)
+    dev = x.device
+    if x.dim() == 2:
+        mean, rstd = _t.empty(2, rows, dtype=_t.float32, device=dev).unbind(0)
+    else:
+        mean, rstd = _t.empty(2, *x.shape[:-1], dtype=_t.float32, device=dev).unbind(0)
     if cols == 0:
         mean.zero_()
         rstd.fill_(float("inf") if eps == 0 else eps ** -0.5)
@@ -153,13 +160,15 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, dgamma=None, dbeta=None,
     dev = x.device
     if dgamma is None and dbeta is None:
         dgamma, dbeta = _t.empty(2, cols, dtype=_t.float32, device=dev).unbind(0)
-    elif dgamma is None:
-        dgamma = _t.empty(cols, dtype=dbeta.dtype, device=dev)
-    elif dbeta is None:
-        dbeta = _t.empty(cols, dtype=dgamma.dtype, device=dev)
-    gd = _vector(dgamma, cols, "dgamma", index)
-    if _vector(dbeta, cols, "dbeta", index) != gd:
-        raise TypeError("dgamma and dbeta must have one dtype")
+        gd = N.DTYPE_F32
+    else:
+        if dgamma is None:
+            dgamma = _t.empty(cols, dtype=dbeta.dtype, device=dev)
+        elif dbeta is None:
+            dbeta = _t.empty(cols, dtype=dgamma.dtype, device=dev)
+        gd = _vector(dgamma, cols, "dgamma", index)
+        if _vector(dbeta, cols, "dbeta", index) != gd:
+            raise TypeError("dgamma and dbeta must have one dtype")
     if out is None:
         out = _t.empty_like(x) if ld == cols else _t.empty(*x.shape, dtype=x.dtype, device=dev)
         old = cols
