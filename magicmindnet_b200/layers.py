@@ -6,9 +6,12 @@ v, out, ffn, ffn2 matrices).
 ``forward`` keeps what ``backward`` needs; ``backward`` returns the input's
 gradient and writes the weights' gradients into the step's grad slots, where
 ``OptimizerStep.step`` reads them. ``accumulate=True`` adds to the slots instead
-(the second and later micro-batches of a step). Work is enqueued on torch's
-current stream, which must be the one the step was made on (or ordered with
-it), as for ``OptimizerStep.param`` and ``.grad`` views.
+(the second and later micro-batches of a step). A layer holds one forward pass
+at a time: the next one before its ``backward`` (or ``discard``) is refused.
+``training=False`` holds nothing. Work is enqueued on torch's current stream,
+which must be the one the step was made on (or ordered with it), as for
+``OptimizerStep.param`` and ``.grad`` views; like those, a layer is of no use
+after the step is closed.
 """
 from __future__ import annotations
 
@@ -17,7 +20,30 @@ from .mxfp4 import Mxfp4Matrix, mxfp4_linear, mxfp4_matmul, mxfp4_quantize
 from .norm import layer_norm, layer_norm_backward
 
 
-class LayerNorm:
+class _Layer:
+    """What a forward pass leaves for its backward pass."""
+
+    _saved = None
+
+    def _hold(self, saved) -> None:
+        self._saved = saved
+
+    def _free(self) -> None:
+        if self._saved is not None:
+            raise N.MmnError(N.MMN_E_STATE, "a forward pass still waits for its backward pass "
+                                            "(discard() drops it)")
+
+    def _held(self):
+        if self._saved is None:
+            raise N.MmnError(N.MMN_E_STATE, "backward without a forward pass")
+        return self._saved
+
+    def discard(self) -> None:
+        """Drops the forward pass that waits for its backward pass, if any."""
+        self._saved = None
+
+
+class LayerNorm(_Layer):
     """Layer norm with the gain in `gamma_slot` and the shift in `beta_slot`."""
 
     def __init__(self, step, gamma_slot: int, beta_slot: int, eps: float = 1e-5):
@@ -27,24 +53,26 @@ class LayerNorm:
         self.step, self.gamma_slot, self.beta_slot, self.eps = step, gamma_slot, beta_slot, eps
         self._gamma, self._beta = step.forward_param(gamma_slot), step.forward_param(beta_slot)
         self._dgamma, self._dbeta = step.grad(gamma_slot), step.grad(beta_slot)
-        self._saved = None
 
-    def forward(self, x, out_dtype=None):
+    def forward(self, x, training: bool = True, out_dtype=None):
+        """The norm of x [..., d]; x itself is kept for backward and must not change
+        before it."""
+        if training:
+            self._free()
         y, mean, rstd = layer_norm(x, self._gamma, self._beta, self.eps, out_dtype)
-        self._saved = (x, mean, rstd)
+        if training:
+            self._hold((x, mean, rstd))
         return y
 
     def backward(self, dy, accumulate: bool = False):
-        if self._saved is None:
-            raise N.MmnError(N.MMN_E_STATE, "backward without a forward pass")
-        x, mean, rstd = self._saved
+        x, mean, rstd = self._held()
         dx, _, _ = layer_norm_backward(dy, x, self._gamma, mean, rstd, self._dgamma, self._dbeta,
                                        accumulate)
         self._saved = None
         return dx
 
 
-class Linear:
+class Linear(_Layer):
     """y = x W^T with W [out, in] in `slot`. The forward pass and both gradient
     products run on 4-bit operands; the weight's 4-bit copies (W for the forward
     pass, W transposed for the input's gradient) are made by ``refresh``, which
@@ -61,11 +89,11 @@ class Linear:
         dev = torch.device("cuda", step.device)
         self.w = Mxfp4Matrix(shape[0], shape[1], dev)
         self.wt = Mxfp4Matrix(shape[1], shape[0], dev)
-        self._saved = None
         self.refresh()
 
     def refresh(self) -> None:
-        """Both 4-bit copies from the slot's present values, in place (one read)."""
+        """Both 4-bit copies from the slot's present values, in place (one read). On
+        several ranks: after the fence that ends the step's parameter exchange."""
         mxfp4_quantize(self._param, "both", out=(self.w, self.wt))
 
     def forward(self, x, training: bool = True, out_dtype=None):
@@ -75,15 +103,14 @@ class Linear:
         if x.shape[-1] != self.w.shape[1]:
             raise N.ShapeError(N.MMN_E_SHAPE,
                                f"x has {x.shape[-1]} columns, the weight {self.w.shape[1]}")
+        self._free()
         xq, xt = mxfp4_quantize(_as_matrix(x), "both")
-        self._saved = xt, x.dtype, x.shape
         y = mxfp4_matmul(xq, self.w, out_dtype=out_dtype or x.dtype)
+        self._hold((xt, x.dtype, x.shape))
         return y.view(tuple(x.shape[:-1]) + (self.w.shape[0],))
 
     def backward(self, dy, accumulate: bool = False):
-        if self._saved is None:
-            raise N.MmnError(N.MMN_E_STATE, "backward without a forward pass")
-        xt, dtype, shape = self._saved
+        xt, dtype, shape = self._held()
         want = tuple(shape[:-1]) + (self.w.shape[0],)
         if tuple(dy.shape) != want:
             raise N.ShapeError(N.MMN_E_SHAPE, f"dy is {tuple(dy.shape)}, expected {want}")

@@ -157,9 +157,21 @@ def test_state_and_shape_errors(mmn):
             layer.backward(torch.zeros(4, D, device="cuda"))
     with pytest.raises(mmn.ShapeError):
         lin.forward(torch.zeros(4, D + 1, device="cuda"))
-    lin.forward(torch.zeros(4, D, device="cuda"))
+    x = torch.zeros(4, D, device="cuda")
+    for layer in (lin, ln):
+        layer.forward(x)
+        layer.forward(x, training=False)  # holds nothing
+        with pytest.raises(mmn.MmnError):  # the first pass still waits
+            layer.forward(x)
     with pytest.raises(mmn.ShapeError):
-        lin.backward(torch.zeros(4, D, device="cuda"))
+        lin.backward(x)
+    lin.discard()
+    lin.forward(x)
+    lin.backward(torch.zeros(4, FFN, device="cuda"))
+    with pytest.raises(mmn.MmnError):  # held once, used once
+        lin.backward(torch.zeros(4, FFN, device="cuda"))
+    with pytest.raises(TypeError):
+        lin.forward(torch.zeros(4, D))  # host memory
     step.close()
 
 
