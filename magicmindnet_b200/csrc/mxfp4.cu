@@ -22,6 +22,7 @@
 
 #include "capi_internal.cuh"
 #include "ns_engine.cuh"
+#include "unaligned.cuh"
 
 namespace mmn {
 namespace {
@@ -137,11 +138,44 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
     }
     asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
   } else {
-    for (int id = tid; id < 128 * 128; id += 256) {
-      const int r = id >> 7, c = id & 127;
-      T v = T(0.0f);
-      if (r < nr && c < nc) v = x[(int64_t)(r0 + r) * a.ld + c0 + c];
-      *reinterpret_cast<T*>(sm + r * kPitch + c * sizeof(T)) = v;
+    // Rows that start anywhere arrive in whole vectors, the tile's first element o
+    // elements into the first (one vector more a row), and move to their place
+    // within shared memory. o is the same in every row of a thread: they lie a
+    // multiple of a vector's elements apart. 16384 x 4095 bf16 43 us, fp32 73 (80 and
+    // 128 with an element a load; 55 and 123 with the vectors moved in registers
+    // on their way to shared memory, which leaves fewer loads in flight).
+    constexpr int kPer = 16 / sizeof(T), kCh = 128 / kPer, kRows = 256 / kCh;
+    static_assert(kRows % kPer == 0, "rows of a thread differ in their offset");
+    auto copy = [&](int r, int j) {
+      const T* row = x + (int64_t)(r0 + r) * a.ld + c0;
+      const int c = j * kPer - vec_offset<T, kPer>(row);  // the vector's first column
+      uint8_t* dst = sm + r * kPitch + j * 16;
+      if (r < nr && c + c0 < 0 && row + c < x) {  // the matrix starts inside this vector
+        for (int k = 0; k < kPer; ++k)
+          if (row + c + k >= x && c + k < nc) reinterpret_cast<T*>(dst)[k] = row[c + k];
+      } else {
+        const int bytes = r < nr ? max(0, min(kPer, a.cols - c0 - c)) * (int)sizeof(T) : 0;
+        cp_async16(dst, bytes ? row + c : x - vec_offset<T, kPer>(x), bytes);
+      }
+    };
+    const int r1 = tid / kCh, j1 = tid % kCh;
+#pragma unroll
+    for (int i = 0; i < 128 / kRows; ++i) copy(i * kRows + r1, j1);
+    if (tid < 128) copy(tid, kCh);
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    const int o = vec_offset<T, kPer>(x + (int64_t)(r0 + r1) * a.ld + c0);
+#pragma unroll
+    for (int i = 0; i < 128 / kRows; ++i) {
+      // (the lanes of a warp take whole rows)
+      uint4* at = reinterpret_cast<uint4*>(sm + (i * kRows + r1) * kPitch) + j1;
+      const uint4 u = at[0], v = at[1];
+      const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      uint32_t m[4];
+      shift_down<T, kPer>(w, o, m);
+      if (c0 + 128 > a.cols) keep_first<T, kPer>(m, nc - j1 * kPer);
+      __syncwarp();
+      at[0] = make_uint4(m[0], m[1], m[2], m[3]);
     }
   }
   __syncthreads();
@@ -289,74 +323,114 @@ struct MxDequantArgs {
   int64_t ld, pitch;
   int rows, cols;
   int ka;
-  int nct;  // 256-column tiles
-  int vec;
+  int nct;  // column tiles
 };
 
-// 32 rows x 256 columns per block. A lane turns four bytes into eight bf16, or two
-// bytes into four fp32 (in two halves of the columns), so that every store of a
-// warp is 512 consecutive bytes; the loads of a lane's rows are issued first.
-// 8192 x 4096: 15.6 us to bf16 (5.4 TB/s), 26.1 to fp32 (5.8 TB/s).
-template <typename T>
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// 32 rows x 512 (bf16) or 256 (fp32) columns per block. A lane turns the codes of 32
+// output bytes into one store, so that every sector is written whole; the loads of
+// a lane's rows are issued first, without branches between them (what lies outside
+// is read from the edge and not used). 16384 x 4096: 27.4 us to bf16, 48.6 to fp32
+// (0.95 and 0.96 of a copy's rate; 29.8 and 49.0 with 16-byte stores).
+// SHIFT: output rows that start anywhere. A lane's columns begin where the row's
+// memory is aligned, o columns before its codes; the codes are moved by o nibbles,
+// and the first o values may belong to the block before. 16384 x 4095: 38.9 and
+// 49.5 us (187 and 89 with an element a store).
+template <typename T, bool SHIFT>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const MxDequantArgs a) {
-  constexpr int V = 16 / sizeof(T), NH = 256 / (32 * V), NR = 4;
+  constexpr int V = 32 / sizeof(T), W = V / 8, NR = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ct = blockIdx.x % a.nct, rt = blockIdx.x / a.nct;
   griddep_wait();
   griddep_launch_dependents();
-  uint32_t w[NH][NR], s[NH][NR];
+  T* const out = static_cast<T*>(a.out) + (int64_t)(rt * 32 + warp) * a.ld;
+  // of a lane's rows, eight apart: V divides 8 or 16 of them
+  static_assert(V == 8 || V == 16, "offsets of a lane's rows");
+  const int o2[2] = {SHIFT ? vec_offset<T, V>(out) : 0,
+                     SHIFT ? vec_offset<T, V>(out + 8 * a.ld) : 0};
+  // the lane's codes and those before
+  const int at = (ct * 32 + lane) * V, top = (a.cols - 1) / 32 * 32 + 32 - V;
+  const int e = min(at, top), f = max(min(at - V, top), 0);
+  const uint8_t* const scales = a.scales + (int64_t)(rt >> 2) * a.ka * 512 + (rt & 3) * 4;
+  const uint8_t* const se = scales + (int64_t)(e >> 7) * 512 + ((e >> 5) & 3);
+  const uint8_t* const sf = scales + (int64_t)(f >> 7) * 512 + ((f >> 5) & 3);
+  uint32_t w[NR][2 * W], s[NR], sp[NR];  // w: the codes before, the codes
 #pragma unroll
-  for (int h = 0; h < NH; ++h) {
-    const int c = ct * 256 + (h * 32 + lane) * V;
-    const uint8_t* sc = a.scales + ((int64_t)(rt >> 2) * a.ka + (c >> 7)) * 512 + (rt & 3) * 4 +
-                        ((c >> 5) & 3);
-#pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const int rr = warp + 8 * i;
-      w[h][i] = s[h][i] = 0;
-      if (c < a.cols && rt * 32 + rr < a.rows) {
-        const uint8_t* p = a.codes + (int64_t)(rt * 32 + rr) * a.pitch + c / 2;
-        w[h][i] = V == 8 ? *reinterpret_cast<const uint32_t*>(p)
-                         : *reinterpret_cast<const uint16_t*>(p);
-        s[h][i] = sc[rr * 16];
+  for (int i = 0; i < NR; ++i) {
+    const int rr = min(rt * 32 + warp + 8 * i, a.rows - 1) & 31;
+    const uint32_t* p =
+        reinterpret_cast<const uint32_t*>(a.codes + (int64_t)(rt * 32 + rr) * a.pitch);
+    if constexpr (W == 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p + e / 8);
+      w[i][2] = u.x, w[i][3] = u.y;
+      if constexpr (SHIFT) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p + f / 8);
+        w[i][0] = v.x, w[i][1] = v.y;
       }
+    } else {
+      w[i][1] = p[e / 8];
+      if constexpr (SHIFT) w[i][0] = p[f / 8];
     }
+    s[i] = se[rr * 16];
+    if constexpr (SHIFT) sp[i] = sf[rr * 16];
   }
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    const int r = rt * 32 + warp + 8 * i;
+    const int r = rt * 32 + warp + 8 * i, o = o2[i & 1], c = at - o;
     if (r >= a.rows) break;
+    uint32_t x[W], v[8];
+    if constexpr (!SHIFT) {
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      const int c = ct * 256 + (h * 32 + lane) * V;
-      if (c >= a.cols) break;
-      T* o = static_cast<T*>(a.out) + (int64_t)r * a.ld + c;
-      alignas(16) T v[V];
-      if constexpr (sizeof(T) == 2) {
-        // a value times its scale is a bf16 (down to 2^-128), so the product is exact
-        const uint32_t f = mx_scale_bf16x2(s[h][i]);
-        uint32_t* u = reinterpret_cast<uint32_t*>(v);
+      for (int k = 0; k < W; ++k) x[k] = w[i][W + k];
+    } else if constexpr (W == 1) {
+      x[0] = __funnelshift_l(w[i][0], w[i][1], 4 * o);
+    } else {
+      // (the shift counts modulo 32)
+      const uint32_t t = __funnelshift_l(w[i][1], w[i][2], 4 * o);
+      x[0] = o & 8 ? __funnelshift_l(w[i][0], w[i][1], 4 * o) : t;
+      x[1] = o & 8 ? t : __funnelshift_l(w[i][2], w[i][3], 4 * o);
+    }
+    if constexpr (sizeof(T) == 2) {
+      // a value times its scale is a bf16 (down to 2^-128), so the product is exact
+      const uint32_t fs = mx_scale_bf16x2(s[i]);
+      const uint32_t gs = SHIFT ? mx_scale_bf16x2(sp[i]) : 0u;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint2 p = e2m1x4_bf16(w[h][i] >> (16 * k));
-          u[2 * k] = mul_bf16x2(p.x, f);
-          u[2 * k + 1] = mul_bf16x2(p.y, f);
+      for (int k = 0; k < 4; ++k) {
+        const uint2 p = e2m1x4_bf16(x[k / 2] >> (16 * (k & 1)));
+        // columns 4 k to 4 k + 3 of the lane's: those below o take the first scale
+        const uint32_t m0 = (o > 4 * k ? 0xFFFFu : 0u) | (o > 4 * k + 1 ? 0xFFFF0000u : 0u);
+        const uint32_t m1 = (o > 4 * k + 2 ? 0xFFFFu : 0u) | (o > 4 * k + 3 ? 0xFFFF0000u : 0u);
+        v[2 * k] = mul_bf16x2(p.x, (fs & ~m0) | (gs & m0));
+        v[2 * k + 1] = mul_bf16x2(p.y, (fs & ~m1) | (gs & m1));
+      }
+    } else {
+      const float fs = mx_scale_value(s[i]), gs = SHIFT ? mx_scale_value(sp[i]) : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint2 p = e2m1x4_bf16(x[0] >> (16 * k));
+        const uint32_t u[4] = {p.x << 16, p.x & 0xFFFF0000u, p.y << 16, p.y & 0xFFFF0000u};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[4 * k + j] = __float_as_uint(__uint_as_float(u[j]) * (o > 4 * k + j ? gs : fs));
+      }
+    }
+    T* const row = out + (int64_t)(8 * i) * a.ld + c;
+    if (c >= 0 && c + V <= a.cols) {
+      store32(row, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (c + k >= 0 && c + k < a.cols) {
+          if constexpr (sizeof(T) == 2)
+            reinterpret_cast<uint16_t*>(row)[k] = (uint16_t)(v[k / 2] >> (16 * (k & 1)));
+          else
+            reinterpret_cast<uint32_t*>(row)[k] = v[k];
         }
-      } else {
-        const float f = mx_scale_value(s[h][i]);
-        const uint2 p = e2m1x4_bf16(w[h][i]);
-        v[0] = __uint_as_float(p.x << 16) * f;
-        v[1] = __uint_as_float(p.x & 0xFFFF0000u) * f;
-        v[2] = __uint_as_float(p.y << 16) * f;
-        v[3] = __uint_as_float(p.y & 0xFFFF0000u) * f;
-      }
-      if (a.vec && c + V <= a.cols) {
-        *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(v);
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (c + k < a.cols) o[k] = v[k];
-      }
     }
   }
 }
@@ -753,16 +827,19 @@ extern "C" int mmn_mxfp4_dequantize(const mmn_mxfp4* q, void* out, int64_t out_l
   a.rows = (int)q->rows;
   a.cols = (int)q->cols;
   a.ka = (int)scale_blocks(q->cols);
-  a.nct = (int)((q->cols + 255) / 256);
-  a.vec = vec_rows(out, a.ld, esize(dtype), 8);
+  // 32-byte stores; a row that starts between two has one vector more
+  const int64_t v = 32 / (int64_t)esize(dtype);
+  const bool vec = reinterpret_cast<uintptr_t>(out) % 32 == 0 && a.ld % v == 0;
+  a.nct = (int)((q->cols + (vec ? 0 : v - 1) + 32 * v - 1) / (32 * v));
   const int64_t blocks = (q->rows + 31) / 32 * a.nct;
   if (blocks > (int64_t(1) << 31) - 1) return fail(MMN_E_SHAPE, "matrix too large");
-  const unsigned grid = (unsigned)blocks;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == MMN_DTYPE_BF16)
-    MMN_CUDA_TRY(launch_dependent(mx_dequantize_kernel<__nv_bfloat16>, dim3(grid), 256, 0, s, a));
-  else
-    MMN_CUDA_TRY(launch_dependent(mx_dequantize_kernel<float>, dim3(grid), 256, 0, s, a));
+  const auto kernel = dtype == MMN_DTYPE_BF16
+                          ? (vec ? mx_dequantize_kernel<__nv_bfloat16, false>
+                                 : mx_dequantize_kernel<__nv_bfloat16, true>)
+                          : (vec ? mx_dequantize_kernel<float, false>
+                                 : mx_dequantize_kernel<float, true>);
+  MMN_CUDA_TRY(launch_dependent(kernel, dim3((unsigned)blocks), 256, 0,
+                                static_cast<cudaStream_t>(stream), a));
   return MMN_OK;
 }
 

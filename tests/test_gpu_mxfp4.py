@@ -280,6 +280,32 @@ def test_strided_and_unaligned_inputs(mmn):
         assert not out[:, :2].any() and not out[:, 2 + x.shape[1]:].any()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols,ld", [(1, 3), (33, 41), (130, 133), (300, 301), (520, 552), (1029, 1029)])
+def test_rows_that_start_anywhere(mmn, cols, ld, dtype):
+    """A slice at every offset from an aligned address gives what a copy of it gives, reads
+    nothing around it (NaN) and writes nothing around it."""
+    import torch
+
+    rows = 141
+    for off in range(17):
+        buf = torch.full((rows * ld + 32,), float("nan"), dtype=T(dtype), device="cuda")
+        x = buf[off:off + rows * ld].view(rows, ld)[:, :cols]
+        x.copy_(data(rows, cols, dtype, seed=cols + off))
+        want, want_t = mmn.mxfp4_quantize(x.clone(), "both")
+        q, qt = mmn.mxfp4_quantize(x, "both")
+        for got, ref in ((q, want), (qt, want_t), (mmn.mxfp4_quantize(x), want),
+                         (mmn.mxfp4_quantize(x, "cols"), want_t)):
+            assert torch.equal(got.codes, ref.codes) and torch.equal(got.scales, ref.scales), off
+        same(q.dequantize(), plain_values(x), off)
+        out = torch.full_like(buf, 7.0)
+        view = out[off:off + rows * ld].view(rows, ld)[:, :cols]
+        q.dequantize(out=view)
+        assert torch.equal(view, want.dequantize(T(dtype))), off
+        view.fill_(7.0)
+        assert (out == 7.0).all(), off
+
+
 @pytest.mark.parametrize("out", ["f32", "bf16"])
 @pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("m,n,k", [(700, 1112, 512), (2000, 1304, 300), (40, 264, 512)])
