@@ -16,17 +16,23 @@
 // Which kernel takes a call (measured on one B200, fractions of the 6.53 TB/s a
 // copy reaches):
 //   forward   ln_fwd_ring_kernel  bf16 rows, many and aligned: 16384 x 4096 in
-//                                 43.2 us (0.95), 70.6 us a row per block
+//                                 43.2 us (0.95), 70.6 us a row per block; rows that
+//                                 start anywhere, beyond 1024 columns: 16384 x 4057
+//                                 63.2 us (0.64), fp32 96.5 (0.84)
 //             ln_fwd_rows_kernel  the rest of the rows that can be read four at a
 //                                 time: 16384 x 2048 fp32 to bf16 in 31.6 us (0.97)
-//             ln_fwd_kernel       rows at any alignment, one element at a time:
-//                                 3001 x 1013 fp32 in 7.4 us (0.50)
+//             ln_fwd_kernel       an element at a time, where x and y start differently
+//                                 and for fewer columns: 3001 x 1013 fp32 in 6.7
+//                                 us (0.55), 16384 x 4057 bf16 132 (0.31)
 //             ln_fwd_wide_kernel  rows beyond 16384
 //   backward  ln_bwd_ring_kernel  aligned rows of 65 to 16384: 16384 x 4096 bf16 in
 //                                 72.9 us (0.85) with the closing sums, 113 us with
-//                                 the rows loaded into registers
-//             ln_bwd_kernel       narrow rows and rows at any alignment up to 8192:
-//                                 3001 x 1013 fp32 in 19.7 us (0.28)
+//                                 the rows loaded into registers; rows that start
+//                                 anywhere, beyond 512 columns: 16384 x 4057 106 us
+//                                 (0.57), fp32 141 (0.86)
+//             ln_bwd_kernel       narrow rows, and an element at a time up to 8192
+//                                 columns: 3001 x 1013 fp32 15.8 us (12.8 by vectors),
+//                                 16384 x 4057 bf16 158
 //             ln_bwd_wide_*       the rest
 #include <cuda_bf16.h>
 
@@ -35,6 +41,7 @@
 
 #include "capi_internal.cuh"
 #include "mmn_ptx.cuh"
+#include "unaligned.cuh"
 
 namespace mmn {
 namespace {
@@ -321,6 +328,88 @@ __device__ __forceinline__ float2 ring_sum2(float x, float y, float2* red) {
   }
 }
 
+// Rows that start anywhere (EDGE in the ring kernels). A row's columns are counted
+// from the vector that its first element lies in, o columns earlier, so every access
+// stays a whole vector and only a row's first and last one need care. That works
+// because o repeats every eight rows: a row group takes rows a multiple of eight
+// apart, has one o for all of them, and holds gamma and beta (and the sums of their
+// gradients) moved by it. All matrices of the call have to agree in o.
+//
+// The row comes into a 16-byte aligned slot of shared memory, at its offset from 16
+// bytes: `n` elements from `from` by bulk copy. Those are all whole vectors that the
+// row touches, as long as they lie in the matrix [begin, end); else those inside the
+// row, and the issuing thread copies its ends.
+struct Hull {
+  int from, n;
+};
+template <typename T>
+__device__ __forceinline__ Hull row_hull(uint8_t* slot, const T* row, int cols, const T* begin,
+                                         const T* end) {
+  constexpr int A = 16 / sizeof(T);
+  const int o = vec_offset<T, A>(row), n = (o + cols + A - 1) / A * A;
+  if (row - o >= begin && row - o + n <= end) return {-o, n};
+  const int lo = o ? A : 0, hi = (o + cols) / A * A;
+  T* s = reinterpret_cast<T*>(slot);
+  for (int j = o; j < lo; ++j) s[j] = row[j - o];
+  for (int j = hi; j < o + cols; ++j) s[j] = row[j - o];
+  return {lo - o, hi - lo};
+}
+template <typename T>
+__device__ __forceinline__ void load_hull(uint8_t* slot, const T* row, Hull h, uint64_t* bar) {
+  constexpr int A = 16 / sizeof(T);
+  bulk_load(slot + (vec_offset<T, A>(row) + h.from) * sizeof(T), row + h.from, h.n * sizeof(T), bar);
+}
+__host__ __device__ constexpr int hull_bytes(int64_t cols, int es) {
+  return (int)((cols * es + 15) / 16 * 16 + 16);
+}
+
+// Zeros in place of elements outside [lo, hi) of V.
+template <int V>
+__device__ __forceinline__ void keep_pairs(f2* v, int lo, int hi) {
+#pragma unroll
+  for (int j = 0; j < V / 2; ++j) {
+    const float2 f = unpack2(v[j]);
+    v[j] = pack2(2 * j >= lo && 2 * j < hi ? f.x : 0.0f,
+                 2 * j + 1 >= lo && 2 * j + 1 < hi ? f.y : 0.0f);
+  }
+}
+
+// gamma or beta from column c on; zeros outside [0, cols).
+template <int V>
+__device__ __forceinline__ void load_param_edge(const void* p, bool bf16, int c, int cols, f2* v) {
+  float u[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    u[j] = c + j < 0 || c + j >= cols ? 0.0f
+           : bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[c + j])
+                  : static_cast<const float*>(p)[c + j];
+#pragma unroll
+  for (int j = 0; j < V / 2; ++j) v[j] = pack2(u[2 * j], u[2 * j + 1]);
+}
+
+// Bit i: a thread's chunk i holds a row's first or last elements and others.
+template <int V, int TR, int NC>
+__device__ __forceinline__ uint32_t row_ends(int t, int o, int cols) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (i * TR + t) * V - o;
+    m |= (c < 0 || c + V > cols ? 1u : 0u) << i;
+  }
+  return m;
+}
+
+// Those of the V elements from column c on that lie in [0, cols).
+template <typename T, int V>
+__device__ __forceinline__ void store_edge(T* row, int c, int cols, const f2* v) {
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (c + j >= 0 && c + j < cols) {
+      const float2 f = unpack2(v[j / 2]);
+      from_f32(row[c + j], j & 1 ? f.y : f.x);
+    }
+}
+
 constexpr int kRingMax = 4;  // rows in flight per row group, at most (8 gained nothing)
 constexpr int kFwdRing = 2;  // ... in the forward kernel
 
@@ -397,13 +486,16 @@ __global__ void __launch_bounds__(ln_rows_block(TR), ln_rows_block(TR) > 512 ? 1
 // bf16 rows, many of them: blocks walk the rows. gamma and beta stay in registers,
 // each row group keeps a ring of rows in flight through bulk copies, and a
 // thread takes 32 columns, since the conversions and the two sums across the
-// threads cost more instructions than the arithmetic. Needs rows that start and
-// end on 16 bytes.
+// threads cost more instructions than the arithmetic. Rows that start and end on 16
+// bytes, or (EDGE) anywhere, then of both types, with 16 columns a thread up to 4096,
+// for the ends' sake: 20000 x 2037 bf16 44.7 us, 54.3 with 32.
 __host__ __device__ constexpr int ln_ring_block(int tr) { return tr <= 64 ? 128 : tr; }
-__host__ __device__ constexpr int ln_ring_blocks(int tr) { return 512 / ln_ring_block(tr); }
+__host__ __device__ constexpr int ln_ring_blocks(int tr, int ne) {
+  return (ne > 16 ? 512 : 768) / ln_ring_block(tr);
+}
 
-template <typename XT, typename YT, int TR, int NE>
-__global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR))
+template <typename XT, typename YT, int TR, int NE, bool EDGE>
+__global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR, NE))
     ln_fwd_ring_kernel(const LnFwd a, int depth, int* status) {
   constexpr int V = sizeof(XT) == 2 && sizeof(YT) == 2 ? 8 : 4;
   constexpr int kBlock = ln_ring_block(TR), RB = kBlock / TR, NC = NE / V, H = V / 2;
@@ -412,7 +504,8 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR))
   __shared__ __align__(8) uint64_t bars[RB][kRingMax];
   __shared__ volatile int abort_flag;
   const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
-  const int cols = (int)a.cols, rb = cols * (int)sizeof(XT);
+  const int cols = (int)a.cols;
+  const int rb = EDGE ? hull_bytes(cols, sizeof(XT)) : cols * (int)sizeof(XT);
   uint8_t* ring = dyn + sub * depth * rb;
   const int64_t first = (int64_t)blockIdx.x * RB + sub, step = (int64_t)gridDim.x * RB;
   if (threadIdx.x == 0) {
@@ -427,9 +520,19 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR))
   const int trips = (int)((a.rows - (int64_t)blockIdx.x * RB + step - 1) / step);
   const XT* x = static_cast<const XT*>(a.x) + first * a.x_ld;
   YT* y = static_cast<YT*>(a.y) + first * a.y_ld;
+  const int at = EDGE ? vec_offset<XT, 16 / sizeof(XT)>(x) : 0, o = at & (V - 1);
   auto issue = [&](int k, int slot) {  // row k of this group into a slot
-    mbar_arrive_expect_tx(&bars[sub][slot], rb);
-    bulk_load(ring + slot * rb, x + k * step * a.x_ld, rb, &bars[sub][slot]);
+    const XT* row = x + k * step * a.x_ld;
+    if constexpr (EDGE) {
+      const XT* const begin = static_cast<const XT*>(a.x);
+      const Hull h = row_hull(ring + slot * rb, row, cols, begin,
+                              begin + (a.rows - 1) * a.x_ld + a.cols);
+      mbar_arrive_expect_tx(&bars[sub][slot], h.n * (int)sizeof(XT));
+      load_hull(ring + slot * rb, row, h, &bars[sub][slot]);
+    } else {
+      mbar_arrive_expect_tx(&bars[sub][slot], rb);
+      bulk_load(ring + slot * rb, row, rb, &bars[sub][slot]);
+    }
   };
   griddep_wait();
   griddep_launch_dependents();
@@ -438,27 +541,33 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR))
   f2 ga[NE / 2], be[NE / 2];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int c = (i * TR + t) * V;
-    if (c < cols) {
+    const int c = (i * TR + t) * V - o;
+    if constexpr (EDGE) {
+      load_param_edge<V>(a.gamma, a.param_bf16, c, cols, ga + i * H);
+      load_param_edge<V>(a.beta, a.param_bf16, c, cols, be + i * H);
+    } else if (c < cols) {
       load_param_pairs<V>(a.gamma, a.param_bf16, c, ga + i * H);
       load_param_pairs<V>(a.beta, a.param_bf16, c, be + i * H);
     }
   }
+  const uint32_t ends = EDGE ? row_ends<V, TR, NC>(t, o, cols) : 0u;
   const float inv_n = 1.0f / (float)cols;
   int slot = 0;
   uint32_t phase = 0;
   for (int k = 0; k < trips; ++k) {
-    const int lim = k < mine ? cols : 0;
-    const XT* sx = reinterpret_cast<const XT*>(ring + slot * rb);
+    const bool ok = k < mine;
+    const int lim = ok ? cols : -V;  // (below a row's first vector: no row, no columns)
+    const XT* sx = reinterpret_cast<const XT*>(ring + slot * rb) + at;
     // (a wait that gives up marks the status; the loop runs on so that every
     // barrier is met)
-    if (lim) mbar_wait(&bars[sub][slot], phase, &abort_flag);
+    if (ok) mbar_wait(&bars[sub][slot], phase, &abort_flag);
     f2 v[NE / 2], s = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (i * TR + t) * V;
+      const int c = (i * TR + t) * V - o;
       if (c < lim) {
         load_pairs<XT, V>(sx + c, v + i * H);
+        if (EDGE && (ends >> i & 1)) keep_pairs<V>(v + i * H, -c, cols - c);
 #pragma unroll
         for (int j = 0; j < H; ++j) s = add2(s, v[i * H + j]);
       }
@@ -471,28 +580,31 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR))
     f2 q = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
-      if ((i * TR + t) * V < lim) {
+      if (const int c = (i * TR + t) * V - o; c < lim) {
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-          v[i * H + j] = add2(v[i * H + j], nm);
-          q = fma2(v[i * H + j], v[i * H + j], q);
-        }
+        for (int j = 0; j < H; ++j) v[i * H + j] = add2(v[i * H + j], nm);
+        if (EDGE && (ends >> i & 1)) keep_pairs<V>(v + i * H, -c, cols - c);
+#pragma unroll
+        for (int j = 0; j < H; ++j) q = fma2(v[i * H + j], v[i * H + j], q);
       }
     const float var = row_sum1<TR>(sum2(q), red[1][sub]) * inv_n;
     const float rstd = 1.0f / sqrtf(var + a.eps);
-    if (t == 0 && lim) {
+    if (t == 0 && ok) {
       if (a.mean) a.mean[first + k * step] = mean;
       if (a.rstd) a.rstd[first + k * step] = rstd;
     }
     const f2 r2 = dup2(rstd);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (i * TR + t) * V;
+      const int c = (i * TR + t) * V - o;
       if (c < lim) {
 #pragma unroll
         for (int j = 0; j < H; ++j)
           v[i * H + j] = fma2(mul2(v[i * H + j], r2), ga[i * H + j], be[i * H + j]);
-        store_pairs<YT, V>(y + c, v + i * H);
+        if (EDGE && (ends >> i & 1))
+          store_edge<YT, V>(y, c, cols, v + i * H);
+        else
+          store_pairs<YT, V>(y + c, v + i * H);
       }
     }
     y += step * a.y_ld;
@@ -627,10 +739,10 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
 // ring of `depth` rows of x and dy in flight in shared memory, so the loads of
 // the next rows run under the sums, the barrier and the stores of this one
 // (16384 x 4096 bf16: 113 us with the rows loaded into registers).
-// Needs rows that start and end on 16 bytes. NE <= 16: gamma, h and g live in
-// registers. NE = 32 (rows of 8192 to 16384): gamma is kept in shared memory, and
+// Rows that start and end on 16 bytes, or (EDGE) anywhere. NE <= 16: gamma, h and g
+// live in registers. NE = 32 (rows of 8192 to 16384): gamma is kept in shared memory, and
 // the second pass reads the row again.
-template <typename XT, typename DT, int V, int TR, int NE>
+template <typename XT, typename DT, int V, int TR, int NE, bool EDGE>
 __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
     ln_bwd_ring_kernel(const LnBwd a, int depth, int* status) {
   constexpr int kBlock = ln_bwd_block(TR), RB = kBlock / TR, NC = NE / V, H = V / 2;
@@ -640,17 +752,33 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
   __shared__ __align__(8) uint64_t bars[RB][kRingMax];
   __shared__ volatile int abort_flag;
   const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
-  const int xb = (int)(a.cols * sizeof(XT)), db = (int)(a.cols * sizeof(DT)), rb = xb + db;
-  const int gb = kReread ? (int)a.cols * 4 : 0;
+  const int cols = (int)a.cols;
+  const int xb = EDGE ? hull_bytes(cols, sizeof(XT)) : cols * (int)sizeof(XT);
+  const int db = EDGE ? hull_bytes(cols, sizeof(DT)) : cols * (int)sizeof(DT), rb = xb + db;
+  const int gb = kReread ? (EDGE ? (cols + 2 * V) / 4 * 16 : cols * 4) : 0;
   float* gs = reinterpret_cast<float*>(dyn);  // gamma (kReread)
   uint8_t* ring = dyn + gb + sub * depth * rb;
   const int64_t first = (int64_t)blockIdx.x * RB + sub, step = (int64_t)gridDim.x * RB;
+  const XT* const x0 = static_cast<const XT*>(a.x);
+  const DT* const d0 = static_cast<const DT*>(a.dy);
+  const int ax = EDGE ? vec_offset<XT, 16 / sizeof(XT)>(x0 + first * a.x_ld) : 0;
+  const int ad = EDGE ? vec_offset<DT, 16 / sizeof(DT)>(d0 + first * a.dy_ld) : 0;
+  const int o = ax & (V - 1);
   auto issue = [&](int64_t k, int slot) {  // row k of this group into a slot
-    const int64_t row = first + k * step;
-    mbar_arrive_expect_tx(&bars[sub][slot], rb);
-    bulk_load(ring + slot * rb, static_cast<const XT*>(a.x) + row * a.x_ld, xb, &bars[sub][slot]);
-    bulk_load(ring + slot * rb + xb, static_cast<const DT*>(a.dy) + row * a.dy_ld, db,
-              &bars[sub][slot]);
+    const XT* x = x0 + (first + k * step) * a.x_ld;
+    const DT* d = d0 + (first + k * step) * a.dy_ld;
+    uint8_t* to = ring + slot * rb;
+    if constexpr (EDGE) {
+      const Hull hx = row_hull(to, x, cols, x0, x0 + (a.rows - 1) * a.x_ld + a.cols);
+      const Hull hd = row_hull(to + xb, d, cols, d0, d0 + (a.rows - 1) * a.dy_ld + a.cols);
+      mbar_arrive_expect_tx(&bars[sub][slot], hx.n * (int)sizeof(XT) + hd.n * (int)sizeof(DT));
+      load_hull(to, x, hx, &bars[sub][slot]);
+      load_hull(to + xb, d, hd, &bars[sub][slot]);
+    } else {
+      mbar_arrive_expect_tx(&bars[sub][slot], rb);
+      bulk_load(to, x, xb, &bars[sub][slot]);
+      bulk_load(to + xb, d, db, &bars[sub][slot]);
+    }
   };
   if (threadIdx.x == 0) {
     for (int g = 0; g < RB; ++g)
@@ -668,18 +796,25 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
     for (int k = 0; k < depth && k < mine; ++k) issue(k, k);
   f2 ga[kReread ? 1 : NE / 2];
   if constexpr (kReread) {
-    for (int c = threadIdx.x; c < a.cols; c += kBlock)
-      gs[c] = a.param_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.gamma)[c])
-                           : static_cast<const float*>(a.gamma)[c];
+    for (int k = threadIdx.x; k < gb / 4; k += kBlock) {
+      const int c = k - o;
+      gs[k] = EDGE && (c < 0 || c >= cols) ? 0.0f
+              : a.param_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.gamma)[c])
+                             : static_cast<const float*>(a.gamma)[c];
+    }
     __syncthreads();
   } else {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (i * TR + t) * V;
-      if (c < a.cols) load_param_pairs<V>(a.gamma, a.param_bf16, c, ga + i * H);
+      const int c = (i * TR + t) * V - o;
+      if constexpr (EDGE)
+        load_param_edge<V>(a.gamma, a.param_bf16, c, cols, ga + i * H);
+      else if (c < cols)
+        load_param_pairs<V>(a.gamma, a.param_bf16, c, ga + i * H);
     }
   }
-  const float inv_n = 1.0f / (float)a.cols;
+  const uint32_t ends = EDGE ? row_ends<V, TR, NC>(t, o, cols) : 0u;
+  const float inv_n = 1.0f / (float)cols;
   f2 sg[NE / 2], sb[NE / 2];
 #pragma unroll
   for (int k = 0; k < NE / 2; ++k) sg[k] = sb[k] = 0;
@@ -693,7 +828,16 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
   for (int64_t k = 0; k < trips; ++k) {
     const bool ok = k < mine;
     const int64_t row = first + k * step;
-    const uint8_t* sx = ring + slot * rb;
+    const XT* const sx = reinterpret_cast<const XT*>(ring + slot * rb) + ax;
+    const DT* const sd = reinterpret_cast<const DT*>(ring + slot * rb + xb) + ad;
+    auto get = [&](int i, int c, f2* x, f2* d) {
+      load_pairs<XT, V>(sx + c, x);
+      load_pairs<DT, V>(sd + c, d);
+      if (EDGE && (ends >> i & 1)) {
+        keep_pairs<V>(x, -c, cols - c);
+        keep_pairs<V>(d, -c, cols - c);
+      }
+    };
     float mean2 = 0.0f, rstd2 = 0.0f;  // of the group's next row
     if (k + 1 < mine) {
       mean2 = a.mean[row + step];
@@ -707,12 +851,11 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
     f2 s1 = 0, s2 = 0;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (i * TR + t) * V;
-      if (ok && c < a.cols) {
+      const int c = (i * TR + t) * V - o;
+      if (ok && c < cols) {
         f2 x[H], d[H], gm[H];
-        load_pairs<XT, V>(reinterpret_cast<const XT*>(sx) + c, x);
-        load_pairs<DT, V>(reinterpret_cast<const DT*>(sx + xb) + c, d);
-        if constexpr (kReread) load_pairs<float, V>(gs + c, gm);
+        get(i, c, x, d);
+        if constexpr (kReread) load_pairs<float, V>(gs + o + c, gm);
 #pragma unroll
         for (int j = 0; j < H; ++j) {
           const int e = i * H + j;
@@ -737,23 +880,25 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
       XT* dx = static_cast<XT*>(a.dx) + row * a.dx_ld;
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        const int c = (i * TR + t) * V;
-        if (c < a.cols) {
-          f2 o[H];
+        const int c = (i * TR + t) * V - o;
+        if (c < cols) {
+          f2 u[H];
           if constexpr (kReread) {
             f2 x[H], d[H], gm[H];
-            load_pairs<XT, V>(reinterpret_cast<const XT*>(sx) + c, x);
-            load_pairs<DT, V>(reinterpret_cast<const DT*>(sx + xb) + c, d);
-            load_pairs<float, V>(gs + c, gm);
+            get(i, c, x, d);
+            load_pairs<float, V>(gs + o + c, gm);
 #pragma unroll
             for (int j = 0; j < H; ++j)
-              o[j] = mul2(fma2(mul2(add2(x[j], nm), r2), c2, add2(mul2(d[j], gm[j]), c1)), r2);
+              u[j] = mul2(fma2(mul2(add2(x[j], nm), r2), c2, add2(mul2(d[j], gm[j]), c1)), r2);
           } else {
 #pragma unroll
             for (int j = 0; j < H; ++j)
-              o[j] = mul2(fma2(h[i * H + j], c2, add2(g[i * H + j], c1)), r2);
+              u[j] = mul2(fma2(h[i * H + j], c2, add2(g[i * H + j], c1)), r2);
           }
-          store_pairs<XT, V>(dx + c, o);
+          if (EDGE && (ends >> i & 1))
+            store_edge<XT, V>(dx, c, cols, u);
+          else
+            store_pairs<XT, V>(dx + c, u);
         }
       }
     }
@@ -771,13 +916,16 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
   if constexpr (RB == 1) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (i * TR + t) * V;
-      if (c < a.cols) {
+      const int c = (i * TR + t) * V - o;
+      if constexpr (EDGE) {
+        store_edge<float, V>(out, c, cols, sg + i * H);
+        store_edge<float, V>(out + cols, c, cols, sb + i * H);
+      } else if (c < cols) {
 #pragma unroll
         for (int j = 0; j < H; ++j) {
           const float2 u = unpack2(sg[i * H + j]), w = unpack2(sb[i * H + j]);
           *reinterpret_cast<float2*>(out + c + 2 * j) = u;
-          *reinterpret_cast<float2*>(out + a.cols + c + 2 * j) = w;
+          *reinterpret_cast<float2*>(out + cols + c + 2 * j) = w;
         }
       }
     }
@@ -788,17 +936,22 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
     for (int pass = 0; pass < 2; ++pass) {
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
+      for (int i = 0; i < NC; ++i) {
+        const int c = (i * TR + t) * V - o;
+        float* to = acc + sub * TR * NE;
+        if constexpr (EDGE)
+          store_edge<float, V>(to, c, cols, (pass ? sb : sg) + i * H);
+        else
 #pragma unroll
-        for (int j = 0; j < H; ++j)
-          *reinterpret_cast<float2*>(acc + sub * TR * NE + (i * TR + t) * V + 2 * j) =
-              unpack2(pass ? sb[i * H + j] : sg[i * H + j]);
+          for (int j = 0; j < H; ++j)
+            *reinterpret_cast<float2*>(to + c + 2 * j) = unpack2(pass ? sb[i * H + j] : sg[i * H + j]);
+      }
       __syncthreads();
-      for (int c = threadIdx.x; c < a.cols; c += kBlock) {
+      for (int c = threadIdx.x; c < cols; c += kBlock) {
         float v = 0.0f;
 #pragma unroll
         for (int r = 0; r < RB; ++r) v += acc[r * TR * NE + c];
-        out[pass * a.cols + c] = v;
+        out[pass * cols + c] = v;
       }
     }
   }
@@ -952,37 +1105,78 @@ void fwd_width(const LnFwd& a, cudaStream_t s) {
     fwd_rows<XT, YT, 1024, 16>(a, s);
 }
 
-template <typename XT, typename YT, int TR, int NE>
+// Blocks of a ring kernel, RB rows at a time. For rows that start anywhere the rows of
+// a group lie a multiple of eight apart.
+int ring_grid(int64_t rows, int rb, int64_t most, bool edge) {
+  int64_t grid = std::min((rows + rb - 1) / rb, most);
+  if (edge && grid * rb < rows) grid -= grid % (8 / std::min(rb, 8));
+  return (int)grid;
+}
+
+// Whether the rows of two matrices start alike, counted modulo v elements.
+bool rows_agree(const void* p, int64_t p_ld, size_t p_es, const void* q, int64_t q_ld, size_t q_es,
+                int v) {
+  const uintptr_t d = reinterpret_cast<uintptr_t>(p) / p_es - reinterpret_cast<uintptr_t>(q) / q_es;
+  return d % v == 0 && (p_ld - q_ld) % v == 0;
+}
+
+template <typename XT, typename YT, int TR, int NE, bool EDGE>
 int ring_fwd_launch(const LnFwd& a, int sms, int device, cudaStream_t s) {
-  constexpr int RB = ln_ring_block(TR) / TR, kBlocks = ln_ring_blocks(TR);
+  constexpr int RB = ln_ring_block(TR) / TR, kBlocks = ln_ring_blocks(TR, NE);
   static std::mutex mu;
   static uint64_t done = 0;
-  auto* kernel = ln_fwd_ring_kernel<XT, YT, TR, NE>;
+  auto* kernel = ln_fwd_ring_kernel<XT, YT, TR, NE, EDGE>;
   int* status = nullptr;
   int rc;
   if ((rc = raise_smem(kernel, device, mu, done)) != MMN_OK) return rc;
   if ((rc = kernel_status_word(device, &status)) != MMN_OK) return rc;
-  const int64_t row = a.cols * (int64_t)sizeof(XT);
+  const int64_t row = EDGE ? hull_bytes(a.cols, sizeof(XT)) : a.cols * (int64_t)sizeof(XT);
   // more rows in flight cost bandwidth (16384 x 4096: 43.6 us with 2, 45.6 with 3,
   // 47.2 with 4)
   const int depth = (int)std::min<int64_t>(kFwdRing, (224 * 1024 / kBlocks - 4096) / (row * RB));
-  const int64_t grid = std::min<int64_t>((a.rows + RB - 1) / RB, (int64_t)sms * kBlocks);
+  const int64_t grid = ring_grid(a.rows, RB, (int64_t)sms * kBlocks, EDGE);
   launch_dependent(kernel, dim3((unsigned)grid), ln_ring_block(TR), depth * row * RB, s, a, depth,
                    status);
   return MMN_OK;
 }
 
+// bf16 rows in whole vectors, many of them.
 template <typename XT, typename YT>
-int fwd_types(const LnFwd& a, bool vec, bool ring, int sms, int device, cudaStream_t s) {
-  if constexpr (sizeof(XT) == 2) {
-    if (ring) {
-      if (a.cols <= 512) return ring_fwd_launch<XT, YT, 32, 16>(a, sms, device, s);
-      if (a.cols <= 1024) return ring_fwd_launch<XT, YT, 32, 32>(a, sms, device, s);
-      if (a.cols <= 2048) return ring_fwd_launch<XT, YT, 64, 32>(a, sms, device, s);
-      if (a.cols <= 4096) return ring_fwd_launch<XT, YT, 128, 32>(a, sms, device, s);
-      if (a.cols <= 8192) return ring_fwd_launch<XT, YT, 256, 32>(a, sms, device, s);
-      return ring_fwd_launch<XT, YT, 512, 32>(a, sms, device, s);
-    }
+int ring_whole(const LnFwd& a, int sms, int device, cudaStream_t s) {
+  if (a.cols <= 512) return ring_fwd_launch<XT, YT, 32, 16, false>(a, sms, device, s);
+  if (a.cols <= 1024) return ring_fwd_launch<XT, YT, 32, 32, false>(a, sms, device, s);
+  if (a.cols <= 2048) return ring_fwd_launch<XT, YT, 64, 32, false>(a, sms, device, s);
+  if (a.cols <= 4096) return ring_fwd_launch<XT, YT, 128, 32, false>(a, sms, device, s);
+  if (a.cols <= 8192) return ring_fwd_launch<XT, YT, 256, 32, false>(a, sms, device, s);
+  return ring_fwd_launch<XT, YT, 512, 32, false>(a, sms, device, s);
+}
+
+// Rows that start anywhere; w: the columns and what the start may add.
+template <typename XT, typename YT>
+int ring_edge(const LnFwd& a, int64_t w, int sms, int device, cudaStream_t s) {
+  if (w <= 2048) return ring_fwd_launch<XT, YT, 128, 16, true>(a, sms, device, s);
+  if (w <= 4096) return ring_fwd_launch<XT, YT, 256, 16, true>(a, sms, device, s);
+  if (w <= 8192) return ring_fwd_launch<XT, YT, 256, 32, true>(a, sms, device, s);
+  return ring_fwd_launch<XT, YT, 512, 32, true>(a, sms, device, s);
+}
+
+// vec, vec8: rows in whole vectors of four or eight elements; alike: x and y start alike.
+template <typename XT, typename YT>
+int fwd_types(const LnFwd& a, bool vec, bool vec8, bool alike, int sms, int device, cudaStream_t s) {
+  // bf16 rows: with fewer a block of its own per row is quicker
+  if constexpr (sizeof(XT) == 2)
+    if (vec8 && a.cols > 64 && a.cols <= kFwdMaxCols && a.rows >= 8 * (int64_t)sms)
+      return ring_whole<XT, YT>(a, sms, device, s);
+  // Rows that start anywhere: vectors with care at the ends, or an element at a time.
+  // 16384 x 4057 63.2 us and 132, fp32 96.9 and 115; 20000 x 2037 44.7 and 79.0, fp32 61.8
+  // and 68.0; 8 x 4001 2.9 and 5.4. Up to 1024 columns the ends outweigh the rest
+  // (3001 x 1013 fp32 8.1 and 6.7 us), and so they do for fp32 rows that the start pushes
+  // into the next class (16384 x 4095 124 and 116; bf16 100 and 132).
+  if (const int64_t w = a.cols + (sizeof(XT) == 2 && sizeof(YT) == 2 ? 7 : 3);
+      alike && !vec && a.cols > 1024 && w <= kFwdMaxCols) {
+    int64_t cls = 2048;
+    while (cls < a.cols) cls *= 2;
+    if (sizeof(XT) == 2 || w <= cls) return ring_edge<XT, YT>(a, w, sms, device, s);
   }
   if (a.cols > kFwdMaxCols)
     launch_dependent(ln_fwd_wide_kernel<XT, YT>, dim3((unsigned)a.rows), 512, 0, s, a);
@@ -992,6 +1186,8 @@ int fwd_types(const LnFwd& a, bool vec, bool ring, int sms, int device, cudaStre
     fwd_scalar<XT, YT, 8, 8>(a, s);
   else if (a.cols <= 256)
     fwd_scalar<XT, YT, 32, 8>(a, s);
+  else if (a.cols <= 512)
+    fwd_scalar<XT, YT, 32, 16>(a, s);
   else if (a.cols <= 1024)
     fwd_scalar<XT, YT, 128, 8>(a, s);
   else if (a.cols <= 2048)
@@ -1011,12 +1207,15 @@ int bwd_tr(int64_t cols) {
          : cols <= 4096 ? 256 : 512;
 }
 
-// Blocks of the backward kernel (partial sums to add): one per row group, at
-// most what the GPU holds at once.
-int bwd_parts(int64_t rows, int64_t cols, int sms) {
-  if (rows <= 0 || cols <= 0) return 0;
-  const int tr = bwd_tr(cols), rb = ln_bwd_block(tr) / tr;
-  return (int)std::min<int64_t>((rows + rb - 1) / rb, (int64_t)sms * ln_bwd_min_blocks(tr));
+// Blocks of the backward kernel (partial sums to add) for tr threads a row: one per
+// row group, at most what the GPU holds at once.
+int bwd_parts(int64_t rows, int tr, int sms, bool edge) {
+  return ring_grid(rows, ln_bwd_block(tr) / tr, (int64_t)sms * ln_bwd_min_blocks(tr), edge);
+}
+
+// ... at most, however the rows start.
+int bwd_max_parts(int64_t rows, int64_t cols, int sms) {
+  return rows <= 0 || cols <= 0 ? 0 : bwd_parts(rows, bwd_tr(cols), sms, false);
 }
 
 template <typename XT, typename DT, int V, int TR, int NE>
@@ -1024,31 +1223,33 @@ void bwd_launch(const LnBwd& a, int parts, cudaStream_t s) {
   launch_dependent(ln_bwd_kernel<XT, DT, V, TR, NE>, dim3(parts), ln_bwd_block(TR), 0, s, a);
 }
 
-template <typename XT, typename DT, int V>
-void bwd_width(const LnBwd& a, int parts, cudaStream_t s) {
+// Rows of any width up to 8192, one element at a time.
+template <typename XT, typename DT>
+void bwd_scalar(const LnBwd& a, int parts, cudaStream_t s) {
   switch (bwd_tr(a.cols)) {
     case 8:
-      return bwd_launch<XT, DT, V, 8, 8>(a, parts, s);
+      return bwd_launch<XT, DT, 1, 8, 8>(a, parts, s);
     case 32:
-      return bwd_launch<XT, DT, V, 32, 8>(a, parts, s);
+      return bwd_launch<XT, DT, 1, 32, 8>(a, parts, s);
     case 64:
-      return bwd_launch<XT, DT, V, 64, 8>(a, parts, s);
+      return bwd_launch<XT, DT, 1, 64, 8>(a, parts, s);
     case 128:
-      return bwd_launch<XT, DT, V, 128, 16>(a, parts, s);
+      return bwd_launch<XT, DT, 1, 128, 16>(a, parts, s);
     case 256:
-      return bwd_launch<XT, DT, V, 256, 16>(a, parts, s);
+      return bwd_launch<XT, DT, 1, 256, 16>(a, parts, s);
     default:
-      return bwd_launch<XT, DT, V, 512, 16>(a, parts, s);
+      return bwd_launch<XT, DT, 1, 512, 16>(a, parts, s);
   }
 }
 
 // Rows in flight per group with bulk copies: what an SM's 224 KB hold, shared by
-// the blocks on it.
+// the blocks on it. w: the columns and what an uneven start adds.
 template <typename XT, typename DT>
-int ring_depth(int64_t cols, int* smem) {
-  const int tr = bwd_tr(cols), rb = ln_bwd_block(tr) / tr;
-  const int64_t row = cols * (int64_t)(sizeof(XT) + sizeof(DT));
-  const int64_t gamma = cols > kBwdMaxCols ? cols * 4 : 0;
+int ring_depth(int64_t cols, int64_t w, bool edge, int* smem) {
+  const int tr = bwd_tr(w), rb = ln_bwd_block(tr) / tr;
+  const int64_t row = edge ? hull_bytes(cols, sizeof(XT)) + hull_bytes(cols, sizeof(DT))
+                           : cols * (int64_t)(sizeof(XT) + sizeof(DT));
+  const int64_t gamma = w > kBwdMaxCols ? (edge ? (w + 9) / 4 * 16 : cols * 4) : 0;
   const int64_t budget = 224 * 1024 / ln_bwd_min_blocks(tr) - 4096 - gamma;
   const int depth = (int)std::min<int64_t>(kRingMax, budget / (row * rb));
   // (the closing sums of several groups use the same memory)
@@ -1057,44 +1258,68 @@ int ring_depth(int64_t cols, int* smem) {
   return depth;
 }
 
-template <typename XT, typename DT, int V, int TR, int NE>
+template <typename XT, typename DT, int TR, int NE, bool EDGE>
 int ring_launch(const LnBwd& a, int parts, int depth, int smem, int* status, int device,
                 cudaStream_t s) {
+  constexpr int V = sizeof(XT) == 2 && sizeof(DT) == 2 ? 8 : 4;
   static std::mutex mu;
   static uint64_t done = 0;
-  auto* kernel = ln_bwd_ring_kernel<XT, DT, V, TR, NE>;
+  auto* kernel = ln_bwd_ring_kernel<XT, DT, V, TR, NE, EDGE>;
   const int rc = raise_smem(kernel, device, mu, done);
   if (rc != MMN_OK) return rc;
   launch_dependent(kernel, dim3(parts), ln_bwd_block(TR), smem, s, a, depth, status);
   return MMN_OK;
 }
 
-template <typename XT, typename DT>
-int bwd_types(const LnBwd& a, int parts, bool vec, bool ring, int device, cudaStream_t s) {
-  constexpr int V = sizeof(XT) == 2 && sizeof(DT) == 2 ? 8 : 4;
-  int smem = 0;
-  const int depth = ring && a.cols > 64 && a.cols <= kRingMaxCols ? ring_depth<XT, DT>(a.cols, &smem) : 0;
-  if (depth >= 2) {
-    int* status = nullptr;
-    const int rc = kernel_status_word(device, &status);
-    if (rc != MMN_OK) return rc;
-    if (a.cols <= 256) return ring_launch<XT, DT, V, 32, 8>(a, parts, depth, smem, status, device, s);
-    if (a.cols <= 512) return ring_launch<XT, DT, V, 64, 8>(a, parts, depth, smem, status, device, s);
-    if (a.cols <= 1024) return ring_launch<XT, DT, V, 128, 8>(a, parts, depth, smem, status, device, s);
-    if (a.cols <= 2048) return ring_launch<XT, DT, V, 128, 16>(a, parts, depth, smem, status, device, s);
-    if (a.cols <= 4096) return ring_launch<XT, DT, V, 256, 16>(a, parts, depth, smem, status, device, s);
-    if (a.cols <= 8192) return ring_launch<XT, DT, V, 512, 16>(a, parts, depth, smem, status, device, s);
-    return ring_launch<XT, DT, V, 512, 32>(a, parts, depth, smem, status, device, s);
+template <typename XT, typename DT, bool EDGE>
+int ring_bwd(const LnBwd& a, int64_t w, int parts, int depth, int smem, int device, cudaStream_t s) {
+  int* st = nullptr;
+  const int rc = kernel_status_word(device, &st);
+  if (rc != MMN_OK) return rc;
+  if constexpr (!EDGE) {
+    if (w <= 256) return ring_launch<XT, DT, 32, 8, false>(a, parts, depth, smem, st, device, s);
+    if (w <= 512) return ring_launch<XT, DT, 64, 8, false>(a, parts, depth, smem, st, device, s);
   }
+  if (w <= 1024) return ring_launch<XT, DT, 128, 8, EDGE>(a, parts, depth, smem, st, device, s);
+  if (w <= 2048) return ring_launch<XT, DT, 128, 16, EDGE>(a, parts, depth, smem, st, device, s);
+  if (w <= 4096) return ring_launch<XT, DT, 256, 16, EDGE>(a, parts, depth, smem, st, device, s);
+  if (w <= 8192) return ring_launch<XT, DT, 512, 16, EDGE>(a, parts, depth, smem, st, device, s);
+  return ring_launch<XT, DT, 512, 32, EDGE>(a, parts, depth, smem, st, device, s);
+}
+
+// vec: rows in whole vectors; ring: ... of 16 bytes; alike: the rows of all three
+// matrices start alike. parts: the blocks launched.
+template <typename XT, typename DT>
+int bwd_types(const LnBwd& a, int* parts, bool vec, bool ring, bool alike, int sms, int device,
+              cudaStream_t s) {
+  constexpr int V = sizeof(XT) == 2 && sizeof(DT) == 2 ? 8 : 4;
+  const int64_t w = a.cols + (ring ? 0 : V - 1);  // ... and what an uneven start may add
+  // Rows that start anywhere: vectors with care at the ends, or an element at a time.
+  // 16384 x 4057 106 us and 158, fp32 141 and 184; 32768 x 1013 74.6 and 109, fp32 67.4 and
+  // 118. Element-wise where the start pushes the row into the next class (16384 x 4095
+  // 205 and 158), for few columns (32768 x 501 47.9 and 36.9) and few bf16 rows (600 x
+  // 1013 13.8 and 9.6; fp32 8.7 and 10.1).
+  const bool edge = alike && a.cols > 512 && bwd_tr(w) == bwd_tr(a.cols) &&
+                    (V == 4 || a.rows >= 8 * (int64_t)sms);
+  if (a.cols > 64 && (ring || edge) && w <= kRingMaxCols) {
+    int smem = 0;
+    const int depth = ring_depth<XT, DT>(a.cols, w, !ring, &smem);
+    if (depth >= 2) {
+      *parts = bwd_parts(a.rows, bwd_tr(w), sms, !ring);
+      return ring ? ring_bwd<XT, DT, false>(a, w, *parts, depth, smem, device, s)
+                  : ring_bwd<XT, DT, true>(a, w, *parts, depth, smem, device, s);
+    }
+  }
+  *parts = bwd_parts(a.rows, bwd_tr(a.cols), sms, false);
   if (a.cols > kBwdMaxCols) {
-    const int64_t chunk = (a.rows + parts - 1) / parts;
+    const int64_t chunk = (a.rows + *parts - 1) / *parts;
     launch_dependent(ln_bwd_wide_cols_kernel<XT, DT>,
-                     dim3((unsigned)((a.cols + 127) / 128), (unsigned)parts), 128, 0, s, a, chunk);
+                     dim3((unsigned)((a.cols + 127) / 128), (unsigned)*parts), 128, 0, s, a, chunk);
     launch_dependent(ln_bwd_wide_rows_kernel<XT, DT>, dim3((unsigned)a.rows), 512, 0, s, a);
-  } else if (vec) {
-    bwd_width<XT, DT, V>(a, parts, s);
+  } else if (vec && a.cols <= 64) {
+    bwd_launch<XT, DT, V, 8, 8>(a, *parts, s);
   } else {
-    bwd_width<XT, DT, 1>(a, parts, s);
+    bwd_scalar<XT, DT>(a, *parts, s);
   }
   return MMN_OK;
 }
@@ -1150,24 +1375,24 @@ extern "C" int mmn_layer_norm(const void* x, int64_t x_ld, int x_dtype, const vo
   const int v = 4;
   const bool vec = cols % v == 0 && vec_rows(x, a.x_ld, esize(x_dtype), v) &&
                    vec_rows(y, a.y_ld, esize(y_dtype), v) &&
-                   vec_rows(gamma, cols, esize(param_dtype), v) &&
-                   vec_rows(beta, cols, esize(param_dtype), v);
+                   vec_rows(gamma, 0, esize(param_dtype), v) &&
+                   vec_rows(beta, 0, esize(param_dtype), v);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool xb = x_dtype == MMN_DTYPE_BF16, yb = y_dtype == MMN_DTYPE_BF16;
-  // (with fewer rows a block of its own per row is quicker)
-  const bool ring = xb && vec && cols > 64 && cols <= kFwdMaxCols && rows >= 8 * (int64_t)sms &&
-                    cols % 8 == 0 && vec_rows(x, a.x_ld, 2, 8) &&
+  const bool vec8 = vec && cols % 8 == 0 && vec_rows(x, a.x_ld, esize(x_dtype), 8) &&
                     vec_rows(y, a.y_ld, esize(y_dtype), 8) &&
-                    vec_rows(gamma, cols, esize(param_dtype), 8) &&
-                    vec_rows(beta, cols, esize(param_dtype), 8);
+                    vec_rows(gamma, 0, esize(param_dtype), 8) &&
+                    vec_rows(beta, 0, esize(param_dtype), 8);
+  const bool alike = rows_agree(x, a.x_ld, esize(x_dtype), y, a.y_ld, esize(y_dtype),
+                                xb && yb ? 8 : 4);
   if (xb && yb)
-    rc = fwd_types<__nv_bfloat16, __nv_bfloat16>(a, vec, ring, sms, device, s);
+    rc = fwd_types<__nv_bfloat16, __nv_bfloat16>(a, vec, vec8, alike, sms, device, s);
   else if (xb)
-    rc = fwd_types<__nv_bfloat16, float>(a, vec, ring, sms, device, s);
+    rc = fwd_types<__nv_bfloat16, float>(a, vec, vec8, alike, sms, device, s);
   else if (yb)
-    rc = fwd_types<float, __nv_bfloat16>(a, vec, ring, sms, device, s);
+    rc = fwd_types<float, __nv_bfloat16>(a, vec, vec8, alike, sms, device, s);
   else
-    rc = fwd_types<float, float>(a, vec, ring, sms, device, s);
+    rc = fwd_types<float, float>(a, vec, vec8, alike, sms, device, s);
   if (rc != MMN_OK) return rc;
   MMN_CUDA_TRY(cudaGetLastError());
   return MMN_OK;
@@ -1179,7 +1404,7 @@ extern "C" int mmn_layer_norm_backward_workspace(int64_t rows, int64_t cols, int
   int rc, sms = 0;
   if ((rc = check_extent(rows, cols)) != MMN_OK) return rc;
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
-  *bytes = (int64_t)bwd_parts(rows, cols, sms) * 2 * cols * 4;
+  *bytes = (int64_t)bwd_max_parts(rows, cols, sms) * 2 * cols * 4;
   return MMN_OK;
 }
 
@@ -1216,7 +1441,7 @@ extern "C" int mmn_layer_norm_backward(const void* dy, int64_t dy_ld, int dy_dty
   if (!empty && reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(MMN_E_INVALID, "workspace is not 16-byte aligned");
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
-  const int parts = bwd_parts(rows, cols, sms);
+  int parts = bwd_max_parts(rows, cols, sms);
   if (workspace_bytes < (int64_t)parts * 2 * cols * 4)
     return fail(MMN_E_INVALID, "workspace is smaller than mmn_layer_norm_backward_workspace gives");
   if (cols == 0) return MMN_OK;
@@ -1247,21 +1472,24 @@ extern "C" int mmn_layer_norm_backward(const void* dy, int64_t dy_ld, int dy_dty
     const bool vec = cols % v == 0 && vec_rows(x, a.x_ld, esize(x_dtype), v) &&
                      vec_rows(dy, a.dy_ld, esize(dy_dtype), v) &&
                      vec_rows(dx, a.dx_ld, esize(x_dtype), v) &&
-                     vec_rows(gamma, cols, esize(param_dtype), v);
+                     vec_rows(gamma, 0, esize(param_dtype), v);
     // dx in place of an input that a later row still reads is no hazard: a row is
     // read before its dx is written, and no other row is touched
     const bool ring = vec && (cols * esize(x_dtype)) % 16 == 0 && (cols * esize(dy_dtype)) % 16 == 0 &&
                       vec_rows(x, a.x_ld, esize(x_dtype), 16) &&
                       vec_rows(dy, a.dy_ld, esize(dy_dtype), 16);
+    const bool alike =
+        rows_agree(x, a.x_ld, esize(x_dtype), dy, a.dy_ld, esize(dy_dtype), v) &&
+        rows_agree(x, a.x_ld, esize(x_dtype), dx, a.dx_ld, esize(x_dtype), v);
     const bool xb = x_dtype == MMN_DTYPE_BF16, db = dy_dtype == MMN_DTYPE_BF16;
     if (xb && db)
-      rc = bwd_types<__nv_bfloat16, __nv_bfloat16>(a, parts, vec, ring, device, s);
+      rc = bwd_types<__nv_bfloat16, __nv_bfloat16>(a, &parts, vec, ring, alike, sms, device, s);
     else if (xb)
-      rc = bwd_types<__nv_bfloat16, float>(a, parts, vec, ring, device, s);
+      rc = bwd_types<__nv_bfloat16, float>(a, &parts, vec, ring, alike, sms, device, s);
     else if (db)
-      rc = bwd_types<float, __nv_bfloat16>(a, parts, vec, ring, device, s);
+      rc = bwd_types<float, __nv_bfloat16>(a, &parts, vec, ring, alike, sms, device, s);
     else
-      rc = bwd_types<float, float>(a, parts, vec, ring, device, s);
+      rc = bwd_types<float, float>(a, &parts, vec, ring, alike, sms, device, s);
     if (rc != MMN_OK) return rc;
     MMN_CUDA_TRY(cudaGetLastError());
   }

@@ -239,7 +239,12 @@ def test_strided_unaligned_and_in_place(mmn, cols):
     # forward in place, backward in place of dy and of x
     z = x0.clone()
     z2, m2, r2 = mmn.layer_norm(z, gamma, beta, 1e-5, out=z)
-    assert torch.equal(z, y.contiguous()) and torch.equal(m2, mean) and torch.equal(r2, rstd)
+    # bit for bit what the same layout gives out of place; against the slices' result, which
+    # another kernel sums in another order, within the bounds
+    for a, b in zip((z, m2, r2), mmn.layer_norm(x0, gamma, beta, 1e-5)):
+        assert torch.equal(a, b)
+    check_forward(z.view(rows, cols), m2.view(-1), r2.view(-1), x0.view(rows, cols), gamma, beta,
+                  1e-5)
     dy = torch.randn(2, 15, cols, device="cuda")
     want = mmn.layer_norm_backward(dy, x0, gamma, mean, rstd)
     for which in (0, 1):
@@ -248,6 +253,43 @@ def test_strided_unaligned_and_in_place(mmn, cols):
         assert got[0] is args[which]
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("xd,yd", list(itertools.product(("f32", "bf16"), repeat=2)))
+@pytest.mark.parametrize("cols,ld,rows", [(66, 67, 5), (130, 133, 2500), (509, 509, 1300),
+                                          (1021, 1024, 40), (2043, 2043, 700), (4095, 4097, 19),
+                                          (8185, 8185, 9), (8200, 8201, 170), (16377, 16377, 3),
+                                          (16383, 16383, 3), (600, 601, 1300), (1013, 1015, 1250),
+                                          (1500, 1501, 2400), (4051, 4051, 1201), (6002, 6003, 1190),
+                                          (9001, 9001, 1200)])
+def test_rows_that_start_anywhere(mmn, cols, ld, rows, xd, yd):
+    """Slices at offsets from an aligned address, x, dy and the outputs alike and not
+    alike: the bounds hold, NaN around the inputs is not read into the results, and what
+    lies around the outputs stays."""
+    import torch
+
+    x, gamma, beta, dy = make(rows, cols, xd, yd, seed=cols)
+
+    def place(t, off, fill):
+        buf = torch.full((rows * ld + 32,), fill, dtype=t.dtype, device="cuda")
+        v = buf[off:off + rows * ld].view(rows, ld)[:, :cols]
+        v.copy_(t)
+        return buf, v
+
+    nan = float("nan")
+    for off, out_off in ((0, 0), (1, 1), (3, 3), (7, 7), (2, 5)):
+        _, xv = place(x, off, nan)
+        ybuf, yv = place(torch.zeros_like(dy), out_off, 7.0)
+        _, mean, rstd = mmn.layer_norm(xv, gamma, beta, 1e-5, out=yv)
+        check_forward(yv, mean, rstd, x, gamma, beta, 1e-5)
+        yv.fill_(7.0)
+        assert (ybuf == 7.0).all(), off
+        _, dyv = place(dy, off, nan)
+        dbuf, dxv = place(torch.zeros_like(x), out_off, 7.0)
+        _, dgamma, dbeta = mmn.layer_norm_backward(dyv, xv, gamma, mean, rstd, out=dxv)
+        check_backward(dxv, dgamma, dbeta, dy, x, gamma, mean, rstd)
+        dxv.fill_(7.0)
+        assert (dbuf == 7.0).all(), off
 
 
 @pytest.mark.parametrize("rows,cols", [(270000, 8192), (70000, 32768)])
