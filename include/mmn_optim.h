@@ -519,7 +519,7 @@ int mmn_mxfp4_dequantize(const mmn_mxfp4 *q, void *out, int64_t out_ld, int dtyp
 
 /* out (a.rows x b.rows, fp32 or bf16) = A B^T, summed over the cols of both in
  * fp32 on the tensor cores and rounded once; accumulate = 1 adds it to what out
- * holds first. With W of a Linear layer ([out, in], crates/mmn-nn/src/lib.rs:305-307):
+ * holds first (fp32 values below 2^-126 may count as zero there). With W of a Linear layer ([out, in], crates/mmn-nn/src/lib.rs:305-307):
  * y = x W^T from (x, W); dx = dy W from (dy, W transposed); dW = dy^T x from (dy
  * transposed, x transposed), for example into a grad slot. A NaN block makes
  * the rows (columns) of out that sum over it NaN. */

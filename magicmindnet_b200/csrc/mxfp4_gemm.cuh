@@ -448,87 +448,105 @@ __global__ void __launch_bounds__(320, 1)
 }
 
 // Writes (or adds) a 32 x 32 block held one row per lane (v[j] = column j) to
-// out rows r0.., columns c0.., through the warp's 32 x 33 stage.
+// out rows r0.., columns c0.., through the warp's 32 x 33 stage: what cannot go by TMA,
+// rows that are not aligned and sums of bf16. 4096 x 14335 x 4095: 118 us bf16, 140
+// fp32 (14336: 101 and 118 by TMA; 136 with a bf16 element a lane and a store); added
+// to, 175 and 152 (292 and 366 with loads of eight rows before their stores); 14336
+// bf16, added to, 125 (161 with a load and a store at a time).
 __device__ __forceinline__ void mx_store_block(const MxGemmArgs& a, long long r0, long long c0,
                                                int rows, int cols, const float (&v)[32],
                                                float* tst) {
   const int lane = threadIdx.x & 31;
+  if (a.out_bf16 && !a.accumulate) {
+    // bf16 rows that start anywhere: each is packed into the words that its memory
+    // has (its first element left over where it starts half-way into one), and two rows
+    // are stored at a time.
+    __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(a.out) + r0 * a.ld + c0;
+    const int at = (int)(reinterpret_cast<uintptr_t>(out) >> 1), ld1 = (int)a.ld;
+    const int odd = (at + lane * ld1) & 1;
+    uint32_t w[17];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&p);
+    }
+    w[16] = 0;
+    if (odd && lane < rows)
+      *reinterpret_cast<uint16_t*>(out + lane * a.ld) = (uint16_t)w[0];
+    uint32_t* const ws = reinterpret_cast<uint32_t*>(tst);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], 16 * odd);
+#pragma unroll
+    for (int j = 0; j < 16; j += 4)
+      *reinterpret_cast<uint4*>(ws + lane * 20 + j) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+    __syncwarp();
+    const int h = lane >> 4, j = lane & 15;
+    const int o = (at + h * ld1) & 1, c = 2 * j + o;  // (rows two apart start alike)
+    __nv_bfloat16* to = out + h * a.ld + c;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t u = ws[(2 * i + h) * 20 + j];
+      if (2 * i + h < rows) {
+        if (c + 1 < cols)
+          *reinterpret_cast<uint32_t*>(to) = u;
+        else if (c < cols)
+          *reinterpret_cast<uint16_t*>(to) = (uint16_t)u;
+      }
+      to += 2 * a.ld;
+    }
+    __syncwarp();
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 32; ++j) tst[lane * 33 + j] = v[j];
   __syncwarp();
-  if (a.vec && cols == 32) {
-    if (a.out_bf16) {
-      const int rs = lane >> 2, c8 = (lane & 3) * 8;
+  if (!a.out_bf16) {
+    float* to = static_cast<float*>(a.out) + r0 * a.ld + c0 + lane;
+    if (a.accumulate) {
+      // (one addend per element, so the order is no matter; like TMA's, this addition
+      // flushes values below 2^-126 to zero)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = q * 8 + rs;
-        if (r < rows) {
-          uint4* p = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) +
-                                              (r0 + r) * a.ld + c0 + c8);
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = tst[r * 33 + c8 + i];
-          if (a.accumulate) {
-            const uint4 old = *p;
-            const __nv_bfloat162* o2 = reinterpret_cast<const __nv_bfloat162*>(&old);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f[2 * i] += __low2float(o2[i]);
-              f[2 * i + 1] += __high2float(o2[i]);
-            }
-          }
-          uint4 u;
-          __nv_bfloat162* u2 = reinterpret_cast<__nv_bfloat162*>(&u);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) u2[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-          *p = u;
-        }
-      }
+      for (int r = 0; r < 32; ++r, to += a.ld)
+        if (r < rows && lane < cols) atomicAdd(to, tst[r * 33 + lane]);
     } else {
-      const int rs = lane >> 3, c4 = (lane & 7) * 4;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int r = q * 4 + rs;
-        if (r < rows) {
-          float4* p =
-              reinterpret_cast<float4*>(static_cast<float*>(a.out) + (r0 + r) * a.ld + c0 + c4);
-          const float* t = tst + r * 33 + c4;
-          float4 u = make_float4(t[0], t[1], t[2], t[3]);
-          if (a.accumulate) {
-            const float4 o = *p;
-            u.x += o.x;
-            u.y += o.y;
-            u.z += o.z;
-            u.w += o.w;
-          }
-          *p = u;
-        }
-      }
+      for (int r = 0; r < 32; ++r, to += a.ld)
+        if (r < rows && lane < cols) *to = tst[r * 33 + lane];
+    }
+  } else if (a.vec && cols == 32) {
+    const int rs = lane >> 2, c8 = (lane & 3) * 8;
+    uint4* const p = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) +
+                                              (r0 + rs) * a.ld + c0 + c8);
+    uint4 old[4];  // all before the first store
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q * 8 + rs < rows) old[q] = p[q * a.ld];  // (8 rows are ld vectors of 8)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float* f = tst + (q * 8 + rs) * 33 + c8;
+      const __nv_bfloat162* o2 = reinterpret_cast<const __nv_bfloat162*>(&old[q]);
+      uint4 u;
+      __nv_bfloat162* u2 = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        u2[i] = __floats2bfloat162_rn(f[2 * i] + __low2float(o2[i]),
+                                      f[2 * i + 1] + __high2float(o2[i]));
+      if (q * 8 + rs < rows) p[q * a.ld] = u;
     }
   } else if (lane < cols) {
-    // a row per turn, one column per lane; loads of eight rows before their stores
-    const long long i0 = r0 * a.ld + c0 + lane;
+    // a row per turn, one column per lane; loads of sixteen rows before their stores
+    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + r0 * a.ld + c0 + lane;
 #pragma unroll 1
-    for (int r = 0; r < rows; r += 8) {
-      float f[8];
+    for (int r = 0; r < rows; r += 16) {
+      __nv_bfloat16 old[16];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        f[k] = tst[(r + k) * 33 + lane];
-        if (a.accumulate && r + k < rows) {
-          const long long i = i0 + (r + k) * a.ld;
-          f[k] += a.out_bf16 ? __bfloat162float(static_cast<__nv_bfloat16*>(a.out)[i])
-                             : static_cast<float*>(a.out)[i];
-        }
-      }
+      for (int k = 0; k < 16; ++k)
+        if (r + k < rows) old[k] = to[k * a.ld];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (r + k < rows) {
-          const long long i = i0 + (r + k) * a.ld;
-          if (a.out_bf16)
-            static_cast<__nv_bfloat16*>(a.out)[i] = __float2bfloat16_rn(f[k]);
-          else
-            static_cast<float*>(a.out)[i] = f[k];
-        }
+      for (int k = 0; k < 16; ++k)
+        if (r + k < rows)
+          to[k * a.ld] = __float2bfloat16_rn(tst[(r + k) * 33 + lane] + __bfloat162float(old[k]));
+      to += 16 * a.ld;
     }
   }
   __syncwarp();

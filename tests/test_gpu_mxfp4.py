@@ -326,6 +326,27 @@ def test_aligned_slices_leave_their_neighbours(mmn, m, n, k, accumulate, out):
     assert torch.equal(buf[outside], keep[outside])
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("m,n,k", [(700, 1111, 512), (1999, 1301, 300), (515, 1030, 130), (40, 263, 512)])
+def test_unaligned_slices_leave_their_neighbours(mmn, m, n, k, accumulate, out):
+    """The same with rows that start anywhere, at even and odd pitches and offsets."""
+    import torch
+
+    a, b = data(m, k, "f32", 3, 1.0), data(n, k, "f32", 4, 1.0)
+    qa, qb = mmn.mxfp4_quantize(a), mmn.mxfp4_quantize(b)
+    for pad, off in ((9, 1), (10, 2), (13, 7), (16, 3)):
+        buf = torch.randn(m + 2, n + pad, device="cuda").to(T(out))
+        keep = buf.clone()
+        view = buf[1:1 + m, off:off + n]
+        mmn.mxfp4_matmul(qa, qb, out=view, accumulate=accumulate)
+        check_product(view, plain_values(a), plain_values(b),
+                      keep[1:1 + m, off:off + n] if accumulate else None)
+        outside = torch.ones_like(buf, dtype=torch.bool)
+        outside[1:1 + m, off:off + n] = False
+        assert torch.equal(buf[outside], keep[outside])
+
+
 @pytest.mark.parametrize("m", [3, 200])
 def test_linear_within_one_buffer(mmn, m):
     """x and the result as column slices of one buffer; slices that meet are refused."""
