@@ -65,7 +65,6 @@ struct MxQuantArgs {
   int64_t pitch, pitch_t;       // bytes of one row of codes
   int ka, ka_t;                 // scale blocks of one 128-row tile
   int nct;                      // column tiles of the grid
-  int vec;                      // rows of x are 16-byte aligned
 };
 
 // The larger magnitudes of two pairs of bf16 (m >= 0); a NaN stays one.
@@ -100,10 +99,10 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes
 // a copy's rate); 16384 x 8192: 52, 53 and 74 us (1.0, 0.98, 0.85). With few waves
 // of blocks their loads and their work fall together; within a block "both" is 14
 // instructions an element (issue slots 69% busy, the shared-memory pipe 62%).
-template <typename T>
+template <typename T, bool SHIFT>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
   constexpr int kPitch = MxTile<T>::kPitch;
-  constexpr bool kBf16 = sizeof(T) == 2;
+  constexpr bool kBf16 = sizeof(T) == 2, kMove = SHIFT && !kBf16;
   extern __shared__ __align__(16) uint8_t sm[];
   uint8_t* codes_s = sm;  // the transposed codes take the tile's place once it is read
   uint8_t* sf_row = sm + 128 * kPitch;
@@ -127,8 +126,15 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
   }
   const T* x = static_cast<const T*>(a.x);
   const int nr = min(128, a.rows - r0), nc = min(128, a.cols - c0);
-  if (a.vec) {
-    constexpr int kPer = 16 / sizeof(T), kCh = 128 / kPer;
+  constexpr int kPer = 16 / sizeof(T), kCh = 128 / kPer;
+  // where row r's first element of the tile lies past a vector's start (the same in
+  // rows kPer apart)
+  const uint32_t e0 = (uint32_t)(reinterpret_cast<uintptr_t>(x) / sizeof(T)) +
+                      (uint32_t)r0 * (uint32_t)a.ld + (uint32_t)c0;
+  auto offset = [&](int r) {
+    return SHIFT ? (int)((e0 + (uint32_t)r * (uint32_t)a.ld) & (kPer - 1)) : 0;
+  };
+  if constexpr (!SHIFT) {
 #pragma unroll
     for (int i = 0; i < 128 * kCh / 256; ++i) {
       const int id = i * 256 + tid, r = id / kCh, c = (id % kCh) * kPer;
@@ -136,19 +142,15 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
       const T* src = bytes ? x + (int64_t)(r0 + r) * a.ld + c0 + c : x;
       cp_async16(sm + r * kPitch + c * sizeof(T), src, bytes);
     }
-    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
   } else {
-    // Rows that start anywhere arrive in whole vectors, the tile's first element o
-    // elements into the first (one vector more a row), and move to their place
-    // within shared memory. o is the same in every row of a thread: they lie a
-    // multiple of a vector's elements apart. 16384 x 4095 bf16 43 us, fp32 73 (80 and
-    // 128 with an element a load; 55 and 123 with the vectors moved in registers
-    // on their way to shared memory, which leaves fewer loads in flight).
-    constexpr int kPer = 16 / sizeof(T), kCh = 128 / kPer, kRows = 256 / kCh;
-    static_assert(kRows % kPer == 0, "rows of a thread differ in their offset");
+    // Rows that start anywhere arrive in whole vectors, one more a row. bf16 moves to
+    // its place within shared memory (44 to 45 us moved as it is read), fp32 as it is
+    // read (73 to 75 moved before). 16384 x 4095 bf16 43 us, fp32 69 along the rows and
+    // 64 along the columns (80 and 128 with an element a load; 55 and 123 with the
+    // vectors moved on their way to shared memory, which leaves fewer loads in flight).
     auto copy = [&](int r, int j) {
       const T* row = x + (int64_t)(r0 + r) * a.ld + c0;
-      const int c = j * kPer - vec_offset<T, kPer>(row);  // the vector's first column
+      const int c = j * kPer - offset(r);  // the vector's first column
       uint8_t* dst = sm + r * kPitch + j * 16;
       if (r < nr && c + c0 < 0 && row + c < x) {  // the matrix starts inside this vector
         for (int k = 0; k < kPer; ++k)
@@ -158,27 +160,29 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
         cp_async16(dst, bytes ? row + c : x - vec_offset<T, kPer>(x), bytes);
       }
     };
-    const int r1 = tid / kCh, j1 = tid % kCh;
 #pragma unroll
-    for (int i = 0; i < 128 / kRows; ++i) copy(i * kRows + r1, j1);
+    for (int i = 0; i < 128 * kCh / 256; ++i) copy((i * 256 + tid) / kCh, tid % kCh);
     if (tid < 128) copy(tid, kCh);
-    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
-    const int o = vec_offset<T, kPer>(x + (int64_t)(r0 + r1) * a.ld + c0);
+  }
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  if constexpr (SHIFT && kBf16) {
+    constexpr int kRows = 256 / kCh;
+    static_assert(kRows % kPer == 0, "rows of a thread differ in their offset");
+    const int r1 = tid / kCh, j1 = tid % kCh, o = offset(r1);
 #pragma unroll
     for (int i = 0; i < 128 / kRows; ++i) {
       // (the lanes of a warp take whole rows)
       uint4* at = reinterpret_cast<uint4*>(sm + (i * kRows + r1) * kPitch) + j1;
       const uint4 u = at[0], v = at[1];
-      const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-      uint32_t m[4];
-      shift_down<T, kPer>(w, o, m);
-      if (c0 + 128 > a.cols) keep_first<T, kPer>(m, nc - j1 * kPer);
+      uint32_t d[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      shift_down<T, 4>(d, o);
+      if (nc < 128) keep_first<T, 4>(d, nc - j1 * kPer);
       __syncwarp();
-      at[0] = make_uint4(m[0], m[1], m[2], m[3]);
+      at[0] = make_uint4(d[0], d[1], d[2], d[3]);
     }
+    __syncthreads();
   }
-  __syncthreads();
 
   if (a.codes) {
     // a thread per block of 32: eight rows at a time read the same columns, so the
@@ -186,48 +190,40 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = (i * 8 + (tid >> 5)) * 8 + (tid & 7), k4 = (tid >> 3) & 3;
-      uint32_t q4[4], s;
+      constexpr int N = 8 * (int)sizeof(T);  // words of a block
+      uint32_t d[N + 4], q4[4], s;
+#pragma unroll
+      for (int q = 0; q < N / 4 + (kMove ? 1 : 0); ++q) {
+        const uint4 u =
+            *reinterpret_cast<const uint4*>(sm + r * kPitch + k4 * 32 * sizeof(T) + q * 16);
+        d[4 * q] = u.x, d[4 * q + 1] = u.y, d[4 * q + 2] = u.z, d[4 * q + 3] = u.w;
+      }
+      if constexpr (kMove) {
+        shift_down<T, N>(d, offset(r));
+        if (nc < 128) keep_first<T, N>(d, nc - k4 * 32);
+      }
       if constexpr (kBf16) {
-        uint4 u[4];
         uint32_t mm = 0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          u[q] = *reinterpret_cast<const uint4*>(sm + r * kPitch + k4 * 64 + q * 16);
-          mm = max_abs2(max_abs2(mm, u[q].x), u[q].y);
-          mm = max_abs2(max_abs2(mm, u[q].z), u[q].w);
-        }
+        for (int k = 0; k < 16; ++k) mm = max_abs2(mm, d[k]);
         s = mx_scale(max(mm & 0xFFFFu, mm >> 16) << 16);
-        const float inv = mx_inv_scale(s);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t w[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
-          float v[8];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            v[2 * k] = __uint_as_float(w[k] << 16) * inv;
-            v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u) * inv;
-          }
-          q4[q] = e2m1x8(v);
-        }
       } else {
-        float w[32];
         uint32_t m = 0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float4 f = *reinterpret_cast<const float4*>(sm + r * kPitch + k4 * 128 + q * 16);
-          w[4 * q] = f.x, w[4 * q + 1] = f.y, w[4 * q + 2] = f.z, w[4 * q + 3] = f.w;
-        }
-#pragma unroll
-        for (int k = 0; k < 32; ++k) m = max(m, __float_as_uint(w[k]) & 0x7FFFFFFFu);
+        for (int k = 0; k < 32; ++k) m = max(m, d[k] & 0x7FFFFFFFu);
         s = mx_scale(m);
-        const float inv = mx_inv_scale(s);
+      }
+      const float inv = mx_inv_scale(s);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[8];
+      for (int q = 0; q < 4; ++q) {
+        float v[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = w[q * 8 + k] * inv;
-          q4[q] = e2m1x8(v);
-        }
+        for (int k = 0; k < 8; ++k)
+          v[k] = __uint_as_float(!kBf16  ? d[(q * 8 + k) % N]
+                                 : k & 1 ? d[q * 4 + k / 2] & 0xFFFF0000u
+                                         : d[q * 4 + k / 2] << 16) *
+                 inv;
+        q4[q] = e2m1x8(v);
       }
       const int64_t off = (int64_t)ct * 64 + k4 * 16;
       if (r < nr && off < a.pitch)
@@ -272,7 +268,8 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          w[i] = *reinterpret_cast<const float*>(sm + (rb * 32 + i) * kPitch + c * 4);
+          w[i] = *reinterpret_cast<const float*>(sm + (rb * 32 + i) * kPitch + (c + (kMove ? offset(i) : 0)) * 4);
+          if (kMove && c >= nc) w[i] = 0.0f;
           m = max(m, __float_as_uint(w[i]) & 0x7FFFFFFFu);
         }
         sb[half] = mx_scale(m);
@@ -519,7 +516,8 @@ int kernel_setup(int device) {
   std::lock_guard<std::mutex> lock(mu);
   if (device < 64 && (done >> device) & 1u) return MMN_OK;
   const auto smem = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_quantize_kernel<float>, smem, MxTile<float>::kSmem));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_quantize_kernel<float, false>, smem, MxTile<float>::kSmem));
+  MMN_CUDA_TRY(cudaFuncSetAttribute(mx_quantize_kernel<float, true>, smem, MxTile<float>::kSmem));
   int rc;
   if ((rc = split_setup<16, 0>()) != MMN_OK || (rc = split_setup<32, 0>()) != MMN_OK ||
       (rc = split_setup<64, 0>()) != MMN_OK || (rc = split_setup<128, 0>()) != MMN_OK ||
@@ -552,15 +550,16 @@ int launch_quantize(const void* x, int64_t ld, int dtype, int64_t rows, int64_t 
   a.ka_t = (int)scale_blocks(rows);
   a.nct = q ? a.ka : (int)((cols + 127) / 128);
   const int64_t nrt = qt ? a.ka_t : (rows + 127) / 128;
-  a.vec = vec_rows(x, ld, esize(dtype), 16);
+  const bool vec = vec_rows(x, ld, esize(dtype), 16);
   const int64_t blocks = nrt * a.nct;
   if (blocks > (int64_t(1) << 31) - 1) return fail(MMN_E_SHAPE, "matrix too large");
   const dim3 grid((unsigned)blocks);
-  if (dtype == MMN_DTYPE_BF16)
-    MMN_CUDA_TRY(launch_dependent(mx_quantize_kernel<__nv_bfloat16>, grid, 256,
-                                  MxTile<__nv_bfloat16>::kSmem, s, a));
-  else
-    MMN_CUDA_TRY(launch_dependent(mx_quantize_kernel<float>, grid, 256, MxTile<float>::kSmem, s, a));
+  const bool bf = dtype == MMN_DTYPE_BF16;
+  const auto kernel = bf ? (vec ? mx_quantize_kernel<__nv_bfloat16, false>
+                                : mx_quantize_kernel<__nv_bfloat16, true>)
+                         : (vec ? mx_quantize_kernel<float, false> : mx_quantize_kernel<float, true>);
+  MMN_CUDA_TRY(launch_dependent(kernel, grid, 256,
+                                bf ? MxTile<__nv_bfloat16>::kSmem : MxTile<float>::kSmem, s, a));
   return MMN_OK;
 }
 
