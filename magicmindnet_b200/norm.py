@@ -10,6 +10,7 @@ object and a shape tuple for every tensor, about half without.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 from . import _native as N
 from .optim import _CUDA_STREAM_LEGACY
@@ -123,9 +124,11 @@ def layer_norm(x, gamma, beta, eps: float = 1e-5, out_dtype=None, out=None):
         old = _rows_view(out, "out")[2]
     dev = x.device
     if x.dim() == 2:
-        mean, rstd = _t.empty(2, rows, dtype=_t.float32, device=dev).unbind(0)
+        mean = _t.empty(rows, dtype=_t.float32, device=dev)
+        rstd = _t.empty(rows, dtype=_t.float32, device=dev)
     else:
-        mean, rstd = _t.empty(2, *x.shape[:-1], dtype=_t.float32, device=dev).unbind(0)
+        mean = _t.empty(x.shape[:-1], dtype=_t.float32, device=dev)
+        rstd = _t.empty(x.shape[:-1], dtype=_t.float32, device=dev)
     if cols == 0:
         mean.zero_()
         rstd.fill_(float("inf") if eps == 0 else eps ** -0.5)
@@ -134,6 +137,14 @@ def layer_norm(x, gamma, beta, eps: float = 1e-5, out_dtype=None, out=None):
         out.data_ptr(), old, _dtype(out, "out"), mean.data_ptr(), rstd.data_ptr(), index,
         _stream(index)))
     return out, mean, rstd
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, cols: int, index: int) -> int:
+    """mmn_layer_norm_backward_workspace, which depends on nothing else."""
+    need = ctypes.c_int64()
+    N.check(N.lib().mmn_layer_norm_backward_workspace(rows, cols, index, need))
+    return need.value
 
 
 def layer_norm_backward(dy, x, gamma, mean, rstd, dgamma=None, dbeta=None,
@@ -159,7 +170,8 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, dgamma=None, dbeta=None,
         raise ValueError("accumulate=True needs dgamma and dbeta to add to")
     dev = x.device
     if dgamma is None and dbeta is None:
-        dgamma, dbeta = _t.empty(2, cols, dtype=_t.float32, device=dev).unbind(0)
+        dgamma = _t.empty(cols, dtype=_t.float32, device=dev)
+        dbeta = _t.empty(cols, dtype=_t.float32, device=dev)
         gd = N.DTYPE_F32
     else:
         if dgamma is None:
@@ -177,12 +189,10 @@ def layer_norm_backward(dy, x, gamma, mean, rstd, dgamma=None, dbeta=None,
         if out.shape != x.shape or out.dtype != x.dtype:
             raise N.ShapeError(N.MMN_E_SHAPE, "out must have x's shape and dtype")
         old = _rows_view(out, "out")[2]
-    L = N.lib()
-    need = ctypes.c_int64()
-    N.check(L.mmn_layer_norm_backward_workspace(rows, cols, index, need))
-    ws = _t.empty(need.value, dtype=_t.uint8, device=dev)
-    N.check(L.mmn_layer_norm_backward(
+    need = _workspace_bytes(rows, cols, index)
+    ws = _t.empty(need, dtype=_t.uint8, device=dev)
+    N.check(N.lib().mmn_layer_norm_backward(
         dy.data_ptr(), dld, dd, x.data_ptr(), ld, xd, gamma.data_ptr(), pd, mean.data_ptr(),
         rstd.data_ptr(), rows, cols, out.data_ptr(), old, dgamma.data_ptr(), dbeta.data_ptr(), gd,
-        bool(accumulate), ws.data_ptr(), need.value, index, _stream(index)))
+        bool(accumulate), ws.data_ptr(), need, index, _stream(index)))
     return out, dgamma, dbeta

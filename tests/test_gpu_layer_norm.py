@@ -292,6 +292,18 @@ def test_rows_that_start_anywhere(mmn, cols, ld, rows, xd, yd):
         assert (dbuf == 7.0).all(), off
 
 
+def test_one_row_as_a_vector(mmn):
+    import torch
+
+    x, gamma, beta, dy = make(1, 200, "f32", "f32", seed=3)
+    y, mean, rstd = mmn.layer_norm(x[0], gamma, beta)
+    assert y.shape == (200,) and mean.shape == rstd.shape == ()
+    check_forward(y[None], mean[None], rstd[None], x, gamma, beta, 1e-5)
+    dx, dgamma, dbeta = mmn.layer_norm_backward(dy[0], x[0], gamma, mean, rstd)
+    assert dx.shape == (200,)
+    check_backward(dx[None], dgamma, dbeta, dy, x, gamma, mean, rstd)
+
+
 @pytest.mark.parametrize("rows,cols", [(270000, 8192), (70000, 32768)])
 def test_offsets_beyond_32_bits(mmn, rows, cols):
     """More than 2^31 elements: the last rows, and the sums over all of them."""
