@@ -23,15 +23,14 @@ int cuda_fail(cudaError_t e, const char* what);
     if (_e != cudaSuccess) return cuda_fail(_e, #expr); \
   } while (0)
 
-// Makes `dev` current for a scope and restores the previous device after it.
+// Makes `dev` current for a scope and restores the previous device after it. The
+// device is set even where cudaGetDevice names it already: a thread may hold a context
+// of its own on that GPU, and the library's memory and kernels are in the primary
+// one, which cudaSetDevice makes current.
 struct DeviceGuard {
   int prev = -1;
   explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev == dev) {
-      prev = -1;  // nothing to change or restore
-      return;
-    }
+    if (cudaGetDevice(&prev) != cudaSuccess || prev == dev) prev = -1;
     cudaSetDevice(dev);
   }
   ~DeviceGuard() {
