@@ -1357,10 +1357,15 @@ extern "C" int mmn_layer_norm(const void* x, int64_t x_ld, int x_dtype, const vo
     const MatrixIn mx{x, rows > 1 ? x_ld : cols, rows, cols, esize(x_dtype)};
     const MatrixIn my{y, rows > 1 ? y_ld : cols, rows, cols, esize(y_dtype)};
     const MatrixIn mm{mean, rows, mean ? 1 : 0, rows, 4}, mr{rstd, rows, rstd ? 1 : 0, rows, 4};
+    const MatrixIn mg{gamma, cols, 1, cols, esize(param_dtype)};
+    const MatrixIn mb{beta, cols, 1, cols, esize(param_dtype)};
     if ((rc = check_out_overlap(my, "y", mx)) != MMN_OK) return rc;
-    if (matrices_overlap(mm, mr) || matrices_overlap(mm, my) || matrices_overlap(mr, my) ||
-        matrices_overlap(mm, mx) || matrices_overlap(mr, mx))
-      return fail(MMN_E_INVALID, "mean or rstd overlaps another buffer");
+    if (matrices_overlap(my, mg) || matrices_overlap(my, mb))
+      return fail(MMN_E_INVALID, "y overlaps gamma or beta");
+    if (matrices_overlap(mm, mr)) return fail(MMN_E_INVALID, "mean and rstd overlap");
+    for (const MatrixIn& m : {mx, my, mg, mb})
+      if (matrices_overlap(mm, m) || matrices_overlap(mr, m))
+        return fail(MMN_E_INVALID, "mean or rstd overlaps another buffer");
   }
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
   if (empty) return MMN_OK;
@@ -1430,13 +1435,18 @@ extern "C" int mmn_layer_norm_backward(const void* dy, int64_t dy_ld, int dy_dty
   if (matrices_overlap(mg, mb)) return fail(MMN_E_INVALID, "dgamma and dbeta overlap");
   if (!empty) {
     const MatrixIn mdx{dx, rows > 1 ? dx_ld : cols, rows, cols, esize(x_dtype)};
-    if ((rc = check_out_overlap(mdx, "dx", {x, rows > 1 ? x_ld : cols, rows, cols,
-                                            esize(x_dtype)})) != MMN_OK ||
-        (rc = check_out_overlap(mdx, "dx", {dy, rows > 1 ? dy_ld : cols, rows, cols,
-                                            esize(dy_dtype)})) != MMN_OK)
+    const MatrixIn mx{x, rows > 1 ? x_ld : cols, rows, cols, esize(x_dtype)};
+    const MatrixIn mdy{dy, rows > 1 ? dy_ld : cols, rows, cols, esize(dy_dtype)};
+    const MatrixIn small[] = {{gamma, cols, 1, cols, esize(param_dtype)}, {mean, rows, 1, rows, 4},
+                              {rstd, rows, 1, rows, 4}};
+    if ((rc = check_out_overlap(mdx, "dx", mx)) != MMN_OK ||
+        (rc = check_out_overlap(mdx, "dx", mdy)) != MMN_OK)
       return rc;
-    if (matrices_overlap(mg, mdx) || matrices_overlap(mb, mdx))
-      return fail(MMN_E_INVALID, "dgamma or dbeta overlaps dx");
+    for (const MatrixIn& m : small)
+      if (matrices_overlap(mdx, m)) return fail(MMN_E_INVALID, "dx overlaps gamma, mean or rstd");
+    for (const MatrixIn& m : {mdx, mx, mdy, small[0], small[1], small[2]})
+      if (matrices_overlap(mg, m) || matrices_overlap(mb, m))
+        return fail(MMN_E_INVALID, "dgamma or dbeta overlaps another buffer");
   }
   if (!empty && reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(MMN_E_INVALID, "workspace is not 16-byte aligned");

@@ -83,6 +83,45 @@ def test_backward_allowed_up_to_the_device(N, kw):
     assert bwd(N, **kw) == gate(N)
 
 
+# gamma, beta, mean and rstd lie at G, B, M, R; x at X, and dy (backward) or y at Y.
+# An output that a block writes while another still reads it as an input is refused.
+@pytest.mark.parametrize("kw", [
+    dict(y=G), dict(y=B), dict(y=vp(0x300000 - 4 * 255)),  # y's last element is gamma's first
+    dict(mean=G), dict(rstd=G), dict(mean=vp(0x400000 + 4 * 63)), dict(rstd=vp(0x400000 - 12)),
+    dict(y=vp(0x300000 - 2 * 64), yd=BF16), dict(beta=vp(0x200000), pd=BF16),
+])
+def test_forward_refuses_outputs_over_the_parameters(N, kw):
+    assert fwd(N, **kw) == N.MMN_E_INVALID
+    assert b"overlap" in N.lib().mmn_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(dx=a) for a in (G, M, R)] + [
+    dict(dx=vp(0x300000 + 4 * 63)), dict(dx=vp(0x500000 - 4 * 255)), dict(mean=vp(0x900010)),
+] + [{d: a} for d in ("dgamma", "dbeta") for a in (X, Y, G, M, R)] + [
+    dict(dgamma=vp(0x500000 - 4 * 63)), dict(dbeta=vp(0x300000 + 2 * 63), pd=BF16, gd=BF16),
+])
+def test_backward_refuses_outputs_over_the_inputs(N, kw):
+    assert bwd(N, **kw) == N.MMN_E_INVALID
+    assert b"overlap" in N.lib().mmn_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(y=vp(0x300000 - 4 * 256)), dict(mean=vp(0x300000 - 16)), dict(rstd=vp(0x400000 + 4 * 64)),
+    # gamma in the gap between the rows of y
+    dict(y_ld=256, y=vp(0x300000 - 4 * 64)),
+])
+def test_forward_allows_neighbours_of_the_parameters(N, kw):
+    assert fwd(N, **kw) == gate(N)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dx=vp(0x300000 - 4 * 256)), dict(dgamma=vp(0x500000 + 16)), dict(dbeta=vp(0x300000 - 256)),
+    dict(dx_ld=256, dx=vp(0x300000 - 4 * 64)),
+])
+def test_backward_allows_neighbours_of_the_inputs(N, kw):
+    assert bwd(N, **kw) == gate(N)
+
+
 def test_workspace_arguments(N):
     n = ctypes.c_int64()
     f = N.lib().mmn_layer_norm_backward_workspace
