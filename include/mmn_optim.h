@@ -115,6 +115,10 @@ int mmn_abi_version(void);
  * MMN_OK if it did not time out. No counterpart in the reference. */
 int mmn_selftest_bounded_wait(int device, uint64_t limit_ns);
 
+/* Enqueues the same wait on `stream` (NULL = legacy default stream) and returns;
+ * its time-out is reported as a layer operator's is (mmn_kernel_status). */
+int mmn_selftest_layer_wait(int device, uint64_t limit_ns, void *stream);
+
 /* AdamWConfig::default() / MuonConfig::default() (lib.rs:13-21, 71-80). */
 mmn_adamw_config mmn_adamw_config_default(void);
 mmn_muon_config mmn_muon_config_default(void);
@@ -318,7 +322,10 @@ int mmn_optim_step(mmn_optim_t *h, float grad_divisor);
 int mmn_optim_step_host(mmn_optim_t *h, const void *const *grads, float *const *params,
                         float grad_divisor);
 
-/* Wait for the handle's stream; reports MMN_E_TIMEOUT if a kernel gave up. */
+/* Wait for the handle's stream; reports MMN_E_TIMEOUT if a kernel of the handle
+ * gave up a bounded wait, or a layer operator's kernel on its device (see
+ * mmn_kernel_status), whose results may be the grads that a step has used, since
+ * this handle was made or last reported one. mmn_optim_step_host reports alike. */
 int mmn_optim_sync(mmn_optim_t *h);
 
 /* Loss-scaling state (after mmn_optim_sync): current scale, steps skipped. */
@@ -536,8 +543,9 @@ int mmn_mxfp4_linear(const void *x, int64_t x_ld, int x_dtype, int64_t rows, con
                      void *stream);
 
 /* Waits for `stream` and reports MMN_E_TIMEOUT when a kernel of the calls above
- * gave up a bounded wait on `device` since the last report (mmn_optim_sync does
- * this for a handle's kernels). */
+ * gave up a bounded wait on `device` since this function's last report; what
+ * such a kernel wrote is not to be used. Every mmn_optim_sync and
+ * mmn_optim_step_host on that device reports it too, each handle for itself. */
 int mmn_kernel_status(int device, void *stream);
 
 /* Parameter counts: total registered, stepped by AdamW, stepped by Muon. */

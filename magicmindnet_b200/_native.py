@@ -91,6 +91,7 @@ SIGNATURES = {
     "mmn_last_error": (ctypes.c_char_p, []),
     "mmn_abi_version": (_i, []),
     "mmn_selftest_bounded_wait": (_i, [_i, _u64]),
+    "mmn_selftest_layer_wait": (_i, [_i, _u64, _vp]),
     "mmn_adamw_config_default": (AdamWConfigC, []),
     "mmn_muon_config_default": (MuonConfigC, []),
     "mmn_adamw_create": (_i, [ctypes.POINTER(AdamWConfigC), _i, _vp, ctypes.POINTER(_vp)]),

@@ -159,6 +159,9 @@ struct mmn_optim {
   // reduce_grads / scan_shard handles: the grads of the coming step went
   // through mmn_optim_reduce_grads / mmn_optim_scan_grads
   bool grads_ready = false;
+  int layer_timeouts = 0;  // of the caller-buffer kernels, as last reported
+  int* timeout_word = nullptr;  // ... where they count them on the device
+  int* status_host = nullptr;   // page-locked: the handle's status word, that count
 
   struct Slot {
     uint64_t id = 0;
@@ -293,6 +296,16 @@ extern "C" mmn_optim_config mmn_optim_config_default(void) {
   return c;
 }
 
+// What a handle needs to see the layer operators' time-outs: it reports those from
+// here on.
+static int watch_layers(mmn_optim_t* h) {
+  const int rc = kernel_timeout_word(h->ctx.device, &h->timeout_word);
+  if (rc != MMN_OK) return rc;
+  MMN_CUDA_TRY(cudaMallocHost(&h->status_host, 2 * sizeof(int)));
+  MMN_CUDA_TRY(cudaMemcpy(&h->layer_timeouts, h->timeout_word, sizeof(int), cudaMemcpyDeviceToHost));
+  return MMN_OK;
+}
+
 extern "C" int mmn_optim_create(const mmn_optim_config* cfg, int device, void* stream,
                                 mmn_optim_t** out) {
   if (!out) return fail(MMN_E_INVALID, "out is null");
@@ -315,8 +328,10 @@ extern "C" int mmn_optim_create(const mmn_optim_config* cfg, int device, void* s
   if (rc == MMN_OK) {
     DeviceGuard g(device);
     rc = h->bc.build(c.adamw.beta1, c.adamw.beta2);
+    if (rc == MMN_OK) rc = watch_layers(h);
   }
   if (rc != MMN_OK) {
+    if (h->status_host) cudaFreeHost(h->status_host);
     h->ctx.release();
     delete h;
     return rc;
@@ -333,6 +348,7 @@ extern "C" int mmn_optim_destroy(mmn_optim_t* h) {
   for (auto& c : h->classes) ns_class_free(c);
   for (void* p : h->peer_maps) cudaIpcCloseMemHandle(p);
   for (void* p : h->allocs) cudaFree(p);
+  if (h->status_host) cudaFreeHost(h->status_host);
   for (auto& set : h->ev_sets)
     for (auto e : set)
       if (e) cudaEventDestroy(e);
@@ -1244,6 +1260,19 @@ extern "C" int mmn_optim_step(mmn_optim_t* h, float grad_divisor) {
   return rc;
 }
 
+// Waits for the handle's stream; a bounded wait that a kernel of the handle gave up,
+// or one of the layer operators, whose results are the grads of a step. Both words
+// come back behind one wait (10 us a call; 24 with two copies that each wait).
+static int check_kernels(mmn_optim_t* h) {
+  const cudaStream_t s = h->ctx.stream;
+  MMN_CUDA_TRY(cudaMemcpyAsync(h->status_host, h->ctx.status, sizeof(int), cudaMemcpyDeviceToHost, s));
+  MMN_CUDA_TRY(cudaMemcpyAsync(h->status_host + 1, h->timeout_word, sizeof(int),
+                               cudaMemcpyDeviceToHost, s));
+  MMN_CUDA_TRY(cudaStreamSynchronize(s));
+  if (h->status_host[0] != kDevOk) return h->ctx.check_status();
+  return report_timeouts(h->status_host[1], &h->layer_timeouts);
+}
+
 extern "C" int mmn_optim_step_host(mmn_optim_t* h, const void* const* grads,
                                    float* const* params, float grad_divisor) {
   if (!h) return fail(MMN_E_INVALID, "null handle");
@@ -1274,13 +1303,13 @@ extern "C" int mmn_optim_step_host(mmn_optim_t* h, const void* const* grads,
   MMN_CUDA_TRY(cudaStreamWaitEvent(h->ctx.stream, h->out_ev, 0));
   if (rc != MMN_OK) return rc;
   MMN_CUDA_TRY(cudaEventSynchronize(h->out_ev));
-  return h->ctx.check_status();
+  return check_kernels(h);
 }
 
 extern "C" int mmn_optim_sync(mmn_optim_t* h) {
   if (!h) return fail(MMN_E_INVALID, "null handle");
   DeviceGuard g(h->ctx.device);
-  return h->ctx.check_status();
+  return check_kernels(h);
 }
 
 extern "C" int mmn_optim_loss_scale(mmn_optim_t* h, float* scale, int64_t* skipped_steps) {

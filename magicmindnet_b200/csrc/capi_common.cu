@@ -159,20 +159,29 @@ int check_device_ptr(const void* p, int device, const char* what) {
   return MMN_OK;
 }
 
-// A caller-buffer kernel that gave up a bounded wait leaves its code here, per
-// device (mmn_kernel_status).
-__device__ int g_kernel_status;
+// How many bounded waits caller-buffer kernels have given up, per device. It only
+// grows: mmn_kernel_status and every handle remember what they have reported, so
+// that none takes a report from another and nothing is lost in between.
+__device__ int g_kernel_timeouts;
 
-int kernel_status_word(int device, int** p) {
+int kernel_timeout_word(int device, int** p) {
   // the address is fixed per device: asked for once (any thread writes the same)
   static std::atomic<int*> known[64];
   int* k = device < 64 ? known[device].load(std::memory_order_relaxed) : nullptr;
   if (!k) {
-    MMN_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(&k), g_kernel_status));
+    MMN_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void**>(&k), g_kernel_timeouts));
     if (device < 64) known[device].store(k, std::memory_order_relaxed);
   }
   *p = k;
   return MMN_OK;
+}
+
+int report_timeouts(int count, int* reported) {
+  const int n = count - *reported;
+  if (n <= 0) return MMN_OK;  // (another thread may have reported a later count)
+  *reported = count;
+  return fail(MMN_E_TIMEOUT, "a layer operator's kernel gave up a bounded wait (" +
+                                 std::to_string(n) + " since the last report)");
 }
 
 int check_device_elems(const void* p, size_t esize, int device, const char* what) {
@@ -268,7 +277,33 @@ __global__ void selftest_wait_kernel(uint64_t limit_ns, int* status) {
   if (threadIdx.x == 0 && !mmn::mbar_wait(&bar, 0, &abort_flag, limit_ns))
     atomicExch(status, mmn::kDevWaitTimeout);
 }
+
+// The same wait, counted as a caller-buffer kernel's.
+__global__ void selftest_layer_wait_kernel(uint64_t limit_ns, int* timeouts) {
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ int abort_flag;
+  if (threadIdx.x == 0) {
+    mmn::mbar_init(&bar, 1);
+    abort_flag = 0;
+    mmn::fence_barrier_init();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && !mmn::mbar_wait(&bar, 0, &abort_flag, limit_ns)) atomicAdd(timeouts, 1);
+}
 }  // namespace
+
+int mmn_selftest_layer_wait(int device, uint64_t limit_ns, void* stream) {
+  using namespace mmn;
+  if (limit_ns == 0 || limit_ns > 2000000000ull) return fail(MMN_E_INVALID, "limit must be in (0, 2 s]");
+  int rc, sms = 0;
+  if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
+  DeviceGuard guard(device);
+  int* word = nullptr;
+  if ((rc = kernel_timeout_word(device, &word)) != MMN_OK) return rc;
+  selftest_layer_wait_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(limit_ns, word);
+  MMN_CUDA_TRY(cudaGetLastError());
+  return MMN_OK;
+}
 
 int mmn_selftest_bounded_wait(int device, uint64_t limit_ns) {
   using namespace mmn;

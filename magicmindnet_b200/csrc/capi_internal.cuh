@@ -83,9 +83,12 @@ int check_device_ptr(const void* p, int device, const char* what);
 // check_device_ptr, and `p` is aligned to its elements of `esize` bytes.
 int check_device_elems(const void* p, size_t esize, int device, const char* what);
 
-// The status word of the caller-buffer kernels (mmn_kernel_status) on `device`,
-// which is current.
-int kernel_status_word(int device, int** p);
+// The word in which the caller-buffer kernels on `device`, which is current, count
+// the bounded waits that they gave up (mmn_kernel_status, mmn_optim_sync).
+int kernel_timeout_word(int device, int** p);
+
+// MMN_E_TIMEOUT when the count has grown past what was *reported, which becomes it.
+int report_timeouts(int count, int* reported);
 
 // The device checks of the caller-buffer entry points: a usable sm_100 GPU,
 // whose SM count goes to *sms.

@@ -496,7 +496,7 @@ __host__ __device__ constexpr int ln_ring_blocks(int tr, int ne) {
 
 template <typename XT, typename YT, int TR, int NE, bool EDGE>
 __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR, NE))
-    ln_fwd_ring_kernel(const LnFwd a, int depth, int* status) {
+    ln_fwd_ring_kernel(const LnFwd a, int depth, int* timeouts) {
   constexpr int V = sizeof(XT) == 2 && sizeof(YT) == 2 ? 8 : 4;
   constexpr int kBlock = ln_ring_block(TR), RB = kBlock / TR, NC = NE / V, H = V / 2;
   extern __shared__ __align__(16) uint8_t dyn[];
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR, NE))
     const bool ok = k < mine;
     const int lim = ok ? cols : -V;  // (below a row's first vector: no row, no columns)
     const XT* sx = reinterpret_cast<const XT*>(ring + slot * rb) + at;
-    // (a wait that gives up marks the status; the loop runs on so that every
+    // (a wait that gives up is counted; the loop runs on so that every
     // barrier is met)
     if (ok) mbar_wait(&bars[sub][slot], phase, &abort_flag);
     f2 v[NE / 2], s = 0;
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR, NE))
       phase ^= 1u;
     }
   }
-  if (abort_flag && threadIdx.x == 0) atomicExch(status, kDevWaitTimeout);
+  if (abort_flag && threadIdx.x == 0) atomicAdd(timeouts, 1);
 }
 
 // ------------------------------------------------------------------ backward
@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
 // the second pass reads the row again.
 template <typename XT, typename DT, int V, int TR, int NE, bool EDGE>
 __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
-    ln_bwd_ring_kernel(const LnBwd a, int depth, int* status) {
+    ln_bwd_ring_kernel(const LnBwd a, int depth, int* timeouts) {
   constexpr int kBlock = ln_bwd_block(TR), RB = kBlock / TR, NC = NE / V, H = V / 2;
   constexpr bool kReread = NE > 16;
   extern __shared__ __align__(16) uint8_t dyn[];
@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
       mean2 = a.mean[row + step];
       rstd2 = a.rstd[row + step];
     }
-    // (a wait that gives up marks the status; the loop runs on so that every
+    // (a wait that gives up is counted; the loop runs on so that every
     // barrier is met)
     if (ok) mbar_wait(&bars[sub][slot], phase, &abort_flag);
     const f2 nm = dup2(-mean), r2 = dup2(rstd);
@@ -911,7 +911,7 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
     }
   }
   griddep_launch_dependents();  // ln_bwd_sum_kernel may take its place; it waits for the sums
-  if (abort_flag && threadIdx.x == 0) atomicExch(status, kDevWaitTimeout);
+  if (abort_flag && threadIdx.x == 0) atomicAdd(timeouts, 1);
   float* out = a.partial + (int64_t)blockIdx.x * 2 * a.cols;
   if constexpr (RB == 1) {
 #pragma unroll
@@ -1126,17 +1126,17 @@ int ring_fwd_launch(const LnFwd& a, int sms, int device, cudaStream_t s) {
   static std::mutex mu;
   static uint64_t done = 0;
   auto* kernel = ln_fwd_ring_kernel<XT, YT, TR, NE, EDGE>;
-  int* status = nullptr;
+  int* timeouts = nullptr;
   int rc;
   if ((rc = raise_smem(kernel, device, mu, done)) != MMN_OK) return rc;
-  if ((rc = kernel_status_word(device, &status)) != MMN_OK) return rc;
+  if ((rc = kernel_timeout_word(device, &timeouts)) != MMN_OK) return rc;
   const int64_t row = EDGE ? hull_bytes(a.cols, sizeof(XT)) : a.cols * (int64_t)sizeof(XT);
   // more rows in flight cost bandwidth (16384 x 4096: 43.6 us with 2, 45.6 with 3,
   // 47.2 with 4)
   const int depth = (int)std::min<int64_t>(kFwdRing, (224 * 1024 / kBlocks - 4096) / (row * RB));
   const int64_t grid = ring_grid(a.rows, RB, (int64_t)sms * kBlocks, EDGE);
   launch_dependent(kernel, dim3((unsigned)grid), ln_ring_block(TR), depth * row * RB, s, a, depth,
-                   status);
+                   timeouts);
   return MMN_OK;
 }
 
@@ -1259,7 +1259,7 @@ int ring_depth(int64_t cols, int64_t w, bool edge, int* smem) {
 }
 
 template <typename XT, typename DT, int TR, int NE, bool EDGE>
-int ring_launch(const LnBwd& a, int parts, int depth, int smem, int* status, int device,
+int ring_launch(const LnBwd& a, int parts, int depth, int smem, int* timeouts, int device,
                 cudaStream_t s) {
   constexpr int V = sizeof(XT) == 2 && sizeof(DT) == 2 ? 8 : 4;
   static std::mutex mu;
@@ -1267,14 +1267,14 @@ int ring_launch(const LnBwd& a, int parts, int depth, int smem, int* status, int
   auto* kernel = ln_bwd_ring_kernel<XT, DT, V, TR, NE, EDGE>;
   const int rc = raise_smem(kernel, device, mu, done);
   if (rc != MMN_OK) return rc;
-  launch_dependent(kernel, dim3(parts), ln_bwd_block(TR), smem, s, a, depth, status);
+  launch_dependent(kernel, dim3(parts), ln_bwd_block(TR), smem, s, a, depth, timeouts);
   return MMN_OK;
 }
 
 template <typename XT, typename DT, bool EDGE>
 int ring_bwd(const LnBwd& a, int64_t w, int parts, int depth, int smem, int device, cudaStream_t s) {
   int* st = nullptr;
-  const int rc = kernel_status_word(device, &st);
+  const int rc = kernel_timeout_word(device, &st);
   if (rc != MMN_OK) return rc;
   if constexpr (!EDGE) {
     if (w <= 256) return ring_launch<XT, DT, 32, 8, false>(a, parts, depth, smem, st, device, s);

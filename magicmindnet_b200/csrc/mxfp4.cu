@@ -19,6 +19,7 @@
 #include "mxfp4_gemm.cuh"
 
 #include <mutex>
+#include <vector>
 
 #include "capi_internal.cuh"
 #include "ns_engine.cuh"
@@ -701,7 +702,7 @@ int gemm_out(MxGemmArgs* g, void* out, int64_t ld, int dtype, int accumulate, in
   g->out_bf16 = dtype == MMN_DTYPE_BF16;
   g->accumulate = accumulate != 0;
   g->vec = vec_rows(out, ld, esize(dtype), 8);
-  return kernel_status_word(device, &g->status);
+  return kernel_timeout_word(device, &g->timeouts);
 }
 
 // out (a.rows x b.rows) = A B^T, on checked arguments. early_w: B was complete
@@ -915,14 +916,14 @@ extern "C" int mmn_kernel_status(int device, void* stream) {
   if ((rc = percall_device(device, &sms)) != MMN_OK) return rc;
   DeviceGuard guard(device);
   int* word = nullptr;
-  if ((rc = kernel_status_word(device, &word)) != MMN_OK) return rc;
+  if ((rc = kernel_timeout_word(device, &word)) != MMN_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int st = 0;
-  MMN_CUDA_TRY(cudaMemcpyAsync(&st, word, sizeof(int), cudaMemcpyDeviceToHost, s));
+  int count = 0;
+  MMN_CUDA_TRY(cudaMemcpyAsync(&count, word, sizeof(int), cudaMemcpyDeviceToHost, s));
   MMN_CUDA_TRY(cudaStreamSynchronize(s));
-  if (st == kDevOk) return MMN_OK;
-  MMN_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), s));
-  MMN_CUDA_TRY(cudaStreamSynchronize(s));
-  return fail(MMN_E_TIMEOUT,
-              "a kernel gave up a bounded wait (device status " + std::to_string(st) + ")");
+  static std::mutex mu;
+  static std::vector<int> reported;  // per device
+  std::lock_guard<std::mutex> lock(mu);
+  if (reported.size() <= (size_t)device) reported.resize((size_t)device + 1, 0);
+  return report_timeouts(count, &reported[(size_t)device]);
 }

@@ -31,7 +31,7 @@ struct MxGemmArgs {
   int vec;             // out and ld are aligned for 16-byte accesses
   int tma_out;         // the pair kernel stores through its tensor map
   int early_w;         // split kernel: the lanes' operand was complete before the previous kernel
-  int* status;
+  int* timeouts;       // counts waits that were given up
 };
 
 // -------------------------------------------------------- block conversions
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(320, 1)
     __syncthreads();
     cluster_sync_all();  // every rank has read this one's partial
   }
-  if (*abort_flag && threadIdx.x == 0) atomicExch(args.status, kDevWaitTimeout);
+  if (*abort_flag && threadIdx.x == 0) atomicAdd(args.timeouts, 1);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, S::kTmemCols);
@@ -892,7 +892,7 @@ __global__ void __launch_bounds__(MxPair<BN>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // peer loads landed, remote arrivals done, MMAs retired
-  if (*abort_flag && threadIdx.x == 0) atomicExch(args.status, kDevWaitTimeout);
+  if (*abort_flag && threadIdx.x == 0) atomicAdd(args.timeouts, 1);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);

@@ -150,6 +150,7 @@ def mxfp4_linear(x, w, out=None, out_dtype=None):
 
 def kernel_status(device: int = 0) -> None:
     """Waits for torch's current stream of the GPU and raises KernelTimeoutError
-    when a kernel of these operators on it gave up a bounded wait."""
+    when a kernel of these operators on it gave up a bounded wait since the last
+    such report. OptimizerStep.sync and .step_host raise it too, each step for itself."""
     _torch()
     N.check(N.lib().mmn_kernel_status(device, _stream(device)))

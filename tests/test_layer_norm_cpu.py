@@ -161,3 +161,10 @@ def test_rows_of_strided_tensors():
             _rows_view(bad, "t")
     with pytest.raises(ValueError):
         _rows_view(torch.zeros(()), "t")
+
+
+def test_layer_wait_selftest_arguments(N):
+    f = N.lib().mmn_selftest_layer_wait
+    assert f(0, 0, None) == N.MMN_E_INVALID and f(0, 2_000_000_001, None) == N.MMN_E_INVALID
+    if not N.lib().mmn_cuda_is_available():
+        assert f(0, 1000, None) == N.MMN_E_NO_DEVICE
