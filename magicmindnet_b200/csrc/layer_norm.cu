@@ -413,6 +413,19 @@ __device__ __forceinline__ void store_edge(T* row, int c, int cols, const f2* v)
 constexpr int kRingMax = 4;  // rows in flight per row group, at most (8 gained nothing)
 constexpr int kFwdRing = 2;  // ... in the forward kernel
 
+// A row group whose block has given up a wait: those of its `asked` rows that are still
+// on their way land, or run out of time too, before the block leaves its shared
+// memory to another. By the thread that issued them; it asks for no more rows once a
+// wait has given up (a slot whose row is still on its way must not be asked for another).
+__device__ __forceinline__ void ring_drain(uint64_t* bars, int asked, int depth) {
+#pragma unroll 1
+  for (int k = asked > depth ? asked - depth : 0; k < asked; ++k) {
+    const uint64_t start = global_timer_ns();
+    while (!mbar_try_wait(&bars[k % depth], (uint32_t)(k / depth) & 1u))
+      if (global_timer_ns() - start > kWaitLimitNs) break;
+  }
+}
+
 // The forward kernel for rows that can be read four elements at a time: TR threads
 // hold one row, NE columns each, a block a row (or a few short ones). Chunks of
 // four keep every access, the fp32 parameters' too, to whole consecutive lines
@@ -503,6 +516,7 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR, NE))
   __shared__ __align__(16) float red[2][RB][32];
   __shared__ __align__(8) uint64_t bars[RB][kRingMax];
   __shared__ volatile int abort_flag;
+  __shared__ int asked[RB];  // rows that each group has asked for in the end
   const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
   const int cols = (int)a.cols;
   const int rb = EDGE ? hull_bytes(cols, sizeof(XT)) : cols * (int)sizeof(XT);
@@ -536,8 +550,10 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR, NE))
   };
   griddep_wait();
   griddep_launch_dependents();
-  if (t == 0)
+  if (t == 0) {
     for (int k = 0; k < depth && k < mine; ++k) issue(k, k);
+    asked[sub] = mine;
+  }
   f2 ga[NE / 2], be[NE / 2];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
@@ -575,7 +591,12 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR, NE))
     const float mean = row_sum1<TR>(sum2(s), red[0][sub]) * inv_n;
     if constexpr (TR <= 32) __syncwarp();
     // every thread of the group has the row in registers: its slot is free
-    if (t == 0 && k + depth < mine) issue(k + depth, slot);
+    if (t == 0 && k + depth < mine) {
+      if (!abort_flag)
+        issue(k + depth, slot);
+      else
+        asked[sub] = min(asked[sub], k + depth);
+    }
     const f2 nm = dup2(-mean);
     f2 q = 0;
 #pragma unroll
@@ -613,7 +634,11 @@ __global__ void __launch_bounds__(ln_ring_block(TR), ln_ring_blocks(TR, NE))
       phase ^= 1u;
     }
   }
-  if (abort_flag && threadIdx.x == 0) atomicAdd(timeouts, 1);
+  if constexpr (TR <= 32) __syncthreads();  // the waits of every group are over
+  if (abort_flag) {
+    if (t == 0) ring_drain(bars[sub], asked[sub], depth);
+    if (threadIdx.x == 0) atomicAdd(timeouts, 1);
+  }
 }
 
 // ------------------------------------------------------------------ backward
@@ -751,6 +776,7 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
   __shared__ __align__(16) float2 red[2][32];
   __shared__ __align__(8) uint64_t bars[RB][kRingMax];
   __shared__ volatile int abort_flag;
+  __shared__ int asked[RB];  // rows that each group has asked for in the end
   const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
   const int cols = (int)a.cols;
   const int xb = EDGE ? hull_bytes(cols, sizeof(XT)) : cols * (int)sizeof(XT);
@@ -792,8 +818,10 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
   const int64_t first0 = (int64_t)blockIdx.x * RB;
   const int64_t trips = first0 < a.rows ? (a.rows - first0 + step - 1) / step : 0;
   griddep_wait();
-  if (t == 0)
+  if (t == 0) {
     for (int k = 0; k < depth && k < mine; ++k) issue(k, k);
+    asked[sub] = (int)mine;
+  }
   f2 ga[kReread ? 1 : NE / 2];
   if constexpr (kReread) {
     for (int k = threadIdx.x; k < gb / 4; k += kBlock) {
@@ -874,7 +902,12 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
     }
     const float2 s = ring_sum2<TR>(sum2(s1), sum2(s2), red[k & 1]);
     // every thread of the group is past the previous row: its slot is free
-    if (t == 0 && k > 0 && k - 1 + depth < mine) issue(k - 1 + depth, prev);
+    if (t == 0 && k > 0 && k - 1 + depth < mine) {
+      if (!abort_flag)
+        issue(k - 1 + depth, prev);
+      else
+        asked[sub] = min(asked[sub], (int)k - 1 + depth);
+    }
     const f2 c1 = dup2(-s.x * inv_n), c2 = dup2(-s.y * inv_n);
     if (ok) {
       XT* dx = static_cast<XT*>(a.dx) + row * a.dx_ld;
@@ -911,7 +944,11 @@ __global__ void __launch_bounds__(ln_bwd_block(TR), ln_bwd_min_blocks(TR))
     }
   }
   griddep_launch_dependents();  // ln_bwd_sum_kernel may take its place; it waits for the sums
-  if (abort_flag && threadIdx.x == 0) atomicAdd(timeouts, 1);
+  if constexpr (TR <= 32) __syncthreads();  // the waits of every group are over
+  if (abort_flag) {
+    if (t == 0) ring_drain(bars[sub], asked[sub], depth);
+    if (threadIdx.x == 0) atomicAdd(timeouts, 1);
+  }
   float* out = a.partial + (int64_t)blockIdx.x * 2 * a.cols;
   if constexpr (RB == 1) {
 #pragma unroll
