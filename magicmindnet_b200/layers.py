@@ -115,8 +115,10 @@ class Linear(_Layer):
         if tuple(dy.shape) != want:
             raise N.ShapeError(N.MMN_E_SHAPE, f"dy is {tuple(dy.shape)}, expected {want}")
         dyq, dyt = mxfp4_quantize(_as_matrix(dy), "both")
-        mxfp4_matmul(dyt, xt, out=self._grad, accumulate=accumulate)
+        # dx first: its room may be missing, and a backward pass that failed leaves the
+        # slot as it was, so that it can be called again
         dx = mxfp4_matmul(dyq, self.wt, out_dtype=dtype)
+        mxfp4_matmul(dyt, xt, out=self._grad, accumulate=accumulate)
         self._saved = None
         return dx.view(shape)
 

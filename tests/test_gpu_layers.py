@@ -256,3 +256,34 @@ def test_two_graphs_at_once(mmn):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
     mmn.kernel_status()
+
+
+def test_backward_that_failed_can_be_called_again(mmn, monkeypatch):
+    """No room for dx: the grad slot keeps what it held, and the second call adds the
+    weight's gradient once."""
+    import torch
+
+    from magicmindnet_b200 import layers
+
+    step = make_step(mmn)
+    lin = mmn.Linear(step, 1)
+    x, dy = data(TOKENS, D, "bf16", 1, 0.3), data(TOKENS, FFN, "bf16", 2, 0.3)
+    base = torch.randn(FFN, D, device="cuda")
+    step.grad(1).copy_(base)
+    lin.forward(x)
+    real = layers.mxfp4_matmul
+
+    def no_room(a, b, out=None, **kw):
+        if out is None:
+            raise torch.cuda.OutOfMemoryError("no room for dx")
+        return real(a, b, out=out, **kw)
+
+    monkeypatch.setattr(layers, "mxfp4_matmul", no_room)
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        lin.backward(dy, accumulate=True)
+    monkeypatch.undo()
+    assert torch.equal(step.grad(1), base)
+    dx = lin.backward(dy, accumulate=True)
+    check_product(step.grad(1), plain_values(dy.t()), plain_values(x.t()), base)
+    check_product(dx, plain_values(dy), plain_values(step.param(1).t()))
+    step.close()
