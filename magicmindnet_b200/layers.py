@@ -76,7 +76,9 @@ class Linear(_Layer):
     """y = x W^T with W [out, in] in `slot`. The forward pass and both gradient
     products run on 4-bit operands; the weight's 4-bit copies (W for the forward
     pass, W transposed for the input's gradient) are made by ``refresh``, which
-    is called once here and again after every ``OptimizerStep.step``."""
+    is called once here and again after every ``OptimizerStep.step``,
+    ``step_host`` or ``set_param``: ``forward`` refuses copies that are older. (What
+    is written straight into an ``OptimizerStep.param`` view it cannot see.)"""
 
     def __init__(self, step, slot: int):
         shape = step.shapes[slot]
@@ -94,10 +96,15 @@ class Linear(_Layer):
     def refresh(self) -> None:
         """Both 4-bit copies from the slot's present values, in place (one read). On
         several ranks: after the fence that ends the step's parameter exchange."""
+        version = self.step.param_version
         mxfp4_quantize(self._param, "both", out=(self.w, self.wt))
+        self._version = version
 
     def forward(self, x, training: bool = True, out_dtype=None):
         """x [..., in] -> [..., out]; training=False keeps nothing for backward."""
+        if self._version != self.step.param_version:
+            raise N.MmnError(N.MMN_E_STATE, "the parameters have changed since the weight's 4-bit "
+                                            "copies were made (refresh() renews them)")
         if not training:
             return mxfp4_linear(x, self.w, out_dtype=out_dtype)
         if x.shape[-1] != self.w.shape[1]:

@@ -159,6 +159,10 @@ class OptimizerStep:
             N.check(N.lib().mmn_optim_slot_owner(h, i, ctypes.byref(owner)))
             self.routes.append("muon" if owner.value >= 0 else "adamw")
         self._views = {}
+        #: grows with every call that may change the parameters (set_param, step,
+        #: step_host); what is derived from them, as Linear's 4-bit copies are, keeps
+        #: the value that it was made at
+        self.param_version = 0
 
     # -- buffers -----------------------------------------------------------------
     def _ptrs(self, slot: int):
@@ -193,6 +197,7 @@ class OptimizerStep:
 
     def set_param(self, slot: int, values: np.ndarray) -> None:
         v = np.ascontiguousarray(values, np.float32)
+        self.param_version += 1
         N.check(N.lib().mmn_optim_set_param(
             self._h, slot, _host_ptr(v, self._numel(slot), 4, "param", slot), N.MEM_HOST))
 
@@ -249,6 +254,7 @@ class OptimizerStep:
 
     # -- stepping ------------------------------------------------------------------
     def step(self, grad_divisor: float = 1.0) -> None:
+        self.param_version += 1
         N.check(N.lib().mmn_optim_step(self._h, grad_divisor))
 
     def step_host(self, grads, params, grad_divisor: float = 1.0) -> None:
@@ -266,6 +272,7 @@ class OptimizerStep:
             numel = int(np.prod(self.shapes[k], dtype=np.int64))
             gp[k] = _host_ptr(grads[k], numel, gsz, "grad", k)
             pp[k] = _host_ptr(params[k], numel, 4, "param", k, writable=True)
+        self.param_version += 1
         N.check(N.lib().mmn_optim_step_host(self._h, gp, pp, grad_divisor))
 
     def sync(self) -> None:

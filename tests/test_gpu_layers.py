@@ -287,3 +287,39 @@ def test_backward_that_failed_can_be_called_again(mmn, monkeypatch):
     check_product(step.grad(1), plain_values(dy.t()), plain_values(x.t()), base)
     check_product(dx, plain_values(dy), plain_values(step.param(1).t()))
     step.close()
+
+
+def test_linear_refuses_copies_older_than_the_weight(mmn):
+    """After anything that changes the parameters, until refresh. A forward pass that
+    came before still gets its backward pass."""
+    import numpy as np
+    import torch
+
+    step = make_step(mmn)
+    lin, other = mmn.Linear(step, 1), mmn.Linear(step, 0)
+    x, dy = data(TOKENS, D, "bf16", 1, 0.3), data(TOKENS, FFN, "bf16", 2, 0.3)
+    n = len(NAMES)
+    for k in range(n):
+        step.grad(k).normal_()
+    changes = (step.step, lambda: step.step_host([None] * n, [None] * n),
+               lambda: step.set_param(1, np.full((FFN, D), 0.25, np.float32)))
+    for change in changes:
+        lin.forward(x)
+        change()
+        step.sync()
+        lin.backward(dy)
+        for training in (True, False):
+            with pytest.raises(mmn.MmnError, match="refresh"):
+                lin.forward(x, training=training)
+        with pytest.raises(mmn.MmnError, match="refresh"):
+            other.forward(data(3, FFN, "bf16", 3), training=False)
+        lin.refresh()
+        other.refresh()
+        y = lin.forward(x, training=False)
+        check_product(y, plain_values(x), plain_values(step.param(1)))
+    assert torch.equal(step.param(1), torch.full((FFN, D), 0.25, device="cuda"))
+    step.sync()  # nothing here changes a parameter
+    step.set_grad(1, np.zeros((FFN, D), np.float32))
+    step.get_param(1)
+    lin.forward(x, training=False)
+    step.close()
