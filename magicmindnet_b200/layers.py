@@ -10,8 +10,8 @@ gradient and writes the weights' gradients into the step's grad slots, where
 at a time: the next one before its ``backward`` (or ``discard``) is refused.
 ``training=False`` holds nothing. Work is enqueued on torch's current stream,
 which must be the one the step was made on (or ordered with it), as for
-``OptimizerStep.param`` and ``.grad`` views; like those, a layer is of no use
-after the step is closed.
+``OptimizerStep.param`` and ``.grad`` views. After the step is closed a layer
+refuses its calls: the slots are gone.
 """
 from __future__ import annotations
 
@@ -24,6 +24,10 @@ class _Layer:
     """What a forward pass leaves for its backward pass."""
 
     _saved = None
+
+    def _open(self) -> None:
+        if not self.step._h:
+            raise N.MmnError(N.MMN_E_STATE, "the step is closed, its slots are gone")
 
     def _hold(self, saved) -> None:
         self._saved = saved
@@ -57,6 +61,7 @@ class LayerNorm(_Layer):
     def forward(self, x, training: bool = True, out_dtype=None):
         """The norm of x [..., d]; x itself is kept for backward and must not change
         before it."""
+        self._open()
         if training:
             self._free()
         y, mean, rstd = layer_norm(x, self._gamma, self._beta, self.eps, out_dtype)
@@ -65,6 +70,7 @@ class LayerNorm(_Layer):
         return y
 
     def backward(self, dy, accumulate: bool = False):
+        self._open()
         x, mean, rstd = self._held()
         dx, _, _ = layer_norm_backward(dy, x, self._gamma, mean, rstd, self._dgamma, self._dbeta,
                                        accumulate)
@@ -96,12 +102,14 @@ class Linear(_Layer):
     def refresh(self) -> None:
         """Both 4-bit copies from the slot's present values, in place (one read). On
         several ranks: after the fence that ends the step's parameter exchange."""
+        self._open()
         version = self.step.param_version
         mxfp4_quantize(self._param, "both", out=(self.w, self.wt))
         self._version = version
 
     def forward(self, x, training: bool = True, out_dtype=None):
         """x [..., in] -> [..., out]; training=False keeps nothing for backward."""
+        self._open()
         if self._version != self.step.param_version:
             raise N.MmnError(N.MMN_E_STATE, "the parameters have changed since the weight's 4-bit "
                                             "copies were made (refresh() renews them)")
@@ -117,6 +125,7 @@ class Linear(_Layer):
         return y.view(tuple(x.shape[:-1]) + (self.w.shape[0],))
 
     def backward(self, dy, accumulate: bool = False):
+        self._open()
         xt, dtype, shape = self._held()
         want = tuple(shape[:-1]) + (self.w.shape[0],)
         if tuple(dy.shape) != want:

@@ -323,3 +323,19 @@ def test_linear_refuses_copies_older_than_the_weight(mmn):
     step.get_param(1)
     lin.forward(x, training=False)
     step.close()
+
+
+def test_layers_of_a_closed_step_refuse(mmn):
+    step = make_step(mmn)
+    lin, ln = mmn.Linear(step, 1), mmn.LayerNorm(step, 2, 3)
+    x = data(TOKENS, D, "bf16", 1, 0.3)
+    dy = [lin.forward(x), ln.forward(x)]
+    step.close()
+    for layer, g in zip((lin, ln), dy):
+        layer_calls = [lambda: layer.forward(x), lambda: layer.forward(x, training=False),
+                       lambda: layer.backward(g)]
+        for call in layer_calls + ([lin.refresh] if layer is lin else []):
+            with pytest.raises(mmn.MmnError, match="closed"):
+                call()
+    with pytest.raises(mmn.MmnError):
+        mmn.Linear(step, 1)
