@@ -434,3 +434,32 @@ def test_refusals(mmn):
         torch.zeros_like(x).data_ptr(), 8, big.data_ptr(), ws.data_ptr(), 0, 0, big.data_ptr(),
         big.numel() * 4, 0, None)
     assert rc == N.MMN_E_INVALID  # the workspace is also dgamma
+
+
+# Dense aligned rows, enough that every row group of the walking kernels takes several
+# and goes round its ring: each width class of the forward kernel (32 threads a row in
+# both depths, 64, 128, 256, 512) and of the backward one (32, 64, 128, 256, 512), few more
+# rows than the forward's threshold, and counts that divide into no grid.
+@pytest.mark.parametrize("xd,yd", list(itertools.product(("f32", "bf16"), repeat=2)))
+@pytest.mark.parametrize("cols,rows", [(72, 1185), (72, 20011), (256, 12007), (384, 1185),
+                                       (384, 12007), (768, 1185), (768, 5003), (1024, 2500),
+                                       (1024, 12007), (2048, 1185), (2048, 2500), (2048, 5003),
+                                       (4096, 1185), (4096, 5003), (8192, 1185), (8192, 2500),
+                                       (16384, 1187)])
+def test_many_aligned_rows(mmn, cols, rows, xd, yd):
+    x, gamma, beta, dy = make(rows, cols, xd, yd, seed=rows + cols)
+    y, mean, rstd = mmn.layer_norm(x, gamma, beta, 1e-5, out_dtype=dy.dtype)
+    check_forward(y, mean, rstd, x, gamma, beta, 1e-5)
+    dx, dgamma, dbeta = mmn.layer_norm_backward(dy, x, gamma, mean, rstd)
+    check_backward(dx, dgamma, dbeta, dy, x, gamma, mean, rstd)
+    # in place too: a row is read before its place is written
+    z = x.clone() if x.dtype == y.dtype else None
+    if z is not None:
+        mmn.layer_norm(z, gamma, beta, 1e-5, out=z)
+        check_forward(z, mean, rstd, x, gamma, beta, 1e-5)
+    base = (dgamma.clone(), dbeta.clone())
+    args = [dy.clone(), x]
+    out = args[0] if dy.dtype == x.dtype else None
+    dx, _, _ = mmn.layer_norm_backward(*args, gamma, mean, rstd, dgamma, dbeta, accumulate=True,
+                                       out=out)
+    check_backward(dx, dgamma, dbeta, dy, x, gamma, mean, rstd, base)
