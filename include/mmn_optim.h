@@ -526,7 +526,9 @@ int mmn_mxfp4_dequantize(const mmn_mxfp4 *q, void *out, int64_t out_ld, int dtyp
 
 /* out (a.rows x b.rows, fp32 or bf16) = A B^T, summed over the cols of both in
  * fp32 on the tensor cores and rounded once; accumulate = 1 adds it to what out
- * holds first (fp32 values below 2^-126 may count as zero there). With W of a Linear layer ([out, in], crates/mmn-nn/src/lib.rs:305-307):
+ * holds first. An fp32 addition may be done by the memory, which takes what the
+ * product or out has below 2^-126 for zero; bf16 ones, and fp32 ones with few rows,
+ * keep it. With W of a Linear layer ([out, in], crates/mmn-nn/src/lib.rs:305-307):
  * y = x W^T from (x, W); dx = dy W from (dy, W transposed); dW = dy^T x from (dy
  * transposed, x transposed), for example into a grad slot. A NaN block makes
  * the rows (columns) of out that sum over it NaN. */

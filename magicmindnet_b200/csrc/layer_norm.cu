@@ -9,31 +9,37 @@
 //   dgamma = sum over rows of dy h, dbeta = sum over rows of dy
 //
 // Bound by memory: a row is read once, into registers or shared memory, the
-// squares are summed about the mean there (so that a row whose mean is large
-// against its spread loses nothing), and the row is written once. All statistics
-// and sums are fp32; y and dx are rounded once.
+// squares are summed about the mean there (so that the variance of a row whose mean
+// is large against its spread does not cancel), and the row is written once. All
+// statistics and sums are fp32; y and dx are rounded once. The mean is an fp32 sum,
+// and (x - mean) r carries its error: 2^-24 |mean| / sigma at least, with the sum's
+// own up to some 2^-24 times the additions an element passes through (32 in a
+// thread, 10 across) times mean|x| / sigma.
 //
-// Which kernel takes a call (measured on one B200, fractions of the 6.53 TB/s a
-// copy reaches):
+// Which kernel takes a call (measured on one B200 with operands that are not in L2,
+// fractions of the 6.53 TB/s a copy reaches):
 //   forward   ln_fwd_ring_kernel  bf16 rows, many and aligned: 16384 x 4096 in
-//                                 43.2 us (0.95), 70.6 us a row per block; rows that
-//                                 start anywhere, beyond 1024 columns: 16384 x 4057
-//                                 63.2 us (0.64), fp32 96.5 (0.84)
+//                                 44.0 us (0.93), 1.28 times as long with a row per
+//                                 block; rows that start anywhere, beyond 1024 columns:
+//                                 16384 x 4057 65.0 us (0.63), fp32 96.3 (0.85)
 //             ln_fwd_rows_kernel  the rest of the rows that can be read four at a
-//                                 time: 16384 x 2048 fp32 to bf16 in 31.6 us (0.97)
+//                                 time: 16384 x 2048 fp32 to bf16 in 34.5 us (0.89)
 //             ln_fwd_kernel       an element at a time, where x and y start differently
-//                                 and for fewer columns: 3001 x 1013 fp32 in 6.7
-//                                 us (0.55), 16384 x 4057 bf16 132 (0.31)
+//                                 and for fewer columns: 3001 x 1013 fp32 in 11.1
+//                                 us (0.34; 6.8 from L2), 16384 x 4057 bf16 132 (0.31)
 //             ln_fwd_wide_kernel  rows beyond 16384
-//   backward  ln_bwd_ring_kernel  aligned rows of 65 to 16384: 16384 x 4096 bf16 in
-//                                 72.9 us (0.85) with the closing sums, 113 us with
-//                                 the rows loaded into registers; rows that start
-//                                 anywhere, beyond 512 columns: 16384 x 4057 106 us
-//                                 (0.57), fp32 141 (0.86)
+//   backward  ln_bwd_ring_kernel  aligned rows of 65 columns to where two rows of x and
+//                                 dy (and beyond 8192 columns gamma) no longer fit one SM's
+//                                 shared memory: 16384 in bf16, 14080 in mixed types,
+//                                 11264 in fp32. 16384 x 4096 bf16 in 75.7 us (0.81) with
+//                                 the closing sums, 113 us with the rows loaded into
+//                                 registers; rows that start anywhere, beyond 512 columns:
+//                                 16384 x 4057 107 us (0.57), fp32 143 (0.85)
 //             ln_bwd_kernel       narrow rows, and an element at a time up to 8192
-//                                 columns: 3001 x 1013 fp32 15.8 us (12.8 by vectors),
+//                                 columns: 3001 x 1013 fp32 15.8 us (12.9 by vectors),
 //                                 16384 x 4057 bf16 158
-//             ln_bwd_wide_*       the rest
+//             ln_bwd_wide_*       the rest: 4096 x 11272 fp32 204 us (11264: 118),
+//                                 16384 320
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -430,9 +436,9 @@ __device__ __forceinline__ void ring_drain(uint64_t* bars, int asked, int depth)
 // hold one row, NE columns each, a block a row (or a few short ones). Chunks of
 // four keep every access, the fp32 parameters' too, to whole consecutive lines
 // per warp. A block lives 2 to 3 us, most of it waiting, so what is in flight is
-// what the blocks on the GPU hold: enough for fp32 rows (16384 x 4096 in 79.3
-// us, 6.77 TB/s; 86 us with a third fewer blocks an SM) and not for bf16 ones (64
-// us, 4.2 TB/s; ln_fwd_ring_kernel).
+// what the blocks on the GPU hold: enough for fp32 rows (16384 x 4096 in 80.9
+// us, 6.6 TB/s; 86 us with a third fewer blocks an SM) and not for bf16 ones (54.8 us
+// on one set of operands, where ln_fwd_ring_kernel takes 42.9).
 __host__ __device__ constexpr int ln_rows_block(int tr) { return tr <= 32 ? 128 : tr; }
 
 template <typename XT, typename YT, int TR, int NE>
@@ -1204,11 +1210,13 @@ int fwd_types(const LnFwd& a, bool vec, bool vec8, bool alike, int sms, int devi
   if constexpr (sizeof(XT) == 2)
     if (vec8 && a.cols > 64 && a.cols <= kFwdMaxCols && a.rows >= 8 * (int64_t)sms)
       return ring_whole<XT, YT>(a, sms, device, s);
-  // Rows that start anywhere: vectors with care at the ends, or an element at a time.
-  // 16384 x 4057 63.2 us and 132, fp32 96.9 and 115; 20000 x 2037 44.7 and 79.0, fp32 61.8
-  // and 68.0; 8 x 4001 2.9 and 5.4. Up to 1024 columns the ends outweigh the rest
-  // (3001 x 1013 fp32 8.1 and 6.7 us), and so they do for fp32 rows that the start pushes
-  // into the next class (16384 x 4095 124 and 116; bf16 100 and 132).
+  // Rows that start anywhere: vectors with care at the ends, or an element at a time
+  // (launches one behind the other). 16384 x 4057 63.4 us and 132, fp32 95.1 and 115; 20000 x
+  // 2037 44.8 and 79.0, fp32 60.5 and 68.0; 8 x 4001 2.8 and 5.4. Up to 1024 columns the
+  // ends outweigh the rest (32768 x 1013 59.9 and 51.5, fp32 63.9 and 49.8; 16384 x 777 32.2
+  // and 22.1, fp32 33.7 and 22.6; 1200 x 1013 6.2 and 4.0; 300 x 600 equal), and so they do
+  // for fp32 rows that the start pushes into the next class (16384 x 4095 124 and 116; bf16
+  // 102 and 132).
   if (const int64_t w = a.cols + (sizeof(XT) == 2 && sizeof(YT) == 2 ? 7 : 3);
       alike && !vec && a.cols > 1024 && w <= kFwdMaxCols) {
     int64_t cls = 2048;
@@ -1332,7 +1340,7 @@ int bwd_types(const LnBwd& a, int* parts, bool vec, bool ring, bool alike, int s
   constexpr int V = sizeof(XT) == 2 && sizeof(DT) == 2 ? 8 : 4;
   const int64_t w = a.cols + (ring ? 0 : V - 1);  // ... and what an uneven start may add
   // Rows that start anywhere: vectors with care at the ends, or an element at a time.
-  // 16384 x 4057 106 us and 158, fp32 141 and 184; 32768 x 1013 74.6 and 109, fp32 67.4 and
+  // 16384 x 4057 106 us and 158, fp32 140 and 184; 32768 x 1013 75.6 and 109, fp32 69.9 and
   // 118. Element-wise where the start pushes the row into the next class (16384 x 4095
   // 205 and 158), for few columns (32768 x 501 47.9 and 36.9) and few bf16 rows (600 x
   // 1013 13.8 and 9.6; fp32 8.7 and 10.1).

@@ -96,8 +96,9 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes
 // blocks of 32 along the rows, then down the columns, whose bytes are collected
 // in shared memory so that global memory sees 64 consecutive bytes per row of
 // codes. A tile gives exactly one 512-byte block of scales in each direction.
-// 8192 x 4096 bf16: rows 15.8 us, columns 15.8, both 21.7 (0.82, 0.82 and 0.73 of
-// a copy's rate); 16384 x 8192: 52, 53 and 74 us (1.0, 0.98, 0.85). With few waves
+// Operands not in L2: 8192 x 4096 bf16 rows 16.1 us, columns 16.2, both 21.7 (0.81, 0.80
+// and 0.73 of a copy's rate); 16384 x 8192 52, 54 and 73 us (1.0, 0.96, 0.87); 14336 x 4096
+// fp32, a weight's copies after a step, 44, 45 and 57 us (0.93, 0.91, 0.80). With few waves
 // of blocks their loads and their work fall together; within a block "both" is 14
 // instructions an element (issue slots 69% busy, the shared-memory pipe 62%).
 template <typename T, bool SHIFT>
@@ -146,9 +147,12 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
   } else {
     // Rows that start anywhere arrive in whole vectors, one more a row. bf16 moves to
     // its place within shared memory (44 to 45 us moved as it is read), fp32 as it is
-    // read (73 to 75 moved before). 16384 x 4095 bf16 43 us, fp32 69 along the rows and
-    // 64 along the columns (80 and 128 with an element a load; 55 and 123 with the
+    // read (73 to 75 moved before). 16384 x 4095 bf16 43 us, fp32 68 along the rows and
+    // 65 along the columns (80 and 128 with an element a load; 55 and 123 with the
     // vectors moved on their way to shared memory, which leaves fewer loads in flight).
+    // Aligned rows take 26 and 48 us: the move is a second pass over shared memory whose
+    // instructions count (the shared-memory pipe 67% busy, an instruction issued in 64% of
+    // the cycles, DRAM 41%); an uneven row of a tile touches 9 sectors for 8.
     auto copy = [&](int r, int j) {
       const T* row = x + (int64_t)(r0 + r) * a.ld + c0;
       const int c = j * kPer - offset(r);  // the vector's first column
@@ -333,12 +337,13 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
 // 32 rows x 512 (bf16) or 256 (fp32) columns per block. A lane turns the codes of 32
 // output bytes into one store, so that every sector is written whole; the loads of
 // a lane's rows are issued first, without branches between them (what lies outside
-// is read from the edge and not used). 16384 x 4096: 27.4 us to bf16, 48.6 to fp32
-// (0.95 and 0.96 of a copy's rate; 29.8 and 49.0 with 16-byte stores).
+// is read from the edge and not used). 16384 x 4096: 28.1 us to bf16, 48.8 to fp32
+// (0.93 and 0.95 of a copy's rate; 29.8 and 49.0 with 16-byte stores).
 // SHIFT: output rows that start anywhere. A lane's columns begin where the row's
 // memory is aligned, o columns before its codes; the codes are moved by o nibbles,
-// and the first o values may belong to the block before. 16384 x 4095: 38.9 and
-// 49.5 us (187 and 89 with an element a store).
+// and the first o values may belong to the block before. 16384 x 4095: 39.5 and
+// 50.3 us (187 and 89 with an element a store); bf16 is bound by instructions (issued
+// in 75% of the cycles), the moving and the second scale's selection among them.
 template <typename T, bool SHIFT>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const MxDequantArgs a) {
   constexpr int V = 32 / sizeof(T), W = V / 8, NR = 4;
@@ -642,8 +647,12 @@ int launch_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int pairs
   if (err.empty()) err = encode_byte_rows(&tb, b->codes, code_pitch(b->cols), b->rows, BN / 2);
   if (err.empty()) err = encode_scale_runs(&tsa, a->scales, runs, (a->rows + 127) / 128, 1);
   if (err.empty()) err = encode_scale_runs(&tsb, b->scales, runs, (b->rows + 127) / 128, 2);
-  // Stores and fp32 additions go through the tensor map where the rows are aligned
-  // (TMA additions flush values below 2^-126 to zero). bf16 values are added in
+  // Stores and fp32 additions go through the tensor map where the rows are aligned.
+  // Additions in memory, TMA's and mx_store_block's, flush values below 2^-126 to zero,
+  // which the header says; loads, additions in registers and stores keep them and
+  // were measured: 4096 x 14336 x 4096 164 us against 139, 8192 x 2048 x 4096 55 against
+  // 44, and with rows that start anywhere 4096 x 14335 x 4095 232 against 156, 2048 x
+  // 4097 x 4096 68 against 30. bf16 values are added in
   // the epilogue's registers: a TMA addition would round the product to bf16
   // before the sum.
   g.tma_out = g.vec && !(g.out_bf16 && g.accumulate);

@@ -93,9 +93,9 @@ __device__ __forceinline__ uint4 mx_block(const float (&w)[32], uint32_t* scale)
 // stages are on their way: a token costs one launch, and no scratch. BN below 128
 // takes one tile of A's rows (its scales then start at a block's first row).
 //
-// Bound by latency at these sizes: 1 x 8192 x 2048 takes 5.2 us (rounded in the
-// kernel: 5.8) where its bytes take 1.4, 48 x 4096 x 4096 6.5 us (1.5), 16 x 14336 x
-// 4096 9.5 us (4.9), 333 x 517 x 1030 6.9 us.
+// Bound by latency at these sizes (operands not in L2): 1 x 8192 x 2048 takes 6.8 us
+// (rounded in the kernel: 7.1) where its bytes take 1.4, 48 x 4096 x 4096 8.4 us (1.5),
+// 16 x 14336 x 4096 10.8 us (rounded in the kernel: 12.6; 4.9), 333 x 517 x 1030 8 us.
 template <int BN, int SRC>
 struct MxSplit {
   static constexpr int kABytes = 128 * 128;
@@ -449,9 +449,9 @@ __global__ void __launch_bounds__(320, 1)
 
 // Writes (or adds) a 32 x 32 block held one row per lane (v[j] = column j) to
 // out rows r0.., columns c0.., through the warp's 32 x 33 stage: what cannot go by TMA,
-// rows that are not aligned and sums of bf16. 4096 x 14335 x 4095: 118 us bf16, 140
-// fp32 (14336: 101 and 118 by TMA; 136 with a bf16 element a lane and a store); added
-// to, 175 and 152 (292 and 366 with loads of eight rows before their stores); 14336
+// rows that are not aligned and sums of bf16. 4096 x 14335 x 4095: 119 us bf16, 134
+// fp32 (14336: 101 and 117 by TMA; 136 with a bf16 element a lane and a store); added
+// to, 176 and 145 (292 and 366 with loads of eight rows before their stores); 14336
 // bf16, added to, 125 (161 with a load and a store at a time).
 __device__ __forceinline__ void mx_store_block(const MxGemmArgs& a, long long r0, long long c0,
                                                int rows, int cols, const float (&v)[32],
