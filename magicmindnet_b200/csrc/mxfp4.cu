@@ -647,7 +647,9 @@ int launch_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int pairs
   if (err.empty()) err = encode_byte_rows(&tb, b->codes, code_pitch(b->cols), b->rows, BN / 2);
   if (err.empty()) err = encode_scale_runs(&tsa, a->scales, runs, (a->rows + 127) / 128, 1);
   if (err.empty()) err = encode_scale_runs(&tsb, b->scales, runs, (b->rows + 127) / 128, 2);
-  // Stores and fp32 additions go through the tensor map where the rows are aligned.
+  // Stores and fp32 additions go through the tensor map where the rows are aligned and
+  // end on 16 bytes: TMA clips a store at the matrix's edge in steps of 16 bytes, so it
+  // would write up to 15 bytes behind a row that ends inside one.
   // Additions in memory, TMA's and mx_store_block's, flush values below 2^-126 to zero,
   // which the header says; loads, additions in registers and stores keep them and
   // were measured: 4096 x 14336 x 4096 164 us against 139, 8192 x 2048 x 4096 55 against
@@ -655,11 +657,12 @@ int launch_pair(const mmn_mxfp4* a, const mmn_mxfp4* b, MxGemmArgs& g, int pairs
   // 4097 x 4096 68 against 30. bf16 values are added in
   // the epilogue's registers: a TMA addition would round the product to bf16
   // before the sum.
-  g.tma_out = g.vec && !(g.out_bf16 && g.accumulate);
+  const int esz = g.out_bf16 ? 2 : 4;
+  g.tma_out = g.vec && b->rows * esz % 16 == 0 && !(g.out_bf16 && g.accumulate);
   if (!g.tma_out)
     to = ta;
   else if (err.empty())
-    err = encode_store_rows(&to, g.out, a->rows, b->rows, g.ld, g.out_bf16 ? 2 : 4);
+    err = encode_store_rows(&to, g.out, a->rows, b->rows, g.ld, esz);
   if (!err.empty()) return fail(MMN_E_CUDA, err);
   g.M = (int)a->rows;
   g.N = (int)b->rows;

@@ -29,7 +29,7 @@ struct MxGemmArgs {
   int out_bf16;
   int accumulate;
   int vec;             // out and ld are aligned for 16-byte accesses
-  int tma_out;         // the pair kernel stores through its tensor map
+  int tma_out;         // the pair kernel stores through its tensor map (rows end on 16 bytes)
   int early_w;         // split kernel: the lanes' operand was complete before the previous kernel
   int* timeouts;       // counts waits that were given up
 };
@@ -606,7 +606,8 @@ __device__ __forceinline__ void mx_tile(int tile, int tiles_m, int tiles_n, int&
 // of 64 bytes (all 32 columns in bf16, 16 of fp32) are staged with the 64-byte
 // swizzle (conflict-free 16-byte stores) in two buffers that alternate, so a
 // store is read out of shared memory while the next is filled. Clipped at the
-// matrix edge by the tensor map. ADD (fp32): added to what out holds.
+// matrix edge by the tensor map, whose rows end on 16 bytes. `add` (fp32): added to
+// what out holds.
 template <bool BF16>
 __device__ __forceinline__ void mx_store_tma(const CUtensorMap* map, uint8_t* stage, int c0, int r0,
                                              bool add, const float (&v)[32], int& buf) {

@@ -97,7 +97,8 @@ std::string encode_scale_runs(CUtensorMap* map, const void* base, int64_t pairs,
 
 // Tensor map for TMA stores of 32-row x 64-byte boxes (64-byte swizzle) into a
 // rows x cols matrix of bf16 (esize 2) or fp32 (esize 4), pitch ld elements;
-// base and pitch are multiples of 16 bytes.
+// base, pitch and row length are multiples of 16 bytes (a store is clipped at the
+// row's end in steps of that).
 std::string encode_store_rows(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int64_t ld,
                               int esize);
 

@@ -505,3 +505,31 @@ def test_refusals(mmn):
     c = N.Mxfp4C(q._c.codes, h.data_ptr() // 16 * 16, 4, 64)
     assert N.lib().mmn_mxfp4_matmul(ctypes.byref(c), ctypes.byref(q._c), x.data_ptr(), 4, 0, 0, 0,
                                     None) == N.MMN_E_INVALID
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("m,n,k", [(700, 1111, 512), (2304, 2049, 64), (2465, 939, 300), (300, 2050, 96),
+                                   (90, 1111, 64), (1030, 1036, 64)])
+def test_aligned_rows_that_end_anywhere_leave_their_neighbours(mmn, m, n, k, accumulate, out):
+    """Rows that start on 16 bytes and end inside 16: what follows each, the last one
+    too, stays bit for bit (NaN and subnormal patterns among it)."""
+    import torch
+
+    a, b = data(m, k, "f32", 1, 1.0), data(n, k, "f32", 2, 1.0)
+    qa, qb = mmn.mxfp4_quantize(a), mmn.mxfp4_quantize(b)
+    bits = {"f32": torch.int32, "bf16": torch.int16}[out]
+    for pad in (8 - n % 8, 16 - n % 8):
+        ld = n + pad
+        for off in (0, 8):
+            buf = torch.randint(-2 ** 15, 2 ** 15, (off + m * ld + 8,), device="cuda").to(bits)
+            raw = buf.clone()
+            # numbers in the slice itself
+            view = buf.view(T(out))[off:off + m * ld].view(m, ld)[:, :n]
+            view.copy_(torch.randn(m, n, device="cuda"))
+            base = view.clone()
+            mmn.mxfp4_matmul(qa, qb, out=view, accumulate=accumulate)
+            check_product(view, plain_values(a), plain_values(b), base if accumulate else None)
+            outside = torch.ones_like(buf, dtype=torch.bool)
+            outside[off:off + m * ld].view(m, ld)[:, :n] = False
+            assert torch.equal(buf[outside], raw[outside]), (pad, off)
